@@ -22,6 +22,14 @@ KVCOPY_FLAG_BULK = 0x1
 KVCOPY_FLAG_TEST_STALL = 0x100
 KVCOPY_PATH_REGISTER, KVCOPY_PATH_BULK, KVCOPY_PATH_BULK_HND = 1, 2, 3
 KVHASH_MAX_BLOCK_SIZE = 8192
+KVPAGE_ERR_PAGE = 0x1
+KVPAGE_ERR_ROW = 0x2
+KVPAGE_ERR_REFS = 0x4
+KVPAGE_ERR_KEEP = 0x8
+KVPAGE_ERR_ALIGN = 0x10
+KVPAGE_OK, KVPAGE_NO_PAGES, KVPAGE_INVALID = 0, 1, 2
+KVPAGE_MAX_CALL = 4096
+KVPAGE_MAX_ROWS = 65536
 KVHASH_ALGOS = {"sha256": 0, "sha256_cbor": 1}
 
 
@@ -121,6 +129,44 @@ class KvCopyDesc(C.Structure):
     ]
 
 
+class KvPageState(C.Structure):
+    """struct kv_page_state (include/kvpage.h)."""
+
+    _fields_ = [
+        ("table", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("refs", C.c_void_p),
+        ("free_list", C.c_void_p),
+        ("free_count", C.c_void_p),
+        ("marks", C.c_void_p),
+        ("error", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("width", C.c_uint32),
+        ("num_rows", C.c_uint32),
+        ("num_pages", C.c_uint32),
+        ("block_size", C.c_uint32),
+        ("device", C.c_int32),
+    ]
+
+
+class KvPageCache(C.Structure):
+    """struct kv_page_cache (include/kvpage.h)."""
+
+    _fields_ = [
+        ("layer_k", C.c_void_p),
+        ("layer_v", C.c_void_p),
+        ("error", C.c_void_p),
+        ("block_stride", C.c_uint64),
+        ("unit_bytes", C.c_uint32),
+        ("head_bytes", C.c_uint32),
+        ("block_size", C.c_uint32),
+        ("num_layers", C.c_uint32),
+        ("num_pages", C.c_uint32),
+        ("base_align", C.c_uint32),
+        ("device", C.c_int32),
+    ]
+
+
 class CacheStats(C.Structure):
     """struct cache_stats (include/cache.h, new)."""
 
@@ -192,6 +238,13 @@ SIGNATURES: dict[str, tuple] = {
     "kv_copy_noalloc": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32,
                                   C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32,
                                   C.c_uint32, C.c_void_p]),
+    # include/kvpage.h (structs and arrays by address: the callers keep them)
+    "kv_page_resize_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "kv_page_copy_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
+    "kv_page_fork_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
+                                      C.c_void_p, C.c_void_p]),
+    "kv_page_compact_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),
     # include/kvhash.h
     "kv_block_hash_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),

@@ -40,6 +40,7 @@ CU_SOURCES = [
     "device/cuda_adaptor.cu",
     "device/block_hash.cu",
     "device/kv_copy_noalloc.cu",
+    "device/kv_page.cu",
 ]
 HEADERS = sorted(str(p) for p in list(INCLUDE.glob("*.h")) + list(CSRC.rglob("*.h")))
 
