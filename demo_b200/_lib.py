@@ -30,6 +30,13 @@ KVPAGE_ERR_ALIGN = 0x10
 KVPAGE_OK, KVPAGE_NO_PAGES, KVPAGE_INVALID = 0, 1, 2
 KVPAGE_MAX_CALL = 4096
 KVPAGE_MAX_ROWS = 65536
+KVATTN_ERR_PAGE = 0x1
+KVATTN_ERR_SEQ = 0x2
+KVATTN_ERR_PARENT = 0x4
+KVATTN_ERR_TIMEOUT = 0x8
+KVATTN_BF16, KVATTN_FP16, KVATTN_E4M3 = 0, 1, 2
+KVATTN_MAX_HEAD_DIM = 256
+KVATTN_MAX_SEQS = 65536
 KVHASH_ALGOS = {"sha256": 0, "sha256_cbor": 1}
 
 
@@ -167,6 +174,48 @@ class KvPageCache(C.Structure):
     ]
 
 
+class KvAttnDesc(C.Structure):
+    """struct kv_attn_desc (include/kvattn.h)."""
+
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("table", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("rows", C.c_void_p),
+        ("q_offsets", C.c_void_p),
+        ("parents", C.c_void_p),
+        ("error", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("block_stride", C.c_uint64),
+        ("table_stride", C.c_int64),
+        ("q_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("width", C.c_uint32),
+        ("num_rows", C.c_uint32),
+        ("num_seqs", C.c_uint32),
+        ("total_q", C.c_uint32),
+        ("num_pages", C.c_uint32),
+        ("block_size", C.c_uint32),
+        ("num_heads", C.c_uint32),
+        ("num_kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("head_major", C.c_uint32),
+        ("q_type", C.c_int32),
+        ("kv_type", C.c_int32),
+        ("scale", C.c_float),
+        ("k_scale", C.c_float),
+        ("v_scale", C.c_float),
+        ("device", C.c_int32),
+    ]
+
+
 class CacheStats(C.Structure):
     """struct cache_stats (include/cache.h, new)."""
 
@@ -245,6 +294,9 @@ SIGNATURES: dict[str, tuple] = {
                                       C.c_void_p, C.c_void_p]),
     "kv_page_compact_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                          C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    # include/kvattn.h
+    "kv_attn_workspace_bytes": (C.c_int64, [C.c_void_p]),
+    "kv_attn_launch": (C.c_int, [C.c_void_p, C.c_void_p]),
     # include/kvhash.h
     "kv_block_hash_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),

@@ -1,0 +1,145 @@
+"""Attention over a paged KV cache (include/kvattn.h) for torch tensors:
+single tokens, chains and trees of drafted tokens, straight from the pages that
+the cache manager loads and stores.
+
+CrossCache leaves attention to the engine; the paged geometries are those of
+cache.layout_from_kv_tensors (vLLM's FlashAttention and FlashInfer layouts).
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Sequence
+
+import torch
+
+from . import _lib
+from ._lib import KvAttnDesc, lib
+from .cache import CacheError, KVLayout
+from .pages import _int32
+
+_TYPES = {torch.bfloat16: _lib.KVATTN_BF16, torch.float16: _lib.KVATTN_FP16}
+
+_ERRORS = ((_lib.KVATTN_ERR_PAGE, "a page id outside the cache"),
+           (_lib.KVATTN_ERR_SEQ, "offsets out of order, or a row or length that fits neither table nor nodes"),
+           (_lib.KVATTN_ERR_PARENT, "a parent that does not come before its node"),
+           (_lib.KVATTN_ERR_TIMEOUT, "a wait inside the kernel ran out"))
+
+
+class TreeAttention:
+    """Attention of fed tokens over the layers of one paged cache.
+
+    layout, k_ptrs, v_ptrs: from cache.layout_from_kv_tensors; K and V planes
+        of 16-bit values of the queries' type, or of float8_e4m3fn values
+        (1-byte elements) that k_scale and v_scale bring back
+    num_heads, num_kv_heads: query heads and K/V heads of this rank
+    scale: of the scores, by default head_dim ** -0.5
+    """
+
+    def __init__(self, layout: KVLayout, k_ptrs: Sequence[int], v_ptrs: Sequence[int], num_heads: int, num_kv_heads: int,
+                 scale: float | None = None, k_scale: float = 1.0, v_scale: float = 1.0):
+        if layout.kv != 2 or v_ptrs is None:
+            raise ValueError("attention needs K and V planes (a K-only latent cache is not supported)")
+        if len(k_ptrs) != layout.num_layers or len(v_ptrs) != layout.num_layers:
+            raise ValueError("one pointer per layer")
+        if num_kv_heads < 1 or num_heads % num_kv_heads or layout.hidden_dim_size % num_kv_heads:
+            raise ValueError("num_kv_heads must divide num_heads and the layout's width")
+        if layout.element_size not in (1, 2):
+            raise ValueError("caches of 1 or 2-byte elements")
+        dim = layout.hidden_dim_size // num_kv_heads
+        if layout.head_bytes and layout.head_bytes != dim * layout.element_size:
+            raise ValueError("num_kv_heads does not fit the layout's head-major pages")
+        if dim % 16 or dim > _lib.KVATTN_MAX_HEAD_DIM:
+            raise ValueError(f"head_dim must be a multiple of 16 up to {_lib.KVATTN_MAX_HEAD_DIM} (got {dim})")
+        if any(not p or p % 16 for p in (*k_ptrs, *v_ptrs)) or layout.block_stride % 16:
+            raise ValueError("planes and pages must be 16-byte aligned")
+        scale = dim ** -0.5 if scale is None else float(scale)
+        if not (0 < scale * k_scale < math.inf) or not 0 < scale < math.inf or not math.isfinite(v_scale):
+            raise ValueError("scale and k_scale must be finite and above 0, v_scale finite")
+        self.layout, self.num_heads, self.num_kv_heads, self.head_dim = layout, num_heads, num_kv_heads, dim
+        self._k, self._v = [int(p) for p in k_ptrs], [int(p) for p in v_ptrs]
+        self._errors: dict[int, torch.Tensor] = {}
+        self._desc = KvAttnDesc(
+            block_stride=layout.block_stride, num_pages=layout.num_blocks, block_size=layout.block_size,
+            num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=dim, head_major=1 if layout.head_bytes else 0,
+            scale=scale, k_scale=k_scale, v_scale=v_scale)
+
+    def __call__(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 q_offsets: torch.Tensor, parents: torch.Tensor | None = None, rows: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None, return_lse: bool = False, stream: torch.cuda.Stream | None = None):
+        """out [total, num_heads, head_dim] (and lse [total, num_heads] in
+        float32) of the packed queries q, both as q's type and layout say.
+
+        q            bfloat16 or float16 [total, num_heads, head_dim], CUDA
+        block_table  int32 [rows, width]; seq_lens int32 [rows], the fed tokens included
+        q_offsets    int32 [sequences + 1]: sequence b feeds q[q_offsets[b]:q_offsets[b + 1]]
+        parents      int32 [total]: the tree (-1: the last token before the fed
+                     ones, -2: padding); None: a chain
+        rows         int32 [sequences]: their rows; None: row b
+
+        Runs on `stream`, by default the current stream of q's device.
+        """
+        if q.dim() != 3 or q.dtype not in _TYPES or q.device.type != "cuda" or q.shape[1] != self.num_heads or \
+                q.shape[2] != self.head_dim or q.stride(2) != 1:
+            raise ValueError(f"q: expected a bfloat16 or float16 CUDA tensor [total, {self.num_heads}, {self.head_dim}]")
+        dev, total = q.device, q.shape[0]
+        if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.device != dev or \
+                block_table.shape[1] < 1 or block_table.stride(1) != 1:
+            raise ValueError(f"block_table: expected an int32 tensor [rows, width] on {dev} with contiguous rows")
+        n_rows, width = block_table.shape
+        seqs = q_offsets.numel() - 1
+        if seqs < 0 or (rows is None and seqs > n_rows):
+            raise ValueError("q_offsets: expected one offset per sequence and the end")
+        if out is None:
+            out = torch.empty((total, self.num_heads, self.head_dim), dtype=q.dtype, device=dev)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+            raise ValueError("out: expected a tensor like q")
+        lse = torch.empty((total, self.num_heads), dtype=torch.float32, device=dev) if return_lse else None
+        index = dev.index
+        error = self._errors.get(index)
+        if error is None:
+            error = self._errors[index] = torch.zeros(1, dtype=torch.int32, device=dev)
+        d = KvAttnDesc.from_buffer_copy(self._desc)     # calls from several threads share nothing
+        d.q, d.out, d.k, d.v = q.data_ptr(), out.data_ptr(), self._k[layer], self._v[layer]
+        d.lse = lse.data_ptr() if return_lse else None
+        d.table, d.lens = block_table.data_ptr(), _int32("seq_lens", seq_lens, dev, n_rows)
+        d.rows = _int32("rows", rows, dev, seqs) if rows is not None else None
+        d.q_offsets = _int32("q_offsets", q_offsets, dev)
+        d.parents = _int32("parents", parents, dev, total) if parents is not None else None
+        d.error = error.data_ptr()
+        d.table_stride = block_table.stride(0) if n_rows > 1 else width
+        d.q_stride, d.q_head_stride = q.stride(0), q.stride(1)
+        d.out_stride, d.out_head_stride = out.stride(0), out.stride(1)
+        d.width, d.num_rows, d.num_seqs, d.total_q = width, n_rows, seqs, total
+        d.q_type = _TYPES[q.dtype]
+        d.kv_type = _lib.KVATTN_E4M3 if self.layout.element_size == 1 else d.q_type
+        d.device = index
+        p = C.addressof(d)
+        need = lib.kv_attn_workspace_bytes(p)
+        if need < 0:
+            raise CacheError("kv_attn_workspace_bytes", need)
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        if stream is None:
+            st = torch.cuda.current_stream(dev).cuda_stream
+        else:
+            st = stream.cuda_stream
+            for t in (out, lse, work):      # the allocator frees them for the current stream otherwise
+                if t is not None:
+                    t.record_stream(stream)
+        d.workspace, d.workspace_bytes = work.data_ptr(), need
+        ret = lib.kv_attn_launch(p, st)
+        if ret:
+            raise CacheError("kv_attn_launch", ret)
+        return (out, lse) if return_lse else out
+
+    def check(self) -> None:
+        """Wait for the device and raise ValueError for what the calls since
+        the last check() found wrong in their arguments."""
+        for error in self._errors.values():
+            bits = int(error.item())
+            if bits:
+                error.zero_()
+                raise ValueError("tree attention: " + "; ".join(text for bit, text in _ERRORS if bits & bit))
+
+
+__all__ = ["TreeAttention"]

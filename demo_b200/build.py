@@ -41,6 +41,7 @@ CU_SOURCES = [
     "device/block_hash.cu",
     "device/kv_copy_noalloc.cu",
     "device/kv_page.cu",
+    "device/kv_attn.cu",
 ]
 HEADERS = sorted(str(p) for p in list(INCLUDE.glob("*.h")) + list(CSRC.rglob("*.h")))
 

@@ -1,0 +1,29 @@
+/* makes a device current for the calling thread while the guard lives */
+#ifndef DEVICE_GUARD_H
+#define DEVICE_GUARD_H
+
+#include <cuda_runtime.h>
+
+struct DeviceGuard {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceGuard(int device)
+    {
+        int now = -1;
+        if (device < 0 || cudaGetDevice(&now) != cudaSuccess)
+            return;
+        if (now != device) {
+            if (cudaSetDevice(device) != cudaSuccess)
+                return;
+            before = now;
+        }
+        ok = true;
+    }
+    ~DeviceGuard()
+    {
+        if (before >= 0)
+            cudaSetDevice(before);
+    }
+};
+
+#endif

@@ -13,6 +13,7 @@
  */
 #include "kvpage.h"
 #include "adaptor.h"
+#include "device_guard.h"
 
 #include <cuda_runtime.h>
 
@@ -26,29 +27,6 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr uint32_t kPlanCluster = 8;
 constexpr int32_t kRefused = INT32_MIN;     /* compact's length for resize of a row that it has refused and reported */
-
-/* makes `device` current for the calling thread while it lives */
-struct DeviceGuard {
-    int before = -1;
-    bool ok = false;
-    explicit DeviceGuard(int device)
-    {
-        int now = -1;
-        if (device < 0 || cudaGetDevice(&now) != cudaSuccess)
-            return;
-        if (now != device) {
-            if (cudaSetDevice(device) != cudaSuccess)
-                return;
-            before = now;
-        }
-        ok = true;
-    }
-    ~DeviceGuard()
-    {
-        if (before >= 0)
-            cudaSetDevice(before);
-    }
-};
 
 /* ---- the cluster's barrier and shared memory ---- */
 __device__ __forceinline__ uint32_t cluster_rank()

@@ -1,0 +1,128 @@
+"""Tree attention without a GPU: what the C entry points and TreeAttention
+refuse before anything is launched, the struct's layout, the oracle."""
+import ctypes as C
+import errno
+import math
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from demo_b200._lib import KVATTN_BF16, KVATTN_E4M3, KVATTN_FP16, KVATTN_MAX_SEQS, KvAttnDesc, lib
+from demo_b200.attention import TreeAttention
+from demo_b200.cache import KVLayout
+from oracle import attention as oa
+
+INCLUDE = Path(__file__).resolve().parent.parent / "include"
+X = 0x1000          # an address that is never followed
+
+
+def desc(**k):
+    d = dict(q=X, out=X, lse=X, k=X, v=X, table=X, lens=X, q_offsets=X, error=X, workspace=X, workspace_bytes=1 << 40,
+             table_stride=8, q_stride=1024, q_head_stride=128, out_stride=1024, out_head_stride=128, width=8, num_rows=4,
+             num_seqs=4, total_q=4, num_pages=32, block_size=16, num_heads=8, num_kv_heads=2, head_dim=128,
+             q_type=KVATTN_BF16, kv_type=KVATTN_BF16, scale=0.1, k_scale=1.0, v_scale=1.0)
+    return KvAttnDesc(**{**d, **k})
+
+
+SHAPES = [dict(num_heads=0), dict(num_kv_heads=0), dict(num_kv_heads=3), dict(head_dim=0), dict(head_dim=120),
+          dict(head_dim=272), dict(block_size=0), dict(num_pages=0), dict(num_pages=1 << 31), dict(width=0),
+          dict(table_stride=7), dict(num_rows=0), dict(q_type=KVATTN_E4M3), dict(q_type=5), dict(kv_type=KVATTN_FP16),
+          dict(block_stride=4096), dict(block_stride=8200), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+          dict(k_scale=0.0), dict(k_scale=math.inf), dict(v_scale=math.nan), dict(device=-1), dict(device=64)]
+POINTERS = [dict(q=None), dict(out=None), dict(k=None), dict(v=None), dict(table=None), dict(lens=None),
+            dict(q_offsets=None), dict(error=None), dict(q=X + 8), dict(out=X + 2), dict(k=X + 8), dict(v=X + 4),
+            dict(q_stride=1020), dict(q_head_stride=4), dict(out_stride=1001), dict(out_head_stride=130)]
+
+
+@pytest.mark.parametrize("bad", SHAPES, ids=str)
+def test_malformed_shapes_are_refused(bad):
+    p = C.addressof(d := desc(**bad))
+    assert lib.kv_attn_workspace_bytes(p) == -errno.EINVAL
+    assert lib.kv_attn_launch(p, None) == -errno.EINVAL, d
+
+
+@pytest.mark.parametrize("bad", POINTERS, ids=str)
+def test_malformed_pointers_are_refused(bad):
+    p = C.addressof(d := desc(**bad))
+    assert lib.kv_attn_workspace_bytes(p) >= 0
+    assert lib.kv_attn_launch(p, None) == -errno.EINVAL, d
+
+
+def test_limits_and_empty_calls():
+    assert lib.kv_attn_launch(None, None) == -errno.EINVAL
+    assert lib.kv_attn_workspace_bytes(None) == -errno.EINVAL
+    d = desc(num_seqs=KVATTN_MAX_SEQS + 1)
+    assert lib.kv_attn_launch(C.addressof(d), None) == -errno.E2BIG
+    n0 = lib.crosscache_kernel_launches()
+    for empty in (desc(num_seqs=0), desc(total_q=0, q=None, out=None)):
+        assert lib.kv_attn_launch(C.addressof(empty), None) == 0
+    assert lib.crosscache_kernel_launches() == n0
+
+
+def layout(**k):
+    return KVLayout(**{**dict(num_layers=1, num_blocks=8, block_size=16, hidden_dim_size=256, element_size=2, kv=2), **k})
+
+
+@pytest.mark.parametrize("make, match", [
+    (lambda: TreeAttention(layout(kv=1), [X], None, 8, 2), "K and V"),
+    (lambda: TreeAttention(layout(), [X, X], [X], 8, 2), "one pointer"),
+    (lambda: TreeAttention(layout(), [X], [X], 8, 3), "must divide"),
+    (lambda: TreeAttention(layout(), [X], [X], 8, 0), "must divide"),
+    (lambda: TreeAttention(layout(hidden_dim_size=240), [X], [X], 8, 2), "multiple of 16"),
+    (lambda: TreeAttention(layout(hidden_dim_size=1024), [X], [X], 8, 2), "multiple of 16"),
+    (lambda: TreeAttention(layout(element_size=4), [X], [X], 8, 2), "1 or 2-byte"),
+    (lambda: TreeAttention(layout(head_bytes=128), [X], [X], 8, 2), "head-major"),
+    (lambda: TreeAttention(layout(), [X + 8], [X], 8, 2), "aligned"),
+    (lambda: TreeAttention(layout(), [X], [0], 8, 2), "aligned"),
+    (lambda: TreeAttention(layout(), [X], [X], 8, 2, scale=0.0), "above 0"),
+    (lambda: TreeAttention(layout(), [X], [X], 8, 2, k_scale=-1.0), "above 0"),
+    (lambda: TreeAttention(layout(), [X], [X], 8, 2, v_scale=math.inf), "finite"),
+])
+def test_construction_refuses(make, match):
+    with pytest.raises(ValueError, match=match):
+        make()
+
+
+def test_calls_refuse_tensors_they_cannot_use():
+    att = TreeAttention(layout(), [X], [X], 8, 2)
+    i32 = torch.zeros(4, dtype=torch.int32)
+    for q in (torch.zeros(4, 8, 128, dtype=torch.bfloat16), torch.zeros(4, 8, 128), torch.zeros(4, 1024)):
+        with pytest.raises(ValueError, match="q: expected"):
+            att(0, q, torch.zeros(4, 2, dtype=torch.int32), i32, torch.zeros(5, dtype=torch.int32))
+
+
+PROBE = r"""
+#include <stdio.h>
+#include <stddef.h>
+#include "kvattn.h"
+#define F(f) printf(#f " %zu\n", offsetof(struct kv_attn_desc, f))
+int main(void) {
+  printf(" %zu\n", sizeof(struct kv_attn_desc));
+  F(parents); F(workspace_bytes); F(table_stride); F(out_head_stride); F(width); F(head_major); F(kv_type); F(v_scale); F(device);
+  return 0;
+}
+"""
+
+
+def test_struct_layout(tmp_path):
+    (tmp_path / "p.c").write_text(PROBE)
+    subprocess.run(["gcc", "-std=c11", f"-I{INCLUDE}", str(tmp_path / "p.c"), "-o", str(tmp_path / "p")], check=True)
+    out = subprocess.run([str(tmp_path / "p")], capture_output=True, text=True, check=True).stdout
+    for line in out.splitlines():
+        field, val = line.split(" ")
+        assert (getattr(KvAttnDesc, field).offset if field else C.sizeof(KvAttnDesc)) == int(val), field
+
+
+def test_the_oracle_on_a_case_worked_by_hand():
+    """scores 0 everywhere: the mean of the values seen"""
+    q = torch.zeros(4, 2, 16, dtype=torch.bfloat16)
+    k = torch.randn(3, 2, 1, 16, dtype=torch.float64)
+    v = torch.arange(6, dtype=torch.float64).reshape(3, 2, 1, 1).expand(3, 2, 1, 16)
+    # one row, pages 2 and 0: values 4, 5, 0, 1; 1 cached token, then the path 0 - 2 and a padding node
+    out, lse, _, _ = oa.attention(q[:3], k, v, [[2, 0]], [4], [0, 3], [-1, -2, 0])
+    assert out[:, 0, 0].tolist() == [4.5, 0.0, 10 / 3]
+    assert lse[:, 1].tolist() == pytest.approx([math.log(2), -math.inf, math.log(3)])
+    assert oa.visible(None, 3) == [{0}, {0, 1}, {0, 1, 2}]
+    assert oa.visible([-1, -2, 1, 0, 7], 5) == [{0}, None, {2}, {0, 3}, None]
