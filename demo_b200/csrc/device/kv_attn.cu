@@ -32,6 +32,7 @@
 #include "kvattn.h"
 #include "adaptor.h"
 #include "device_guard.h"
+#include "fastdiv.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -67,12 +68,19 @@ template <int DP> struct Shape {
     static_assert(2 * kTile + DP <= kTmem && kCtas * kTmem <= 512, "and its TMEM");
 };
 
+/* a row tile that lies across CTAs: its first piece is the last of CTA c (in
+ * that CTA's place `slot`), the others are the first of CTAs c + 1 .. */
+struct Job {
+    int32_t rows, ctas, slot, q0, h, row0;
+};
+
 struct Params {
     kv_attn_desc d;
     uint64_t stride;        /* bytes from page to page */
-    uint32_t group;         /* query heads per K/V head */
+    FastDiv group;          /* query heads per K/V head */
+    FastDiv block;          /* positions of a page */
     uint32_t min_share;     /* tiles that a CTA takes at least */
-    int64_t *prefix;        /* workspace: [num_seqs + 1] tiles before each sequence, then the share */
+    struct Job *jobs;       /* workspace: [CTAs] row tiles to be joined, by the CTA that has their first tiles */
     float *part_ml;         /* [2 * CTAs][128][2] maximum and sum of a piece */
     float *part_o;          /* [2 * CTAs][128][dim] */
 };
@@ -107,27 +115,26 @@ __device__ __forceinline__ bool node_ok(const int32_t *parents, int32_t j)
     return u >= -1 && u < j;
 }
 
-__device__ __forceinline__ int32_t row_tiles(const Seq &s, uint32_t group)
+__device__ __forceinline__ int32_t row_tiles(const Seq &s, const FastDiv &group)
 {
-    return (int32_t)(((int64_t)s.nodes * group + kRows - 1) / kRows);
+    return (int32_t)((s.nodes * group.d + kRows - 1) / kRows);
 }
 
 /* positions that row tile rt's nodes may see: parents come before their nodes */
-__device__ __forceinline__ int32_t visible_end(const Seq &s, uint32_t group, int32_t rt)
+__device__ __forceinline__ int32_t visible_end(const Seq &s, const FastDiv &group, int32_t rt)
 {
-    const int64_t last = ((int64_t)(rt + 1) * kRows - 1) / group;
-    return s.ctx + (int32_t)min((int64_t)s.nodes, last + 1);
+    return s.ctx + min(s.nodes, (int32_t)fdiv((uint32_t)(rt + 1) * kRows - 1, group) + 1);
 }
 
-__device__ __forceinline__ int32_t tiles_of(const Seq &s, uint32_t group, int32_t rt)
+__device__ __forceinline__ int32_t tiles_of(const Seq &s, const FastDiv &group, int32_t rt)
 {
     return (visible_end(s, group, rt) + kTile - 1) / kTile;
 }
 
-/* tiles of one K/V head of the sequence */
-__device__ int64_t head_tiles(const Seq &s, uint32_t group)
+/* tiles of one K/V head of the sequence, all row tiles */
+__device__ __forceinline__ uint64_t head_tiles(const Seq &s, const FastDiv &group)
 {
-    int64_t n = 0;
+    uint64_t n = 0;
     for (int32_t rt = 0; rt < row_tiles(s, group); rt++)
         n += tiles_of(s, group, rt);
     return n;
@@ -137,45 +144,35 @@ __device__ int64_t head_tiles(const Seq &s, uint32_t group)
 struct Piece {
     Seq s;
     int32_t h, rt, t0, t1, n;       /* tiles t0 .. t1 of n */
-    bool at_start;                  /* begins where the CTA's line begins */
     __device__ bool whole() const { return t0 == 0 && t1 == n; }
 };
 
 struct Line {
-    int64_t x, hi, base, per_head;
+    int64_t x, hi, base;
+    uint64_t per_head;
     uint32_t b;
-    Seq s;
-    bool started = false;
+    Seq s;                          /* sequence b, its tiles per K/V head, and the tiles before it */
 
-    __device__ void enter(const Params &p)
-    {
-        per_head = sequence(p.d, b, s) ? head_tiles(s, p.group) : 0;
-    }
     __device__ bool next(const Params &p, Piece &e)
     {
         if (x >= hi)
             return false;
-        const bool first = !started;
-        if (first)
-            enter(p);
-        started = true;
-        while (x >= base + per_head * p.d.num_kv_heads) {
-            base += per_head * p.d.num_kv_heads;
+        while (x >= base + (int64_t)(per_head * p.d.num_kv_heads)) {
+            base += (int64_t)(per_head * p.d.num_kv_heads);
             b++;
-            enter(p);
+            per_head = sequence(p.d, b, s) ? head_tiles(s, p.group) : 0;
         }
-        int64_t y = x - base;
-        e.h = (int32_t)(y / per_head);
+        uint64_t y = x - base;
+        e.h = (int32_t)((y | per_head) >> 32 ? y / per_head : (uint32_t)y / (uint32_t)per_head);
         y -= e.h * per_head;
         e.rt = 0;
-        for (e.n = tiles_of(s, p.group, 0); y >= e.n; e.n = tiles_of(s, p.group, e.rt)) {
+        for (e.n = tiles_of(s, p.group, 0); y >= (uint64_t)e.n; e.n = tiles_of(s, p.group, e.rt)) {
             y -= e.n;
             e.rt++;
         }
         e.s = s;
         e.t0 = (int32_t)y;
-        e.t1 = (int32_t)min((int64_t)e.n, y + (hi - x));
-        e.at_start = first;
+        e.t1 = (int32_t)min((int64_t)e.n, (int64_t)y + (hi - x));
         x += e.t1 - e.t0;
         return true;
     }
@@ -208,9 +205,8 @@ struct Shared {
     uint64_t full[8], empty[8], s_full[2], p_full[2], o_done[2], o_free, q_full, q_empty;
     uint32_t tmem;
     volatile uint32_t dead;         /* a wait ran out: every role leaves */
-    uint32_t found;
-    int64_t lo, hi, base, scan[kThreads / 32];
-    uint32_t b;
+    int64_t share, scan[kThreads / 32];
+    Line line;                      /* the CTA's part of it */
     volatile uint32_t spoilt[16];   /* [piece % 16] == piece + 1: values of its fed nodes that are not finite were set aside */
 };
 static_assert(sizeof(Shared) <= 1024, "the last KiB of the dynamic shared memory");
@@ -243,12 +239,15 @@ __device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint64_t *
     return __all_sync(~0u, wait(sh, error, bar, parity));
 }
 
-/* shared-memory matrix descriptor, 128-byte swizzle */
-__device__ __forceinline__ uint64_t matrix(uint32_t addr, uint32_t lead, uint32_t stride)
+/* shared-memory matrix descriptor, 128-byte swizzle: the low word (where it
+ * starts, and the bytes between 64-value columns of an operand stored row by
+ * row) and the high word, which is the same for all here (1024 bytes from one
+ * group of eight rows to the next) */
+__device__ __forceinline__ uint32_t matrix(uint32_t addr, uint32_t lead)
 {
-    return (uint64_t)(addr >> 4 & 0x3fff) | (uint64_t)(lead >> 4 & 0x3fff) << 16 | (uint64_t)(stride >> 4 & 0x3fff) << 32 |
-           1ull << 46 | 2ull << 61;
+    return (addr >> 4 & 0x3fff) | (lead >> 4 & 0x3fff) << 16;
 }
+constexpr uint32_t kMatrixHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
 
 /* instruction descriptor of kind::f16: 128 rows, n columns, 32-bit sums; b_rows: B is stored row by row (k outermost) */
 __device__ __forceinline__ uint32_t instruction(uint32_t bf16, uint32_t n, uint32_t b_rows)
@@ -256,18 +255,20 @@ __device__ __forceinline__ uint32_t instruction(uint32_t bf16, uint32_t n, uint3
     return 1u << 4 | bf16 << 7 | bf16 << 10 | b_rows << 16 | (n >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t inst, bool add)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t inst, bool add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(inst), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(inst), "r"((uint32_t)add), "r"(kMatrixHigh) : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t inst, bool add)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t inst, bool add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(inst), "r"((uint32_t)add) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "mov.b64 b, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(inst), "r"((uint32_t)add), "r"(kMatrixHigh) : "memory");
 }
 
 /* arrive at `bar` when the products issued so far are done */
@@ -387,52 +388,66 @@ template <typename T, bool F8, int DP> struct Loader {
     static constexpr int kChunks = F8 ? DP / 16 : DP / 8;       /* 16-byte loads of a cached row */
     static constexpr int kPass = kLoaders / kChunks;            /* rows of one pass */
     static constexpr int kPasses = kTile / kPass;
+    static constexpr int kWarpRows = kPass / (kLoaders / 32);   /* of them a warp's */
     static constexpr int kQChunks = DP / 8, kQPass = kLoaders / kQChunks;
+    static_assert(kPasses * kWarpRows == 16, "a lane of each half warp looks after one of the warp's rows");
 
     const Params &p;
     Shared &sh;
     uint8_t *q_smem, *ring;
     uint32_t chunk, row;                /* this thread's chunk, and row of a pass */
+    uint32_t own_row;                   /* the row of a tile whose place this lane works out */
+    uint32_t tok_bytes;
     bool in_dim;
-    uint64_t off[kPasses];              /* of this thread's rows in the planes */
-    uint32_t on;                        /* bit per pass: a position that counts */
+    uint64_t off[kPasses];              /* of this thread's rows in the planes, kNone: read as zeros */
     bool q_due = false;                 /* Q of the piece is still to be loaded */
+    static constexpr uint64_t kNone = ~0ull;
 
     __device__ Loader(const Params &p_, Shared &sh_, uint8_t *q_, uint8_t *ring_) : p(p_), sh(sh_), q_smem(q_), ring(ring_)
     {
-        const uint32_t t = threadIdx.x - kSoftmax;
+        const uint32_t t = threadIdx.x - kSoftmax, lane = t % 32, warp = t / 32;
         chunk = t % kChunks;
         row = t / kChunks;
+        own_row = lane % 16 / kWarpRows * kPass + warp * kWarpRows + lane % kWarpRows;
         in_dim = chunk * (F8 ? 16 : 8) < p.d.head_dim;
+        tok_bytes = (p.d.head_major ? 1 : p.d.num_kv_heads) * p.d.head_dim * (F8 ? 1 : 2);
     }
 
-    __device__ void places(const Piece &e, int32_t t)
+    /* the page of this lane's row of tile t: a load that waits for nothing */
+    __device__ int32_t look_up(const Piece &e, int32_t t) const
+    {
+        const uint32_t pos = t * kTile + own_row;
+        const int32_t *tab = p.d.table + (int64_t)e.s.row * p.d.table_stride;
+        return (int32_t)pos < visible_end(e.s, p.group, e.rt) ? tab[fdiv(pos, p.block)] : -1;
+    }
+
+    /* The places of the thread's rows: each lane works out one, the threads of
+     * a row take it from there. */
+    __device__ void places(const Piece &e, int32_t t, int32_t page)
     {
         const kv_attn_desc &d = p.d;
-        const int32_t end = visible_end(e.s, p.group, e.rt);
-        const int32_t *tab = d.table + (int64_t)e.s.row * d.table_stride;
-        const uint32_t esz = F8 ? 1 : 2;
-        const uint64_t tok = (uint64_t)(d.head_major ? 1 : d.num_kv_heads) * d.head_dim * esz;
-        const uint64_t head = (uint64_t)(d.head_major ? d.block_size : 1) * d.head_dim * esz * e.h + chunk * 16;
-        on = 0;
-#pragma unroll
-        for (int i = 0; i < kPasses; i++) {
-            const int32_t pos = t * kTile + (int32_t)row + i * kPass;
-            off[i] = 0;
-            if (pos >= end)
-                continue;
-            const uint32_t b = (uint32_t)pos / d.block_size;
-            const int32_t page = tab[b];
-            bool good = page >= 0 && (uint32_t)page < d.num_pages;
-            if (!good && chunk == 0)
+        const uint32_t pos = t * kTile + own_row, j = pos - fdiv(pos, p.block) * p.block.d;
+        const bool here = (int32_t)pos < visible_end(e.s, p.group, e.rt);
+        uint64_t own = kNone;
+        if (here) {
+            if ((uint32_t)page < d.num_pages)
+                own = (uint64_t)(uint32_t)page * p.stride + (uint64_t)j * tok_bytes +
+                      (uint64_t)(d.head_major ? d.block_size : 1) * d.head_dim * (F8 ? 1 : 2) * e.h;
+            else
                 atomicOr(d.error, KVATTN_ERR_PAGE);
-            if (pos >= e.s.ctx && d.parents && !node_ok(d.parents + e.s.q0, pos - e.s.ctx))
-                good = false;           /* a padding node */
-            if (good) {
-                off[i] = page * p.stride + (pos - b * d.block_size) * tok + head;
-                on |= (uint32_t)in_dim << i;
-            }
+            if (d.parents && (int32_t)pos >= e.s.ctx && !node_ok(d.parents + e.s.q0, pos - e.s.ctx))
+                own = kNone;            /* padding nodes are not read */
         }
+        const uint32_t from = threadIdx.x % 32 / kChunks;
+#pragma unroll
+        for (int i = 0; i < kPasses; i++)
+            off[i] = __shfl_sync(~0u, own, i * kWarpRows + from);
+    }
+
+    /* pass i's address in a plane (its start, for rows that are zeros) */
+    __device__ const void *address(const void *plane, int i) const
+    {
+        return static_cast<const char *>(plane) + (off[i] == kNone ? 0 : off[i] + chunk * 16);
     }
 
     /* Q of the piece, once the products of the piece before have read theirs;
@@ -445,12 +460,12 @@ template <typename T, bool F8, int DP> struct Loader {
                 return false;
         }
         const uint32_t t = threadIdx.x - kSoftmax, c = t % kQChunks;
-        const int64_t rows = (int64_t)e.s.nodes * p.group - (int64_t)e.rt * kRows;
+        const int32_t rows = (int32_t)(e.s.nodes * p.group.d) - e.rt * kRows;
         if (c * 8 < p.d.head_dim)
-            for (uint32_t r = t / kQChunks; r < kRows && r < rows; r += kQPass) {
-                const uint32_t x = e.rt * kRows + r, node = x / p.group, g = x - node * p.group;
+            for (uint32_t r = t / kQChunks; r < kRows && (int32_t)r < rows; r += kQPass) {
+                const uint32_t x = e.rt * kRows + r, node = fdiv(x, p.group), g = x - node * p.group.d;
                 const T *src = static_cast<const T *>(p.d.q) + (int64_t)(e.s.q0 + node) * p.d.q_stride +
-                               (int64_t)(e.h * p.group + g) * p.d.q_head_stride + c * 8;
+                               (int64_t)(e.h * p.group.d + g) * p.d.q_head_stride + c * 8;
                 copy16(smem_u32(q_smem) + swizzled(kRows, r, c), src, true);
             }
         copy_arrive(&sh.q_full);
@@ -464,9 +479,10 @@ template <typename T, bool F8, int DP> struct Loader {
     {
         uint64_t *bar = &sh.empty[i % S::kSlots];
         const uint32_t parity = ((i / S::kSlots) & 1) ^ 1;
-        if (q_due && !load_q(e, piece, false) && !mbar_try_wait(bar, parity) && !load_q(e, piece, true))
-            return false;
-        return wait(sh, p.d.error, bar, parity);
+        bool ok = true;
+        if (q_due && !load_q(e, piece, false) && !mbar_try_wait(bar, parity))
+            ok = load_q(e, piece, true);
+        return __all_sync(~0u, ok && wait(sh, p.d.error, bar, parity));
     }
 
     __device__ uint8_t *slot(uint32_t i) const { return ring + (i % S::kSlots) * S::kSlotBytes; }
@@ -478,21 +494,24 @@ template <typename T, bool F8, int DP> struct Loader {
         Piece e;
         for (; line.next(p, e); piece++) {
             q_due = true;
+            int32_t page = look_up(e, e.t0);
             for (int32_t t = e.t0; t < e.t1; t++) {
-                places(e, t);
+                places(e, t, page);
+                if (t + 1 < e.t1)
+                    page = look_up(e, t + 1);       /* in flight while the tile is copied */
                 for (int v = 0; v < 2; v++, i++) {
                     if (!acquire(i, e, piece))
                         return;
-                    const char *base = static_cast<const char *>(v ? p.d.v : p.d.k);
+                    const void *plane = v ? p.d.v : p.d.k;
                     const uint32_t to = smem_u32(slot(i));
                     if (in_dim)
 #pragma unroll
                         for (int x = 0; x < kPasses; x++)
-                            copy16(to + swizzled(kTile, row + x * kPass, chunk), base + off[x], on >> x & 1);
+                            copy16(to + swizzled(kTile, row + x * kPass, chunk), address(plane, x), off[x] != kNone);
                     copy_arrive(&sh.full[i % S::kSlots]);
                 }
             }
-            if (q_due && !load_q(e, piece, true))
+            if (!__all_sync(~0u, !q_due || load_q(e, piece, true)))
                 return;
         }
     }
@@ -503,9 +522,9 @@ template <typename T, bool F8, int DP> struct Loader {
 #pragma unroll
         for (int x = 0; x < kPasses; x++) {
             k[x] = v[x] = make_uint4(0, 0, 0, 0);
-            if (on >> x & 1) {
-                k[x] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(p.d.k) + off[x]));
-                v[x] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(p.d.v) + off[x]));
+            if (in_dim && off[x] != kNone) {
+                k[x] = __ldg(static_cast<const uint4 *>(address(p.d.k, x)));
+                v[x] = __ldg(static_cast<const uint4 *>(address(p.d.v, x)));
             }
         }
     }
@@ -535,8 +554,10 @@ template <typename T, bool F8, int DP> struct Loader {
         uint4 k[kPasses], v[kPasses], k2[kPasses], v2[kPasses];
         if (!line.next(p, now))
             return;
-        int32_t t = now.t0;
-        places(now, t);
+        int32_t t = now.t0, page = look_up(now, t);
+        places(now, t, page);
+        if (t + 1 < now.t1)
+            page = look_up(now, t + 1);
         fetch(k, v);
         uint32_t piece = 0, i = 0;
         q_due = true;
@@ -546,7 +567,13 @@ template <typename T, bool F8, int DP> struct Loader {
             if (last)
                 more = moved = line.next(p, then);
             if (more) {
-                places(moved ? then : now, moved ? then.t0 : t + 1);
+                const Piece &e = moved ? then : now;
+                const int32_t u = moved ? then.t0 : t + 1;
+                if (moved)
+                    page = look_up(e, u);
+                places(e, u, page);
+                if (u + 1 < e.t1)
+                    page = look_up(e, u + 1);
                 fetch(k2, v2);
             }
             if (!acquire(i, now, piece))
@@ -555,7 +582,7 @@ template <typename T, bool F8, int DP> struct Loader {
             if (!acquire(i, now, piece))
                 return;
             put(i++, v);
-            if (last && q_due && !load_q(now, piece, true))
+            if (!__all_sync(~0u, !last || !q_due || load_q(now, piece, true)))
                 return;
 #pragma unroll
             for (int x = 0; x < kPasses; x++) {
@@ -585,22 +612,32 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
     using S = Shape<DP>;
     const uint32_t dim = p.d.head_dim, tmem = sh.tmem, o = tmem + 2 * kTile;
     const uint32_t inst_s = instruction(Type<T>::kBf16, kTile, 0), inst_o = instruction(Type<T>::kBf16, dim, 1);
-    const uint32_t q = smem_u32(q_smem), ring0 = smem_u32(ring);
-    uint32_t g = 0, piece = 0;
+    /* one thread issues: descriptors are a constant per step on top of the slot's */
+    const uint32_t q0 = matrix(smem_u32(q_smem), 16), k0 = matrix(smem_u32(ring), 16), v0 = matrix(smem_u32(ring), kTile * 128);
+    uint32_t g = 0, piece = 0, slot = 0, lap = 0;       /* the slot of K of the next S, and the ring's lap */
     Piece e;
     auto scores = [&](uint32_t tile) {
-        const uint32_t i = 2 * tile, slot = i % S::kSlots;
-        if (!wait(sh, p.d.error, &sh.full[slot], (i / S::kSlots) & 1))
+        if (!wait(sh, p.d.error, &sh.full[slot], lap & 1))
             return false;
         fence_async_proxy();
         tmem_fence_after();
-        for (uint32_t k = 0; k < dim / 16; k++)
-            mma_ss(tmem + (tile & 1) * kTile, matrix(q + (k >> 2) * (kRows * 128) + (k & 3) * 32, 16, 1024),
-                   matrix(ring0 + slot * S::kSlotBytes + (k >> 2) * (kTile * 128) + (k & 3) * 32, 16, 1024), inst_s, k > 0);
+        const uint32_t k = k0 + slot * (S::kSlotBytes >> 4);
+        const uint32_t s = tmem + (tile & 1) * kTile;
+#pragma unroll
+        for (uint32_t x = 0; x < DP / 16; x++)
+            if (x * 16 < dim)
+                mma_ss(s, q0 + ((x >> 2) * (kRows * 128) + (x & 3) * 32 >> 4), k + ((x >> 2) * (kTile * 128) + (x & 3) * 32 >> 4),
+                       inst_s, x > 0);
         mma_commit(&sh.empty[slot]);
         mma_commit(&sh.s_full[tile & 1]);
+        slot += 2;
+        if (slot >= S::kSlots) {
+            slot -= S::kSlots;
+            lap++;
+        }
         return true;
     };
+    uint32_t v_slot = 1, v_lap = 0;
     while (line.next(p, e)) {
         const uint32_t n = e.t1 - e.t0;
         if (!wait(sh, p.d.error, &sh.q_full, piece & 1) || !scores(g))
@@ -614,19 +651,24 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
                 if (k + 2 == n)
                     mma_commit(&sh.q_empty);    /* every S of the piece is issued */
             }
-            const uint32_t i = 2 * g + 1, slot = i % S::kSlots;
             if (k == 0 && piece && !wait(sh, p.d.error, &sh.o_free, (piece - 1) & 1))
                 return;
             if (!wait(sh, p.d.error, &sh.p_full[g & 1], (g >> 1) & 1) ||
-                !wait(sh, p.d.error, &sh.full[slot], (i / S::kSlots) & 1))
+                !wait(sh, p.d.error, &sh.full[v_slot], v_lap & 1))
                 return;
             fence_async_proxy();
             tmem_fence_after();
+            const uint32_t v = v0 + v_slot * (S::kSlotBytes >> 4);
+#pragma unroll
             for (uint32_t x = 0; x < kTile / 16; x++)
-                mma_ts(o, tmem + (g & 1) * kTile + x * 8,
-                       matrix(ring0 + slot * S::kSlotBytes + x * 2048, kTile * 128, 1024), inst_o, k > 0 || x > 0);
-            mma_commit(&sh.empty[slot]);
+                mma_ts(o, tmem + (g & 1) * kTile + x * 8, v + (x * 2048 >> 4), inst_o, k > 0 || x > 0);
+            mma_commit(&sh.empty[v_slot]);
             mma_commit(&sh.o_done[g & 1]);
+            v_slot += 2;
+            if (v_slot >= S::kSlots) {
+                v_slot -= S::kSlots;
+                v_lap++;
+            }
         }
         piece++;
     }
@@ -734,9 +776,9 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
     uint32_t g = 0, piece = 0;
     Piece e;
     for (; line.next(p, e); piece++) {
-        const int64_t x = (int64_t)e.rt * kRows + tid;
-        const bool valid = x < (int64_t)e.s.nodes * p.group;
-        const int32_t node = valid ? (int32_t)(x / p.group) : 0, sub = valid ? (int32_t)(x - (int64_t)node * p.group) : 0;
+        const uint32_t x = e.rt * kRows + tid;
+        const bool valid = x < e.s.nodes * p.group.d;
+        const int32_t node = valid ? (int32_t)fdiv(x, p.group) : 0, sub = valid ? (int32_t)(x - node * p.group.d) : 0;
         bool active = valid;
         if (valid && d.parents && !node_ok(d.parents + e.s.q0, node)) {
             active = false;
@@ -807,7 +849,9 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
                 if (set_aside<T, DP>(ring + slot * S::kSlotBytes, d.head_dim))
                     sh.spoilt[piece % 16] = piece + 1;
             }
-            mbar_arrive(&sh.p_full[g & 1]);
+            __syncwarp();
+            if (tid % 32 == 0)
+                mbar_arrive(&sh.p_full[g & 1]);
         }
         /* the piece's result, or its share of it */
         if (!wait_warp(sh, d.error, &sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1))
@@ -815,9 +859,9 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
         tmem_fence_after();
         const bool whole = e.whole();
         const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
-        const uint32_t slot = 2 * blockIdx.x + (e.at_start ? 0 : 1);
+        const uint32_t slot = 2 * blockIdx.x + (piece ? 1 : 0);
         const float inv = !active ? 0.f : whole ? d.v_scale / l : 1.f;
-        T *out = static_cast<T *>(d.out) + (int64_t)(e.s.q0 + node) * d.out_stride + (int64_t)(e.h * p.group + sub) * d.out_head_stride;
+        T *out = static_cast<T *>(d.out) + (int64_t)(e.s.q0 + node) * d.out_stride + (int64_t)(e.h * p.group.d + sub) * d.out_head_stride;
         float *part = p.part_o + ((uint64_t)slot * kRows + tid) * d.head_dim;
         const bool spoilt = sh.spoilt[piece % 16] == piece + 1;
         if (__any_sync(~0u, valid)) {
@@ -845,19 +889,24 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
                         *reinterpret_cast<float4 *>(part + c + 4 * k) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                 }
             }
+            if (tid == 0 && e.t0 == 0 && !whole)
+                p.jobs[blockIdx.x] = {min(kRows, (int32_t)(e.s.nodes * p.group.d) - e.rt * kRows),
+                                      (int32_t)(1 + (e.n - e.t1 + sh.share - 1) / sh.share), (int32_t)slot, e.s.q0, e.h, e.rt * kRows};
             if (valid) {
                 if (!whole) {
                     float *ml = p.part_ml + ((uint64_t)slot * kRows + tid) * 2;
                     ml[0] = active ? from : -INFINITY;
                     ml[1] = active ? l : 0.f;
                 } else if (d.lse) {
-                    d.lse[(int64_t)(e.s.q0 + node) * d.num_heads + e.h * p.group + sub] =
+                    d.lse[(int64_t)(e.s.q0 + node) * d.num_heads + e.h * p.group.d + sub] =
                         active ? (from + log2f(l)) * kLn2 : -INFINITY;
                 }
             }
         }
         tmem_fence_before();
-        mbar_arrive(&sh.o_free);
+        __syncwarp();
+        if (tid % 32 == 0)
+            mbar_arrive(&sh.o_free);
     }
 }
 
@@ -901,49 +950,50 @@ __device__ void void_rows(const Params &p, const Seq &s)
     }
 }
 
-/* the CTA's piece [sh.lo, sh.hi) of the line, the sequence sh.b that lo lies in and its place sh.base */
+/* Counts the tiles of all sequences, kThreads at a time; the CTA's share of
+ * the line, and the sequence that it begins in, go to sh.line.  With more than
+ * kThreads sequences the search is a second walk. */
 template <typename T>
 __device__ void find_line(const Params &p, Shared &sh)
 {
     const kv_attn_desc &d = p.d;
-    int64_t all = 0;
-    for (int pass = 0; pass < 2; pass++) {
+    const bool once = d.num_seqs <= kThreads;
+    for (int walk = 0; walk < (once ? 1 : 2); walk++) {
         int64_t before = 0;
         for (uint32_t b0 = 0; b0 < d.num_seqs; b0 += kThreads) {
             const uint32_t b = b0 + threadIdx.x;
-            int64_t n = 0, sum;
+            uint64_t n = 0;
+            int64_t sum;
+            Seq s;
             if (b < d.num_seqs) {
-                Seq s;
                 if (sequence(d, b, s)) {
-                    n = head_tiles(s, p.group) * d.num_kv_heads;
-                } else if (pass == 0 && blockIdx.x == b % gridDim.x) {
+                    n = head_tiles(s, p.group);
+                } else if (walk == 0 && blockIdx.x == b % gridDim.x) {
                     atomicOr(d.error, KVATTN_ERR_SEQ);
                     void_rows<T>(p, s);
                 }
             }
-            const int64_t upto = before + block_scan(sh, n, sum);
-            if (pass == 0 && blockIdx.x == 0 && b < d.num_seqs)
-                p.prefix[b + 1] = upto;
-            if (pass == 1 && n && upto - n <= sh.lo && sh.lo < upto) {
-                sh.b = b;
-                sh.base = upto - n;
-            }
+            const int64_t all = (int64_t)(n * d.num_kv_heads), upto = before + block_scan(sh, all, sum);
             before += sum;
-        }
-        if (pass == 0) {
-            all = before;
-            if (threadIdx.x == 0) {
-                const int64_t share = max((int64_t)p.min_share, (all + gridDim.x - 1) / gridDim.x);
-                sh.lo = min(all, share * blockIdx.x);
-                sh.hi = min(all, share * (blockIdx.x + 1));
-                if (blockIdx.x == 0) {
-                    p.prefix[0] = 0;
-                    p.prefix[d.num_seqs + 1] = share;
+            if (once || (walk == 0 && b0 + kThreads >= d.num_seqs)) {
+                if (threadIdx.x == 0) {
+                    const int64_t grid = gridDim.x, share = before >> 31 ? (before + grid - 1) / grid
+                                                                         : ((uint32_t)before + gridDim.x - 1) / gridDim.x;
+                    sh.share = max((int64_t)p.min_share, share);
+                    sh.line.x = min(before, sh.share * blockIdx.x);
+                    sh.line.hi = min(before, sh.share * (blockIdx.x + 1));
                 }
+                __syncthreads();
+            }
+            if ((once || walk == 1) && n && upto - all <= sh.line.x && sh.line.x < upto) {
+                sh.line.b = b;
+                sh.line.base = upto - all;
+                sh.line.per_head = n;
+                sh.line.s = s;
             }
         }
-        __syncthreads();
     }
+    __syncthreads();
 }
 
 template <typename T, bool F8, int DP>
@@ -964,9 +1014,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(con
         for (int k = 0; k < 2; k++) {
             mbar_init(&sh.s_full[k], 1);
             mbar_init(&sh.o_done[k], 1);
-            mbar_init(&sh.p_full[k], kSoftmax);
+            mbar_init(&sh.p_full[k], kSoftmax / 32);
         }
-        mbar_init(&sh.o_free, kSoftmax);
+        mbar_init(&sh.o_free, kSoftmax / 32);
         mbar_init(&sh.q_full, kLoaders);
         mbar_init(&sh.q_empty, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -975,7 +1025,9 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(con
             sh.spoilt[k] = 0;
     }
     find_line<T>(p, sh);
-    if (sh.lo >= sh.hi)
+    if (threadIdx.x == 0)
+        p.jobs[blockIdx.x].rows = 0;
+    if (sh.line.x >= sh.line.hi)
         return;
     if (warp == kThreads / 32 - 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(S::kTmem) : "memory");
@@ -984,11 +1036,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(con
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    Line line;
-    line.x = sh.lo;
-    line.hi = sh.hi;
-    line.b = sh.b;
-    line.base = sh.base;
+    const Line line = sh.line;
     if (smem_u32(smem) % 1024 == 0) {
         if (warp < kSoftmax / 32) {
             softmax<T, F8, DP>(p, sh, ring, line);
@@ -1015,72 +1063,52 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(con
 }
 
 /* ------------------------------------------------------------------------
- * join: the pieces of a row tile that lies across CTAs.  CTA c looks at the
- * border between CTAs c - 1 and c of the line, and joins the row tile that it
- * cuts if that is its first cut.
+ * join: the pieces of a row tile that lies across CTAs, in their order.
  * ---------------------------------------------------------------------- */
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid_constant__ Params p)
 {
     const kv_attn_desc &d = p.d;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t share = p.prefix[d.num_seqs + 1], all = p.prefix[d.num_seqs], cut = share * (blockIdx.x + 1);
-    if (cut >= all)
+    const Job job = p.jobs[blockIdx.x];
+    const int32_t r0 = blockIdx.y * kJoinRows;
+    if (r0 >= job.rows)
         return;
-    uint32_t lo = 0, hi = d.num_seqs;           /* prefix[lo] <= cut < prefix[hi] */
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (p.prefix[mid] <= cut)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    Line line;
-    Piece e;
-    line.x = cut;
-    line.hi = cut + 1;
-    line.b = lo;
-    line.base = p.prefix[lo];
-    line.next(p, e);
-    const int64_t begin = cut - e.t0, end = begin + e.n;
-    if (e.t0 == 0 || begin < cut - share)
-        return;
-    const int32_t rows = (int32_t)min((int64_t)kRows, (int64_t)e.s.nodes * p.group - (int64_t)e.rt * kRows);
-    const int64_t c0 = begin / share, c1 = (end - 1) / share;
     const uint32_t quads = d.head_dim / 4;
     for (uint32_t x = threadIdx.x; x < kJoinRows * quads; x += kJoinThreads) {
-        const int32_t r = (int32_t)(blockIdx.y * kJoinRows + x / quads);
+        const int32_t r = r0 + (int32_t)(x / quads);
         const uint32_t c = x % quads * 4;
-        if (r >= rows)
+        if (r >= job.rows)
             return;
-        auto slot = [&](int64_t cta) { return (uint64_t)(2 * cta + (cta * share < begin)) * kRows + r; };
+        /* piece k's row: the first piece's slot, then slot 0 of the CTAs behind */
+        auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (blockIdx.x + k) : (uint32_t)job.slot) * kRows + r; };
         float m = -INFINITY, l = 0;
-        for (int64_t k = c0; k <= c1; k++) {
-            const float *ml = p.part_ml + slot(k) * 2;
-            if (ml[1] > 0 || ml[1] != ml[1])
-                m = fmaxf(m, ml[0]);
+#pragma unroll 4
+        for (int32_t k = 0; k < job.ctas; k++) {
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(k) * 2);
+            m = fmaxf(m, ml.y == 0 ? -INFINITY : ml.x);
         }
         float4 o = make_float4(0, 0, 0, 0);
-        for (int64_t k = c0; k <= c1; k++) {
-            const float *ml = p.part_ml + slot(k) * 2;
-            if (!(ml[1] > 0 || ml[1] != ml[1]))
-                continue;
-            const float f = exp2f(ml[0] - m);
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + slot(k) * d.head_dim + c);
-            l += f * ml[1];
+#pragma unroll 4
+        for (int32_t k = 0; k < job.ctas; k++) {
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(k) * 2);
+            if (ml.y == 0)
+                continue;               /* sees nothing there: its sums were not written */
+            const float f = exp2f(ml.x - m);
+            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at(k) * d.head_dim + c);
+            l += f * ml.y;
             o.x += f * v.x;
             o.y += f * v.y;
             o.z += f * v.z;
             o.w += f * v.w;
         }
-        const int64_t row = (int64_t)e.rt * kRows + r;
-        const int32_t node = (int32_t)(row / p.group), sub = (int32_t)(row - (int64_t)node * p.group);
+        const uint32_t q = job.row0 + r;
+        const int32_t node = (int32_t)fdiv(q, p.group), sub = (int32_t)(q - node * p.group.d);
         const float inv = l == 0 ? 0.f : d.v_scale / l;
-        T *out = static_cast<T *>(d.out) + (int64_t)(e.s.q0 + node) * d.out_stride + (int64_t)(e.h * p.group + sub) * d.out_head_stride;
-        uint2 w = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
-        *reinterpret_cast<uint2 *>(out + c) = w;
+        T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group.d + sub) * d.out_head_stride;
+        *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
         if (c == 0 && d.lse)
-            d.lse[(int64_t)(e.s.q0 + node) * d.num_heads + e.h * p.group + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
+            d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group.d + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
     }
 }
 
@@ -1114,7 +1142,7 @@ int grid_of(const kv_attn_desc *d)
 }
 
 struct Work {
-    uint64_t prefix, ml, o, bytes;
+    uint64_t jobs, ml, o, bytes;
 };
 
 Work workspace(const kv_attn_desc *d)
@@ -1122,8 +1150,8 @@ Work workspace(const kv_attn_desc *d)
     const uint64_t slots = 2ull * grid_of(d);
     auto up = [](uint64_t n) { return (n + 255) / 256 * 256; };
     Work w;
-    w.prefix = 0;
-    w.ml = up((d->num_seqs + 2ull) * sizeof(int64_t));
+    w.jobs = 0;
+    w.ml = up(slots / 2 * sizeof(Job));
     w.o = w.ml + up(slots * kRows * 2 * sizeof(float));
     w.bytes = w.o + slots * kRows * d->head_dim * sizeof(float);
     return w;
@@ -1150,7 +1178,7 @@ int launch(const Params &p, cudaStream_t stream)
     /* started while the first kernel drains; it waits for its results on the device */
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(grid - 1 ? grid - 1 : 1, kRows / kJoinRows);
+    cfg.gridDim = dim3(grid, kRows / kJoinRows);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1188,7 +1216,7 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
 {
     if (!desc_ok(d))
         return -EINVAL;
-    if (d->num_seqs > KVATTN_MAX_SEQS)
+    if (d->num_seqs > KVATTN_MAX_SEQS || (uint64_t)d->total_q * d->num_heads > KVATTN_MAX_QUERIES)
         return -E2BIG;
     if (!d->num_seqs || !d->total_q)
         return 0;
@@ -1206,14 +1234,15 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
     p.d = *d;
     p.stride = d->block_stride ? d->block_stride
                                : (uint64_t)d->block_size * d->num_kv_heads * d->head_dim * (d->kv_type == KVATTN_E4M3 ? 1 : 2);
-    p.group = d->num_heads / d->num_kv_heads;
+    p.group = make_fastdiv(d->num_heads / d->num_kv_heads);
+    p.block = make_fastdiv(d->block_size);
     /* a piece's sums, written and read, are 8 bytes a row and dimension against
      * 256 bytes a dimension of a 16-bit tile: a CTA takes enough tiles to be
      * worth that */
-    const uint64_t rows = (uint64_t)d->total_q * p.group / d->num_seqs;
+    const uint64_t rows = (uint64_t)d->total_q * p.group.d / d->num_seqs;
     p.min_share = 1 + (uint32_t)((rows < kRows ? rows : kRows) / 32);
     char *base = static_cast<char *>(d->workspace);
-    p.prefix = reinterpret_cast<int64_t *>(base + w.prefix);
+    p.jobs = reinterpret_cast<Job *>(base + w.jobs);
     p.part_ml = reinterpret_cast<float *>(base + w.ml);
     p.part_o = reinterpret_cast<float *>(base + w.o);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -30,6 +30,7 @@
  */
 #include "kvcopy.h"
 #include "adaptor.h"
+#include "fastdiv.h"
 
 #include <cuda_runtime.h>
 
@@ -52,30 +53,6 @@ constexpr uint32_t kTileVectors = 2048;
 struct WideShape { static constexpr int threads = 256, unroll = 8, min_blocks = 1; };
 struct NarrowShape { static constexpr int threads = 512, unroll = 4, min_blocks = 2; };
 constexpr uint32_t kNarrowUnitBytes = 1024;   /* units below this use NarrowShape */
-
-/* unsigned 32-bit division by a run-time constant: q = (umulhi(n, m) + n) >> s
- * with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1 (Granlund and
- * Montgomery, "Division by invariant integers using multiplication", 1994). */
-struct FastDiv {
-    uint32_t d, m, s;
-};
-
-FastDiv make_fastdiv(uint32_t d)
-{
-    FastDiv f;
-    uint32_t s = 0;
-    while ((1ull << s) < d)
-        s++;
-    f.d = d;
-    f.s = s;
-    f.m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
-    return f;
-}
-
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv &f)
-{
-    return (uint32_t)(((uint64_t)__umulhi(n, f.m) + n) >> f.s);
-}
 
 struct Params {
     const uint64_t *layer_k;

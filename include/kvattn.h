@@ -47,6 +47,7 @@ extern "C" {
 
 #define KVATTN_MAX_HEAD_DIM 256
 #define KVATTN_MAX_SEQS     65536
+#define KVATTN_MAX_QUERIES  (1u << 30)   /* total_q * num_heads */
 
 struct kv_attn_desc {
     const void *q;               /* [total_q][num_heads][head_dim], see the strides */
@@ -86,8 +87,8 @@ struct kv_attn_desc {
 int64_t kv_attn_workspace_bytes(const struct kv_attn_desc *desc);
 
 /* Asynchronous on `stream`, allocates nothing, may be captured.  Returns 0,
- * -EINVAL for a malformed descriptor, -E2BIG for more than KVATTN_MAX_SEQS
- * sequences, or -EIO when the launch failed. */
+ * -EINVAL for a malformed descriptor, -E2BIG past KVATTN_MAX_SEQS or
+ * KVATTN_MAX_QUERIES, or -EIO when the launch failed. */
 int kv_attn_launch(const struct kv_attn_desc *desc, void *stream);
 
 #ifdef __cplusplus
