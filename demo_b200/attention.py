@@ -46,6 +46,8 @@ class TreeAttention:
             raise ValueError("num_kv_heads must divide num_heads and the layout's width")
         if layout.element_size not in (1, 2):
             raise ValueError("caches of 1 or 2-byte elements")
+        if num_heads // num_kv_heads > 128:
+            raise ValueError("at most 128 query heads per K/V head")
         dim = layout.hidden_dim_size // num_kv_heads
         if layout.head_bytes and layout.head_bytes != dim * layout.element_size:
             raise ValueError("num_kv_heads does not fit the layout's head-major pages")
@@ -83,6 +85,8 @@ class TreeAttention:
                 q.shape[2] != self.head_dim or q.stride(2) != 1:
             raise ValueError(f"q: expected a bfloat16 or float16 CUDA tensor [total, {self.num_heads}, {self.head_dim}]")
         dev, total = q.device, q.shape[0]
+        if 0 in q.stride():                             # an expanded tensor
+            q = q.contiguous()
         if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.device != dev or \
                 block_table.shape[1] < 1 or block_table.stride(1) != 1:
             raise ValueError(f"block_table: expected an int32 tensor [rows, width] on {dev} with contiguous rows")
@@ -108,8 +112,9 @@ class TreeAttention:
         d.parents = _int32("parents", parents, dev, total) if parents is not None else None
         d.error = error.data_ptr()
         d.table_stride = block_table.stride(0) if n_rows > 1 else width
-        d.q_stride, d.q_head_stride = q.stride(0), q.stride(1)
-        d.out_stride, d.out_head_stride = out.stride(0), out.stride(1)
+        row = self.num_heads * self.head_dim            # a stride of one row or one head means nothing
+        d.q_stride, d.out_stride = (q.stride(0), out.stride(0)) if total > 1 else (row, row)
+        d.q_head_stride, d.out_head_stride = (q.stride(1), out.stride(1)) if self.num_heads > 1 else (row, row)
         d.width, d.num_rows, d.num_seqs, d.total_q = width, n_rows, seqs, total
         d.q_type = _TYPES[q.dtype]
         d.kv_type = _lib.KVATTN_E4M3 if self.layout.element_size == 1 else d.q_type

@@ -2,38 +2,38 @@
  * Attention over a paged KV cache for drafted trees, chains and single tokens
  * (include/kvattn.h), sm_100a.
  *
- * A K/V head of a sequence serves rows = nodes x (query heads per K/V head)
- * query rows, in tiles of 128.  Per 64 positions of the context a CTA computes
+ * A K/V head of a sequence serves nodes x (query heads per K/V head) query
+ * rows, in tiles of whole nodes, at most 128 rows.  Per 128 positions of the
+ * context a CTA computes
  *
- *   S = Q K^T        128 x 64, tcgen05.mma, Q and K in shared memory, S in TMEM
+ *   S = Q K^T        128 x 128, tcgen05.mma, Q and K in shared memory, S in TMEM
  *   P = exp2(S - m)  one thread per row, the running maximum and sum in 32 bits
  *   O += P V         128 x dim, tcgen05.mma, P in TMEM (where S was), V in shared
  *
- * Bound: with up to about 200 rows, reading K and V once from HBM; a tile of
- * 64 positions is 32 KiB at 16 bits and dim 128, about 1400 cycles of an SM's
- * share of the bandwidth, and its products take 524 cycles of the tensor cores
- * even with 128 rows of which one is a query.  So one form serves single
- * tokens and trees alike.  Two CTAs share an SM: one's softmax runs beside the
- * other's products.
+ * Bound: with up to about 200 rows, reading K and V once from HBM: a tile of
+ * 128 positions is 64 KiB at 16 bits and dim 128, about 2800 cycles of an SM's
+ * share of the bandwidth, while its products take 1024 cycles of the tensor
+ * cores even if only one of the 128 rows is a query, and its exponentials at
+ * most as long.  So one form serves single tokens and trees alike.  Two CTAs
+ * share an SM: one's softmax runs beside the other's products and loads.
  *
- * A CTA has 9 warps: 0-3 softmax (a thread owns a TMEM lane, a row), 4-7
- * loaders (pages of any size and order, 16 bytes at a time, straight into the
- * 128-byte swizzle that the products read; 8-bit caches are widened on the
- * way), 8 issues the products.  They meet at mbarriers: a ring of K and V
- * slots, two S buffers (S of the next tile is computed under this tile's
- * softmax), and O.  Every wait is bounded.
+ * Warps 0-3 are the softmax (a thread owns a TMEM lane, a row), then come the
+ * loaders, the last warp issues the products.  They meet at mbarriers: a ring
+ * of slots of 128 positions x 64 values of K or V, S and P, and O.  Every wait
+ * is bounded.
  *
  * The (sequence, K/V head, row tile, position tile) quadruples of a call lie on
- * one line, and each CTA takes an equal piece of it, wherever that ends inside a
+ * one line, and each CTA takes an equal part of it, wherever that ends inside a
  * context: ragged batches and a single long row fill the GPU alike, and the
  * lengths are read on the device.  Pieces of a row tile are joined by a second
- * kernel, in order, so results do not depend on timing.
+ * kernel, in a fixed order, so results do not depend on timing.
  */
 #include "kvattn.h"
 #include "adaptor.h"
 #include "device_guard.h"
 #include "fastdiv.h"
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -47,40 +47,58 @@
 namespace {
 
 constexpr int kRows = 128;          /* query rows of a tile: TMEM lanes */
-constexpr int kTile = 64;           /* positions of a tile */
-constexpr int kSoftmax = 128;       /* threads of each role */
-constexpr int kLoaders = 128;
-constexpr int kThreads = kSoftmax + kLoaders + 32;
+constexpr int kTile = 128;          /* positions of a tile */
+constexpr int kColumn = 64;         /* values of a row in a slot: 128 bytes, the swizzle's width */
+constexpr int kSlotBytes = kTile * kColumn * 2;
+constexpr int kSoftmax = 128;       /* threads of the softmax */
+
+/* how K and V come: by TMA (16-bit caches whose pages divide into boxes of 8 or
+ * more rows), by 16-byte copies (16-bit caches of any other page size), or by
+ * 16-byte copies that are widened (8-bit caches) */
+enum Load { kTma, kCopy, kWiden };
+template <Load L> struct Roles {
+    static constexpr int kLoaders = L == kTma ? 32 : 128;
+    static constexpr int kThreads = kSoftmax + kLoaders + 32;
+};
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 16;       /* rows of one joining CTA */
+constexpr int kJoinPieces = 64;     /* pieces that it looks at together */
 constexpr uint32_t kSpinLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-/* DP: head_dim rounded up to whole 128-byte columns (64 values) */
-template <int DP> struct Shape {
+/* DP: head_dim rounded up to whole columns, of which K, V and Q are made */
+template <Load L, int DP> struct Shape {
     static constexpr int kCtas = DP <= 128 ? 2 : 1;                 /* per SM */
-    static constexpr int kSlots = DP == 64 ? 8 : DP == 128 ? 5 : 4; /* K and V tiles in the ring */
-    static constexpr int kSlotBytes = kTile * DP * 2;
+    static constexpr int kRaw = L == kWiden ? 4 : 0;                /* slots of 8-bit values on their way */
+    static constexpr int kSlots = DP == 64 ? (kRaw ? 4 : 6) : DP == 128 ? (kRaw ? 3 : 5) : (kRaw ? 8 : 10);
     static constexpr int kQBytes = kRows * DP * 2;
-    static constexpr int kTmem = DP <= 128 ? 256 : 512;             /* columns: 2 x 64 of S, then O */
-    static constexpr int kSmem = kQBytes + kSlots * kSlotBytes + 1024;
+    static constexpr int kTmem = DP <= 128 ? 256 : 512;             /* columns: 128 of S, then O */
+    static constexpr int kShared = kQBytes + kSlots * kSlotBytes + kRaw * kSlotBytes / 2;   /* where struct Shared stands */
+    static constexpr int kSmem = kShared + 1024;
+    static_assert(kSlots > DP / kColumn, "V of a tile, and one more");
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "the CTAs of an SM share its shared memory");
-    static_assert(2 * kTile + DP <= kTmem && kCtas * kTmem <= 512, "and its TMEM");
+    static_assert(kTile + DP <= kTmem && kCtas * kTmem <= 512, "and its TMEM");
 };
 
 /* a row tile that lies across CTAs: its first piece is the last of CTA c (in
  * that CTA's place `slot`), the others are the first of CTAs c + 1 .. */
 struct Job {
-    int32_t rows, ctas, slot, q0, h, row0;
+    int32_t rows, ctas, slot, q0, h;
 };
 
 struct Params {
+    CUtensorMap q_map;      /* [queries][heads][dim], boxes of 64 values x the rows of a tile */
+    CUtensorMap k_map, v_map;   /* kTma: [pages][kv heads][block][dim], boxes of 64 values x `box` rows */
     kv_attn_desc d;
     uint64_t stride;        /* bytes from page to page */
-    FastDiv group;          /* query heads per K/V head */
     FastDiv block;          /* positions of a page */
+    FastDiv nodes;          /* nodes of a row tile */
+    uint32_t group;         /* query heads per K/V head */
+    uint32_t columns;       /* of Q, K and V */
+    uint32_t box;
     uint32_t min_share;     /* tiles that a CTA takes at least */
-    struct Job *jobs;       /* workspace: [CTAs] row tiles to be joined, by the CTA that has their first tiles */
+    uint32_t join_ctas;     /* that join a row tile */
+    Job *jobs;              /* workspace: [CTAs] row tiles to be joined, by the CTA that has their first tiles */
     float *part_ml;         /* [2 * CTAs][128][2] maximum and sum of a piece */
     float *part_o;          /* [2 * CTAs][128][dim] */
 };
@@ -115,36 +133,33 @@ __device__ __forceinline__ bool node_ok(const int32_t *parents, int32_t j)
     return u >= -1 && u < j;
 }
 
-__device__ __forceinline__ int32_t row_tiles(const Seq &s, const FastDiv &group)
-{
-    return (int32_t)((s.nodes * group.d + kRows - 1) / kRows);
-}
-
 /* positions that row tile rt's nodes may see: parents come before their nodes */
-__device__ __forceinline__ int32_t visible_end(const Seq &s, const FastDiv &group, int32_t rt)
+__device__ __forceinline__ int32_t visible_end(const Params &p, const Seq &s, int32_t rt)
 {
-    return s.ctx + min(s.nodes, (int32_t)fdiv((uint32_t)(rt + 1) * kRows - 1, group) + 1);
+    return s.ctx + min(s.nodes, (rt + 1) * (int32_t)p.nodes.d);
 }
 
-__device__ __forceinline__ int32_t tiles_of(const Seq &s, const FastDiv &group, int32_t rt)
+__device__ __forceinline__ uint32_t tiles_of(const Params &p, const Seq &s, int32_t rt)
 {
-    return (visible_end(s, group, rt) + kTile - 1) / kTile;
+    return ((uint32_t)visible_end(p, s, rt) + kTile - 1) / kTile;
 }
 
 /* tiles of one K/V head of the sequence, all row tiles */
-__device__ __forceinline__ uint64_t head_tiles(const Seq &s, const FastDiv &group)
+__device__ __forceinline__ uint64_t head_tiles(const Params &p, const Seq &s)
 {
     uint64_t n = 0;
-    for (int32_t rt = 0; rt < row_tiles(s, group); rt++)
-        n += tiles_of(s, group, rt);
+    for (int32_t rt = 0; rt * (int32_t)p.nodes.d < s.nodes; rt++)
+        n += tiles_of(p, s, rt);
     return n;
 }
 
 /* a run of tiles of one row tile */
 struct Piece {
-    Seq s;
-    int32_t h, rt, t0, t1, n;       /* tiles t0 .. t1 of n */
+    int32_t q0, nodes, ctx, row;    /* the sequence's */
+    int32_t h, node0, end;          /* K/V head, first node, positions that the nodes may see */
+    int32_t t0, t1, n;              /* tiles t0 .. t1 of n */
     __device__ bool whole() const { return t0 == 0 && t1 == n; }
+    __device__ int32_t rows(const Params &p) const { return min(nodes - node0, (int32_t)p.nodes.d) * (int32_t)p.group; }
 };
 
 struct Line {
@@ -160,19 +175,26 @@ struct Line {
         while (x >= base + (int64_t)(per_head * p.d.num_kv_heads)) {
             base += (int64_t)(per_head * p.d.num_kv_heads);
             b++;
-            per_head = sequence(p.d, b, s) ? head_tiles(s, p.group) : 0;
+            per_head = sequence(p.d, b, s) ? head_tiles(p, s) : 0;
         }
         uint64_t y = x - base;
         e.h = (int32_t)((y | per_head) >> 32 ? y / per_head : (uint32_t)y / (uint32_t)per_head);
         y -= e.h * per_head;
-        e.rt = 0;
-        for (e.n = tiles_of(s, p.group, 0); y >= (uint64_t)e.n; e.n = tiles_of(s, p.group, e.rt)) {
-            y -= e.n;
-            e.rt++;
+        int32_t rt = 0;
+        uint32_t n;
+        for (n = tiles_of(p, s, 0); y >= n; n = tiles_of(p, s, rt)) {
+            y -= n;
+            rt++;
         }
-        e.s = s;
+        e.q0 = s.q0;
+        e.nodes = s.nodes;
+        e.ctx = s.ctx;
+        e.row = s.row;
+        e.node0 = rt * (int32_t)p.nodes.d;
+        e.end = visible_end(p, s, rt);
+        e.n = (int32_t)n;
         e.t0 = (int32_t)y;
-        e.t1 = (int32_t)min((int64_t)e.n, (int64_t)y + (hi - x));
+        e.t1 = (int32_t)min((int64_t)n, (int64_t)y + (hi - x));
         x += e.t1 - e.t0;
         return true;
     }
@@ -202,20 +224,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
 }
 
 struct Shared {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], o_done[2], o_free, q_full, q_empty;
+    uint64_t full[10], empty[10];   /* slots */
+    uint64_t s_full, p_full[2];     /* S of a tile; P of its first and second 64 positions */
+    uint64_t o_done, o_free;        /* O of a piece is complete; has been read */
+    uint64_t q_full, q_empty;
     uint32_t tmem;
     volatile uint32_t dead;         /* a wait ran out: every role leaves */
-    int64_t share, scan[kThreads / 32];
+    volatile uint32_t spoilt[4];    /* [piece % 4] == piece + 1: values of its fed nodes that are not finite were set aside */
+    int64_t share, scan[Roles<kCopy>::kThreads / 32];
     Line line;                      /* the CTA's part of it */
-    volatile uint32_t spoilt[16];   /* [piece % 16] == piece + 1: values of its fed nodes that are not finite were set aside */
 };
 static_assert(sizeof(Shared) <= 1024, "the last KiB of the dynamic shared memory");
 
-/* Waits for the phase of `parity`, about a second at most.  A parity tells a
- * phase from the one before and the one after only.  Softmax does not wait for
- * every O: O is done at two barriers in turn, so that where it waits for one,
- * the one before at that barrier is known to be done (S of a tile is issued
- * behind O of the tile two before) and the one after is not yet issued. */
+/* waits for the phase of `parity`, about a second at most */
 __device__ bool wait(Shared &sh, int32_t *error, uint64_t *bar, uint32_t parity)
 {
     for (uint32_t i = 0;; i++) {
@@ -239,6 +260,19 @@ __device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint64_t *
     return __all_sync(~0u, wait(sh, error, bar, parity));
 }
 
+/* One lane of a converged warp.  What the tensor cores and the TMA are given
+ * lives in uniform registers: the issuing warps run their loops as a whole and
+ * leave only the instruction itself to one lane (with the whole loop in a
+ * lane's branch each product took 80 cycles to issue, each load 160). */
+__device__ __forceinline__ bool elect()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __shfl_sync(~0u, x, 0); }
+
 /* shared-memory matrix descriptor, 128-byte swizzle: the low word (where it
  * starts, and the bytes between 64-value columns of an operand stored row by
  * row) and the high word, which is the same for all here (1024 bytes from one
@@ -248,6 +282,7 @@ __device__ __forceinline__ uint32_t matrix(uint32_t addr, uint32_t lead)
     return (addr >> 4 & 0x3fff) | (lead >> 4 & 0x3fff) << 16;
 }
 constexpr uint32_t kMatrixHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
+constexpr uint32_t kNoLead = 16;    /* operands of one column, or stored k innermost */
 
 /* instruction descriptor of kind::f16: 128 rows, n columns, 32-bit sums; b_rows: B is stored row by row (k outermost) */
 __device__ __forceinline__ uint32_t instruction(uint32_t bf16, uint32_t n, uint32_t b_rows)
@@ -364,61 +399,138 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16u : 0u) : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+/* all but this thread's N last groups have landed */
+template <int N> __device__ __forceinline__ void copy_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 /* arrive at `bar` when this thread's copies so far have landed */
 __device__ __forceinline__ void copy_arrive(uint64_t *bar)
 {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-/* what this thread has seen written to shared memory, before the products it issues */
+/* what this thread has written to shared memory, or seen written, comes before the products behind it */
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-/* where chunk c (16 bytes) of row r stands in a tile of `rows` rows: 128-byte columns, swizzled */
-__device__ __forceinline__ uint32_t swizzled(uint32_t rows, uint32_t r, uint32_t c)
+__device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes)
 {
-    return (c >> 3) * rows * 128 + r * 128 + ((c ^ r) & 7) * 16;
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+}
+
+/* where chunk c (16 bytes) of row r stands in a slot */
+__device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c)
+{
+    return r * (kColumn * 2) + ((c ^ r) & 7) * 16;
 }
 
 /* ------------------------------------------------------------------------
- * loaders: slot 2 g is K of the CTA's tile g, slot 2 g + 1 its V; Q comes with
- * the first K of a piece.
+ * loaders: for each tile the columns of K, then those of V, a slot each.
  * ---------------------------------------------------------------------- */
-template <typename T, bool F8, int DP> struct Loader {
-    using S = Shape<DP>;
-    static constexpr int kChunks = F8 ? DP / 16 : DP / 8;       /* 16-byte loads of a cached row */
-    static constexpr int kPass = kLoaders / kChunks;            /* rows of one pass */
+/* a place in the ring, and how often the ring has been gone around */
+template <int N> struct Turn {
+    uint32_t slot = 0, lap = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++slot == N) {
+            slot = 0;
+            lap++;
+        }
+    }
+};
+
+template <typename T, Load L, int DP> struct Loader {
+    using S = Shape<L, DP>;
+    static constexpr bool F8 = L == kWiden;
+    enum : uint64_t { kNone = ~0ull };
+    static constexpr int kChunks = F8 ? 4 : 8;                  /* 16-byte loads of a row of a slot */
+    static constexpr int kPass = 128 / kChunks;                 /* rows of one pass */
     static constexpr int kPasses = kTile / kPass;
-    static constexpr int kWarpRows = kPass / (kLoaders / 32);   /* of them a warp's */
-    static constexpr int kQChunks = DP / 8, kQPass = kLoaders / kQChunks;
-    static_assert(kPasses * kWarpRows == 16, "a lane of each half warp looks after one of the warp's rows");
+    static constexpr int kWarpRows = kPass / 4;                 /* of them a warp's */
+    static_assert(kPasses * kWarpRows == 32, "a lane looks after one of the warp's rows");
 
     const Params &p;
     Shared &sh;
-    uint8_t *q_smem, *ring;
+    uint8_t *ring;
+    Turn<S::kSlots> at;
+
+    __device__ Loader(const Params &p_, Shared &sh_, uint8_t *ring_) : p(p_), sh(sh_), ring(ring_) {}
+
+    __device__ __forceinline__ uint8_t *slot() const { return ring + at.slot * kSlotBytes; }
+
+    /* the slot may be written; the lanes go on together or not at all */
+    __device__ __forceinline__ bool acquire() { return wait_warp(sh, p.d.error, &sh.empty[at.slot], at.lap & 1 ^ 1); }
+
+    /* Boxes of a page's rows by a column; a lane looks up its box's page.  Rows behind the end, and those of padding nodes, hold
+     * anything: their scores are masked, and softmax makes their values finite.
+     * A page id out of range is out of the map: zeros. */
+    __device__ void run_tma(Line line)
+    {
+        const uint32_t lane = threadIdx.x % 32, boxes = kTile / p.box, box_bytes = p.box * (kColumn * 2);
+        Piece e;
+        while (line.next(p, e)) {
+            const int32_t *tab = p.d.table + (int64_t)e.row * p.d.table_stride;
+            const int32_t t1 = uniform(e.t1), end = uniform(e.end), h = uniform(e.h);
+            int32_t pos = e.t0 * kTile + (int32_t)(lane * p.box);
+            int32_t next = lane < boxes && pos < e.end ? tab[fdiv(pos, p.block)] : 0;
+            for (int32_t t = uniform(e.t0); t < t1; t++) {
+                const int32_t page = next;
+                /* a page of more than 128 rows holds several tiles */
+                const int32_t first = uniform(boxes == 1 ? pos - (int32_t)(fdiv(pos, p.block) * p.block.d) : 0);
+                const uint32_t n = min(boxes, (end - t * kTile + p.box - 1) / p.box);
+                if (lane < n && (uint32_t)page >= p.d.num_pages)
+                    atomicOr(p.d.error, KVATTN_ERR_PAGE);
+                pos += kTile;
+                if (t + 1 < t1)
+                    next = lane < boxes && pos < e.end ? tab[fdiv(pos, p.block)] : 0;   /* in flight while the tile is loaded */
+                for (uint32_t x = 0; x < 2 * p.columns; x++, at.next()) {
+                    if (!acquire())
+                        return;
+                    uint64_t *bar = &sh.full[at.slot];
+                    const CUtensorMap *map = x < p.columns ? &p.k_map : &p.v_map;
+                    const int32_t column = (int32_t)(x < p.columns ? x : x - p.columns) * kColumn;
+                    uint32_t to = smem_u32(slot());
+                    if (elect())
+                        mbar_expect(bar, n * box_bytes);
+                    __syncwarp();
+                    for (uint32_t b = 0; b < n; b++, to += box_bytes) {
+                        const int32_t id = __shfl_sync(~0u, page, b);
+                        if (elect())
+                            tma_load(to, map, column, first, h, id, bar);
+                    }
+                }
+            }
+        }
+    }
+
+    /* ---- 16 bytes at a time: pages of any size ---- */
     uint32_t chunk, row;                /* this thread's chunk, and row of a pass */
     uint32_t own_row;                   /* the row of a tile whose place this lane works out */
-    uint32_t tok_bytes;
-    bool in_dim;
     uint64_t off[kPasses];              /* of this thread's rows in the planes, kNone: read as zeros */
-    bool q_due = false;                 /* Q of the piece is still to be loaded */
-    static constexpr uint64_t kNone = ~0ull;
 
-    __device__ Loader(const Params &p_, Shared &sh_, uint8_t *q_, uint8_t *ring_) : p(p_), sh(sh_), q_smem(q_), ring(ring_)
+    __device__ void take_rows()
     {
         const uint32_t t = threadIdx.x - kSoftmax, lane = t % 32, warp = t / 32;
         chunk = t % kChunks;
         row = t / kChunks;
-        own_row = lane % 16 / kWarpRows * kPass + warp * kWarpRows + lane % kWarpRows;
-        in_dim = chunk * (F8 ? 16 : 8) < p.d.head_dim;
-        tok_bytes = (p.d.head_major ? 1 : p.d.num_kv_heads) * p.d.head_dim * (F8 ? 1 : 2);
+        own_row = lane / kWarpRows * kPass + warp * kWarpRows + lane % kWarpRows;
     }
 
     /* the page of this lane's row of tile t: a load that waits for nothing */
     __device__ int32_t look_up(const Piece &e, int32_t t) const
     {
         const uint32_t pos = t * kTile + own_row;
-        const int32_t *tab = p.d.table + (int64_t)e.s.row * p.d.table_stride;
-        return (int32_t)pos < visible_end(e.s, p.group, e.rt) ? tab[fdiv(pos, p.block)] : -1;
+        return (int32_t)pos < e.end ? p.d.table[(int64_t)e.row * p.d.table_stride + fdiv(pos, p.block)] : -1;
     }
 
     /* The places of the thread's rows: each lane works out one, the threads of
@@ -426,16 +538,16 @@ template <typename T, bool F8, int DP> struct Loader {
     __device__ void places(const Piece &e, int32_t t, int32_t page)
     {
         const kv_attn_desc &d = p.d;
-        const uint32_t pos = t * kTile + own_row, j = pos - fdiv(pos, p.block) * p.block.d;
-        const bool here = (int32_t)pos < visible_end(e.s, p.group, e.rt);
+        const uint32_t pos = t * kTile + own_row, j = pos - fdiv(pos, p.block) * p.block.d, esz = F8 ? 1 : 2;
         uint64_t own = kNone;
-        if (here) {
+        if ((int32_t)pos < e.end) {
             if ((uint32_t)page < d.num_pages)
-                own = (uint64_t)(uint32_t)page * p.stride + (uint64_t)j * tok_bytes +
-                      (uint64_t)(d.head_major ? d.block_size : 1) * d.head_dim * (F8 ? 1 : 2) * e.h;
+                own = (uint64_t)(uint32_t)page * p.stride +
+                      ((uint64_t)j * (d.head_major ? 1 : d.num_kv_heads) + (uint64_t)(d.head_major ? d.block_size : 1) * e.h) *
+                          (d.head_dim * esz);
             else
                 atomicOr(d.error, KVATTN_ERR_PAGE);
-            if (d.parents && (int32_t)pos >= e.s.ctx && !node_ok(d.parents + e.s.q0, pos - e.s.ctx))
+            if (d.parents && (int32_t)pos >= e.ctx && !node_ok(d.parents + e.q0, pos - e.ctx))
                 own = kNone;            /* padding nodes are not read */
         }
         const uint32_t from = threadIdx.x % 32 / kChunks;
@@ -444,233 +556,199 @@ template <typename T, bool F8, int DP> struct Loader {
             off[i] = __shfl_sync(~0u, own, i * kWarpRows + from);
     }
 
-    /* pass i's address in a plane (its start, for rows that are zeros) */
-    __device__ const void *address(const void *plane, int i) const
+    /* this thread's share of column c of K (v = 0) or V, asynchronously, row r of a pass going to at(pass) */
+    template <typename F> __device__ __forceinline__ void copy_column(uint32_t v, uint32_t c, F place)
     {
-        return static_cast<const char *>(plane) + (off[i] == kNone ? 0 : off[i] + chunk * 16);
+        const uint32_t x = c * (F8 ? kColumn : kColumn * 2) + chunk * 16;
+        const char *plane = static_cast<const char *>(v ? p.d.v : p.d.k);
+        if (x >= p.d.head_dim * (F8 ? 1 : 2))
+            return;
+#pragma unroll
+        for (int i = 0; i < kPasses; i++)
+            copy16(place(i), plane + (off[i] == kNone ? 0 : off[i] + x), off[i] != kNone);
     }
 
-    /* Q of the piece, once the products of the piece before have read theirs;
-     * false if that is not yet so (or, with `block`, will not be) */
-    __device__ bool load_q(const Piece &e, uint32_t piece, bool block)
+    __device__ void run_copy(Line line)
     {
-        if (piece) {
-            const uint32_t parity = (piece - 1) & 1;
-            if (!(block ? wait(sh, p.d.error, &sh.q_empty, parity) : mbar_try_wait(&sh.q_empty, parity)))
-                return false;
-        }
-        const uint32_t t = threadIdx.x - kSoftmax, c = t % kQChunks;
-        const int32_t rows = (int32_t)(e.s.nodes * p.group.d) - e.rt * kRows;
-        if (c * 8 < p.d.head_dim)
-            for (uint32_t r = t / kQChunks; r < kRows && (int32_t)r < rows; r += kQPass) {
-                const uint32_t x = e.rt * kRows + r, node = fdiv(x, p.group), g = x - node * p.group.d;
-                const T *src = static_cast<const T *>(p.d.q) + (int64_t)(e.s.q0 + node) * p.d.q_stride +
-                               (int64_t)(e.h * p.group.d + g) * p.d.q_head_stride + c * 8;
-                copy16(smem_u32(q_smem) + swizzled(kRows, r, c), src, true);
-            }
-        copy_arrive(&sh.q_full);
-        q_due = false;
-        return true;
-    }
-
-    /* slot i for writing; Q, if due, goes first where it need not be waited
-     * for, or where the ring is full */
-    __device__ bool acquire(uint32_t i, const Piece &e, uint32_t piece)
-    {
-        uint64_t *bar = &sh.empty[i % S::kSlots];
-        const uint32_t parity = ((i / S::kSlots) & 1) ^ 1;
-        bool ok = true;
-        if (q_due && !load_q(e, piece, false) && !mbar_try_wait(bar, parity))
-            ok = load_q(e, piece, true);
-        return __all_sync(~0u, ok && wait(sh, p.d.error, bar, parity));
-    }
-
-    __device__ uint8_t *slot(uint32_t i) const { return ring + (i % S::kSlots) * S::kSlotBytes; }
-
-    /* 16-bit caches: asynchronous copies, the ring's depth in flight */
-    __device__ void run16(Line line)
-    {
-        uint32_t i = 0, piece = 0;
+        take_rows();
         Piece e;
-        for (; line.next(p, e); piece++) {
-            q_due = true;
+        while (line.next(p, e)) {
             int32_t page = look_up(e, e.t0);
             for (int32_t t = e.t0; t < e.t1; t++) {
                 places(e, t, page);
                 if (t + 1 < e.t1)
                     page = look_up(e, t + 1);       /* in flight while the tile is copied */
-                for (int v = 0; v < 2; v++, i++) {
-                    if (!acquire(i, e, piece))
+                for (uint32_t x = 0; x < 2 * p.columns; x++, at.next()) {
+                    if (!acquire())
                         return;
-                    const void *plane = v ? p.d.v : p.d.k;
-                    const uint32_t to = smem_u32(slot(i));
-                    if (in_dim)
-#pragma unroll
-                        for (int x = 0; x < kPasses; x++)
-                            copy16(to + swizzled(kTile, row + x * kPass, chunk), address(plane, x), off[x] != kNone);
-                    copy_arrive(&sh.full[i % S::kSlots]);
+                    const uint32_t to = smem_u32(slot());
+                    copy_column(x >= p.columns, x < p.columns ? x : x - p.columns,
+                                [&](int i) { return to + swizzled(row + i * kPass, chunk); });
+                    copy_arrive(&sh.full[at.slot]);
                 }
             }
-            if (!__all_sync(~0u, !q_due || load_q(e, piece, true)))
-                return;
         }
     }
 
-    /* 8-bit caches: through registers, one tile ahead */
-    __device__ void fetch(uint4 *k, uint4 *v)
+    /* 8-bit caches: copied as they are, kRaw - 1 slots ahead, to places in
+     * shared memory that only the copying thread uses; that thread widens them
+     * into the ring. */
+    __device__ __forceinline__ uint8_t *raw(uint32_t k, int i) const
     {
+        return ring + S::kSlots * kSlotBytes + (k % S::kRaw) * (kSlotBytes / 2) + i * (128 * 16) + (threadIdx.x - kSoftmax) * 16;
+    }
+
+    __device__ bool widen(uint32_t k, uint32_t c)
+    {
+        if (!acquire())
+            return false;
+        if (c * kColumn + chunk * 16 < p.d.head_dim)
 #pragma unroll
-        for (int x = 0; x < kPasses; x++) {
-            k[x] = v[x] = make_uint4(0, 0, 0, 0);
-            if (in_dim && off[x] != kNone) {
-                k[x] = __ldg(static_cast<const uint4 *>(address(p.d.k, x)));
-                v[x] = __ldg(static_cast<const uint4 *>(address(p.d.v, x)));
+            for (int i = 0; i < kPasses; i++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(raw(k, i));
+                const uint32_t r = row + i * kPass;
+                *reinterpret_cast<uint4 *>(slot() + swizzled(r, 2 * chunk)) =
+                    make_uint4(Type<T>::widen((uint16_t)w.x), Type<T>::widen((uint16_t)(w.x >> 16)),
+                               Type<T>::widen((uint16_t)w.y), Type<T>::widen((uint16_t)(w.y >> 16)));
+                *reinterpret_cast<uint4 *>(slot() + swizzled(r, 2 * chunk + 1)) =
+                    make_uint4(Type<T>::widen((uint16_t)w.z), Type<T>::widen((uint16_t)(w.z >> 16)),
+                               Type<T>::widen((uint16_t)w.w), Type<T>::widen((uint16_t)(w.w >> 16)));
             }
-        }
+        mbar_arrive(&sh.full[at.slot]);
+        at.next();
+        return true;
     }
 
-    __device__ void put(uint32_t i, const uint4 *raw)
+    __device__ void run_widen(Line line)
     {
-        if (in_dim)
-#pragma unroll
-            for (int x = 0; x < kPasses; x++) {
-                const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw[x]);
-                uint32_t o[8];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    o[2 * k] = Type<T>::widen((uint16_t)w[k]);
-                    o[2 * k + 1] = Type<T>::widen((uint16_t)(w[k] >> 16));
+        constexpr uint32_t kAhead = S::kRaw > 0 ? S::kRaw - 1 : 0;
+        take_rows();
+        uint32_t k = 0, done = 0, c = 0;    /* slots fetched, widened, and the column of the next to be widened */
+        Piece e;
+        auto finish = [&] {
+            const uint32_t mine = c;
+            c = c + 1 == p.columns ? 0 : c + 1;
+            return widen(done++, mine);
+        };
+        while (line.next(p, e)) {
+            int32_t page = look_up(e, e.t0);
+            for (int32_t t = e.t0; t < e.t1; t++) {
+                places(e, t, page);
+                if (t + 1 < e.t1)
+                    page = look_up(e, t + 1);
+                for (uint32_t x = 0; x < 2 * p.columns; x++, k++) {
+                    copy_column(x >= p.columns, x < p.columns ? x : x - p.columns, [&](int i) { return smem_u32(raw(k, i)); });
+                    copy_commit();
+                    if (k >= kAhead) {
+                        copy_wait_but<kAhead>();
+                        if (!finish())
+                            return;
+                    }
                 }
-                uint8_t *to = slot(i);
-                *reinterpret_cast<uint4 *>(to + swizzled(kTile, row + x * kPass, 2 * chunk)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4 *>(to + swizzled(kTile, row + x * kPass, 2 * chunk + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
-            }
-        mbar_arrive(&sh.full[i % S::kSlots]);
-    }
-
-    __device__ void run8(Line line)
-    {
-        Piece now, then;
-        uint4 k[kPasses], v[kPasses], k2[kPasses], v2[kPasses];
-        if (!line.next(p, now))
-            return;
-        int32_t t = now.t0, page = look_up(now, t);
-        places(now, t, page);
-        if (t + 1 < now.t1)
-            page = look_up(now, t + 1);
-        fetch(k, v);
-        uint32_t piece = 0, i = 0;
-        q_due = true;
-        for (bool more = true; more;) {
-            const bool last = t + 1 >= now.t1;
-            bool moved = false;
-            if (last)
-                more = moved = line.next(p, then);
-            if (more) {
-                const Piece &e = moved ? then : now;
-                const int32_t u = moved ? then.t0 : t + 1;
-                if (moved)
-                    page = look_up(e, u);
-                places(e, u, page);
-                if (u + 1 < e.t1)
-                    page = look_up(e, u + 1);
-                fetch(k2, v2);
-            }
-            if (!acquire(i, now, piece))
-                return;
-            put(i++, k);
-            if (!acquire(i, now, piece))
-                return;
-            put(i++, v);
-            if (!__all_sync(~0u, !last || !q_due || load_q(now, piece, true)))
-                return;
-#pragma unroll
-            for (int x = 0; x < kPasses; x++) {
-                k[x] = k2[x];
-                v[x] = v2[x];
-            }
-            if (moved) {
-                now = then;
-                t = now.t0;
-                piece++;
-                q_due = true;
-            } else {
-                t++;
             }
         }
+        copy_wait_all();
+        while (done < k)
+            if (!finish())
+                return;
     }
 };
 
 /* ------------------------------------------------------------------------
- * products: S of tile g + 1 is issued before O += P V of tile g, so that it is
- * computed under the softmax of g.  Products of one CTA run in the order they
- * were issued, so S may overwrite a buffer whose P an earlier product reads.
+ * products.  Those of a CTA run in the order in which they were issued, so S of
+ * the next tile may overwrite the P that O += P V before it reads.  The same
+ * warp has Q loaded: of the next piece as soon as the last S of this one is
+ * done, under its softmax.
  * ---------------------------------------------------------------------- */
-template <typename T, int DP>
+__device__ __forceinline__ void load_q(const Params &p, Shared &sh, uint8_t *q_smem, const Piece &e)
+{
+    const int32_t head = uniform(e.h * (int32_t)p.group), q = uniform(e.q0 + e.node0);
+    if (elect()) {
+        mbar_expect(&sh.q_full, p.columns * p.nodes.d * p.group * (kColumn * 2));
+        for (uint32_t c = 0; c < p.columns; c++)    /* rows behind the sequence's are another's, and not used */
+            tma_load(smem_u32(q_smem) + c * (kRows * kColumn * 2), &p.q_map, c * kColumn, head, q, &sh.q_full);
+    }
+    __syncwarp();
+}
+
+template <typename T, Load L, int DP>
 __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *ring, Line line)
 {
-    using S = Shape<DP>;
-    const uint32_t dim = p.d.head_dim, tmem = sh.tmem, o = tmem + 2 * kTile;
-    const uint32_t inst_s = instruction(Type<T>::kBf16, kTile, 0), inst_o = instruction(Type<T>::kBf16, dim, 1);
-    /* one thread issues: descriptors are a constant per step on top of the slot's */
-    const uint32_t q0 = matrix(smem_u32(q_smem), 16), k0 = matrix(smem_u32(ring), 16), v0 = matrix(smem_u32(ring), kTile * 128);
-    uint32_t g = 0, piece = 0, slot = 0, lap = 0;       /* the slot of K of the next S, and the ring's lap */
+    using S = Shape<L, DP>;
+    constexpr uint32_t kSteps = kColumn / 16;           /* of 16 values or positions */
+    const uint32_t dim = p.d.head_dim, s = uniform(sh.tmem), o = s + kTile;
+    const uint32_t inst_s = instruction(Type<T>::kBf16, kTile, 0);
+    const uint32_t q0 = matrix(smem_u32(q_smem), kNoLead), r0 = matrix(smem_u32(ring), kNoLead);
+    Turn<S::kSlots> at;
+    uint32_t g = 0, piece = 0;
     Piece e;
-    auto scores = [&](uint32_t tile) {
-        if (!wait(sh, p.d.error, &sh.full[slot], lap & 1))
-            return false;
-        fence_async_proxy();
-        tmem_fence_after();
-        const uint32_t k = k0 + slot * (S::kSlotBytes >> 4);
-        const uint32_t s = tmem + (tile & 1) * kTile;
-#pragma unroll
-        for (uint32_t x = 0; x < DP / 16; x++)
-            if (x * 16 < dim)
-                mma_ss(s, q0 + ((x >> 2) * (kRows * 128) + (x & 3) * 32 >> 4), k + ((x >> 2) * (kTile * 128) + (x & 3) * 32 >> 4),
-                       inst_s, x > 0);
-        mma_commit(&sh.empty[slot]);
-        mma_commit(&sh.s_full[tile & 1]);
-        slot += 2;
-        if (slot >= S::kSlots) {
-            slot -= S::kSlots;
-            lap++;
-        }
-        return true;
-    };
-    uint32_t v_slot = 1, v_lap = 0;
-    while (line.next(p, e)) {
-        const uint32_t n = e.t1 - e.t0;
-        if (!wait(sh, p.d.error, &sh.q_full, piece & 1) || !scores(g))
+    bool more = line.next(p, e);
+    if (more)
+        load_q(p, sh, q_smem, e);
+    for (; uniform(more); piece++) {
+        if (!wait_warp(sh, p.d.error, &sh.q_full, piece & 1))
             return;
-        if (n == 1)
-            mma_commit(&sh.q_empty);
-        for (uint32_t k = 0; k < n; k++, g++) {
-            if (k + 1 < n) {
-                if (!scores(g + 1))
+        const int32_t n = uniform(e.t1 - e.t0);
+        for (int32_t k = 0; k < n; k++, g++) {
+            for (uint32_t c = 0; c < p.columns; c++, at.next()) {
+                if (!wait_warp(sh, p.d.error, &sh.full[at.slot], at.lap & 1))
                     return;
-                if (k + 2 == n)
-                    mma_commit(&sh.q_empty);    /* every S of the piece is issued */
-            }
-            if (k == 0 && piece && !wait(sh, p.d.error, &sh.o_free, (piece - 1) & 1))
-                return;
-            if (!wait(sh, p.d.error, &sh.p_full[g & 1], (g >> 1) & 1) ||
-                !wait(sh, p.d.error, &sh.full[v_slot], v_lap & 1))
-                return;
-            fence_async_proxy();
-            tmem_fence_after();
-            const uint32_t v = v0 + v_slot * (S::kSlotBytes >> 4);
+                if (L != kTma)
+                    fence_async_proxy();
+                tmem_fence_after();
+                const uint32_t a = q0 + c * (kRows * kColumn * 2 >> 4), b = r0 + at.slot * (kSlotBytes >> 4);
+                if (elect()) {
 #pragma unroll
-            for (uint32_t x = 0; x < kTile / 16; x++)
-                mma_ts(o, tmem + (g & 1) * kTile + x * 8, v + (x * 2048 >> 4), inst_o, k > 0 || x > 0);
-            mma_commit(&sh.empty[v_slot]);
-            mma_commit(&sh.o_done[g & 1]);
-            v_slot += 2;
-            if (v_slot >= S::kSlots) {
-                v_slot -= S::kSlots;
-                v_lap++;
+                    for (uint32_t x = 0; x < kSteps; x++)
+                        if (c * kColumn + x * 16 < dim)
+                            mma_ss(s, a + x * 2, b + x * 2, inst_s, c > 0 || x > 0);
+                    mma_commit(&sh.empty[at.slot]);
+                    if (c + 1 == p.columns) {
+                        mma_commit(&sh.s_full);
+                        if (k + 1 == n)
+                            mma_commit(&sh.q_empty);
+                    }
+                }
+                __syncwarp();
+            }
+            if (k + 1 == n) {
+                more = line.next(p, e);
+                if (!wait_warp(sh, p.d.error, &sh.q_empty, piece & 1))
+                    return;
+                if (uniform(more))
+                    load_q(p, sh, q_smem, e);
+            }
+            if (k == 0 && piece && !wait_warp(sh, p.d.error, &sh.o_free, (piece - 1) & 1))
+                return;
+            for (uint32_t half = 0; half < 2; half++) {
+                if (!wait_warp(sh, p.d.error, &sh.p_full[half], g & 1))
+                    return;
+                Turn<S::kSlots> v = at;
+                for (uint32_t c = 0; c < p.columns; c++, v.next()) {
+                    if (half == 0 && !wait_warp(sh, p.d.error, &sh.full[v.slot], v.lap & 1))
+                        return;
+                    if (L != kTma)
+                        fence_async_proxy();
+                    tmem_fence_after();
+                    const uint32_t b = r0 + v.slot * (kSlotBytes >> 4) + half * (64 * kColumn * 2 >> 4);
+                    const uint32_t inst_o = instruction(Type<T>::kBf16, min(dim - c * kColumn, (uint32_t)kColumn), 1);
+                    if (elect()) {
+#pragma unroll
+                        for (uint32_t x = 0; x < kSteps; x++)
+                            mma_ts(o + c * kColumn, s + half * 32 + x * 8, b + x * (16 * kColumn * 2 >> 4), inst_o,
+                                   k > 0 || half > 0 || x > 0);
+                        if (half) {
+                            mma_commit(&sh.empty[v.slot]);
+                            if (k + 1 == n && c + 1 == p.columns)
+                                mma_commit(&sh.o_done);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (half)
+                    at = v;
             }
         }
-        piece++;
     }
 }
 
@@ -679,16 +757,16 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
  * powers of two), so that O, which lives in TMEM, is rescaled rarely; the
  * result is the same quotient.
  * ---------------------------------------------------------------------- */
-/* the positions of tile t that node j sees, a bit each */
-__device__ uint64_t seen(const Params &p, const Piece &e, int32_t j, int32_t t)
+/* the positions p0 .. p0 + 64 that node j sees, a bit each */
+__device__ uint64_t seen(const Params &p, const Piece &e, int32_t j, int32_t p0)
 {
-    const int32_t p0 = t * kTile, before = e.s.ctx - p0;
+    const int32_t before = e.ctx - p0;
     uint64_t bits = before >= 64 ? ~0ull : before > 0 ? (1ull << before) - 1 : 0;
     if (!p.d.parents) {
         const int32_t upto = before + j + 1;
         return upto >= 64 ? ~0ull : upto > 0 ? (1ull << upto) - 1 : 0;
     }
-    const int32_t *par = p.d.parents + e.s.q0;
+    const int32_t *par = p.d.parents + e.q0;
     for (int32_t a = j; before + a >= 0;) {
         if (before + a < 64)
             bits |= 1ull << (before + a);
@@ -700,50 +778,50 @@ __device__ uint64_t seen(const Params &p, const Piece &e, int32_t j, int32_t t)
     return bits;
 }
 
-/* what was set aside of the values that node j sees in tiles t0 .. t1, dims d0 .. d0 + 16 */
+/* what was set aside of dimension x of the values that node j sees in tiles t0 .. t1 */
 template <typename T, bool F8>
-__device__ __noinline__ void add_spoilt(const Params &p, const Piece &e, int32_t j, uint32_t d0, float *o)
+__device__ __noinline__ float spoilt_at(const Params &p, const Piece &e, int32_t j, uint32_t x)
 {
     const kv_attn_desc &d = p.d;
-    const int32_t *par = d.parents ? d.parents + e.s.q0 : nullptr;
-    const int32_t *tab = d.table + (int64_t)e.s.row * d.table_stride;
+    const int32_t *par = d.parents ? d.parents + e.q0 : nullptr;
+    const int32_t *tab = d.table + (int64_t)e.row * d.table_stride;
+    float sum = 0;
     for (int32_t a = j; a >= 0;) {
-        const int32_t pos = e.s.ctx + a;
+        const int32_t pos = e.ctx + a;
         if (pos < e.t0 * kTile)
             break;
-        const int32_t page = tab[pos / (int32_t)d.block_size];
+        const int32_t page = tab[fdiv(pos, p.block)];
         if (pos < e.t1 * kTile && page >= 0 && (uint32_t)page < d.num_pages) {
-            const uint64_t at = (uint64_t)page * p.stride +
-                                ((uint64_t)(pos % (int32_t)d.block_size) * (d.head_major ? 1 : d.num_kv_heads) * d.head_dim +
-                                 (uint64_t)(d.head_major ? d.block_size : 1) * d.head_dim * e.h + d0) * (F8 ? 1 : 2);
-            for (int x = 0; x < 16; x++) {
-                uint32_t w;
-                if (F8)
-                    w = Type<T>::widen(static_cast<const uint8_t *>(d.v)[at + x]);
-                else
-                    w = *reinterpret_cast<const uint16_t *>(static_cast<const uint8_t *>(d.v) + at + 2 * x);
-                if (!Type<T>::finite(w))
-                    o[x] += Type<T>::value(w & 0xffff);
-            }
+            const uint64_t at = ((uint64_t)(pos - fdiv(pos, p.block) * p.block.d) * (d.head_major ? 1 : d.num_kv_heads) +
+                                 (uint64_t)(d.head_major ? d.block_size : 1) * e.h) * d.head_dim + x;
+            const char *base = static_cast<const char *>(d.v) + (uint64_t)page * p.stride;
+            const uint32_t w = F8 ? Type<T>::widen(reinterpret_cast<const uint8_t *>(base)[at])
+                                  : reinterpret_cast<const uint16_t *>(base)[at];
+            if (!Type<T>::finite(w))
+                sum += Type<T>::value(w & 0xffff);
         }
         const int32_t u = par ? par[a] : a - 1;
         if (u < 0 || (par && !node_ok(par, u)))
             break;
         a = u;
     }
+    return sum;
 }
 
-/* A fed node's value that is not finite would reach the rows that do not see
- * it, as 0 * value: the softmax threads set such values of a tile with fed
- * nodes to 0 before it is used, and add them to the rows that do see them. */
-template <typename T, int DP>
-__device__ bool set_aside(uint8_t *tile, uint32_t dim)
+/* Rows first .. of a slot of V, behind the cached context: the softmax threads
+ * set values that are not finite to 0, which would otherwise reach the rows that
+ * do not see them, as 0 * value.  True if one of them is a fed node's (and not
+ * what a row behind the end or a padding node's happens to hold): such values
+ * are added to the rows that do see them. */
+template <typename T>
+__device__ bool set_aside(const Params &p, const Piece &e, int32_t t, uint8_t *slot, uint32_t values)
 {
     bool any = false;
-    for (uint32_t x = threadIdx.x; x < kTile * DP / 8; x += kSoftmax) {
-        if (x / (kTile * 8) * 8 + ((x ^ x >> 3) & 7) >= dim / 8)
-            continue;                   /* behind the head's dimensions */
-        uint4 v = *reinterpret_cast<uint4 *>(tile + x * 16);
+    for (uint32_t x = threadIdx.x; x < kSlotBytes / 16; x += kSoftmax) {
+        const int32_t j = t * kTile + (int32_t)(x / 8) - e.ctx;
+        if (j < 0 || ((x ^ x >> 3) & 7) * 8 >= values)
+            continue;                   /* the context's, or behind the head's dimensions */
+        uint4 v = *reinterpret_cast<uint4 *>(slot + x * 16);
         uint32_t *w = reinterpret_cast<uint32_t *>(&v);
         bool here = false;
 #pragma unroll
@@ -758,66 +836,100 @@ __device__ bool set_aside(uint8_t *tile, uint32_t dim)
             }
         }
         if (here) {
-            *reinterpret_cast<uint4 *>(tile + x * 16) = v;
-            any = true;
+            *reinterpret_cast<uint4 *>(slot + x * 16) = v;
+            any |= j < e.nodes && (!p.d.parents || node_ok(p.d.parents + e.q0, j));
         }
     }
     return any;
 }
 
-template <typename T, bool F8, int DP>
+/* 64 scores of a row, those that are not seen being -inf */
+__device__ __forceinline__ void scores64(uint32_t addr, uint32_t *raw, bool mask, uint64_t bits)
+{
+    tmem_ld64(addr, raw);
+    if (mask)
+#pragma unroll
+        for (int c = 0; c < 64; c++)
+            raw[c] = bits >> c & 1 ? raw[c] : 0xff800000u;
+}
+
+__device__ __forceinline__ float max64(const float *s)
+{
+    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int c = 4; c < 64; c++)
+        top[c & 3] = fmaxf(top[c & 3], s[c]);
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+template <typename T, Load L, int DP>
 __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
 {
-    using S = Shape<DP>;
+    using S = Shape<L, DP>;
     const kv_attn_desc &d = p.d;
     const uint32_t tid = threadIdx.x, lanes = (tid / 32 * 32) << 16;
-    const uint32_t tmem = sh.tmem + lanes, o_at = tmem + 2 * kTile;
+    const uint32_t s_at = sh.tmem + lanes, o_at = s_at + kTile;
     const float s2 = d.scale * d.k_scale * kLog2e;
+    const int32_t my_node = (int32_t)(tid / p.group), sub = (int32_t)(tid % p.group);
     uint32_t g = 0, piece = 0;
+    Turn<S::kSlots> at;                 /* K of the tile */
     Piece e;
     for (; line.next(p, e); piece++) {
-        const uint32_t x = e.rt * kRows + tid;
-        const bool valid = x < e.s.nodes * p.group.d;
-        const int32_t node = valid ? (int32_t)fdiv(x, p.group) : 0, sub = valid ? (int32_t)(x - node * p.group.d) : 0;
+        const bool valid = (int32_t)tid < e.rows(p);
+        const int32_t node = valid ? e.node0 + my_node : 0;
         bool active = valid;
-        if (valid && d.parents && !node_ok(d.parents + e.s.q0, node)) {
+        if (valid && d.parents && !node_ok(d.parents + e.q0, node)) {
             active = false;
-            if (d.parents[e.s.q0 + node] != -2)
+            if (d.parents[e.q0 + node] != -2)
                 atomicOr(d.error, KVATTN_ERR_PARENT);
         }
         const bool work = __any_sync(~0u, active);
         float m = -INFINITY, l = 0;
         for (int32_t t = e.t0; t < e.t1; t++, g++) {
-            const uint32_t s_at = tmem + (g & 1) * kTile;
-            if (!wait_warp(sh, d.error, &sh.s_full[g & 1], (g >> 1) & 1))
+            const bool mask = (t + 1) * kTile > e.ctx;
+            if (!wait_warp(sh, d.error, &sh.s_full, g & 1))
                 return;
-            if (work) {
-                uint32_t raw[kTile];
-                float *s = reinterpret_cast<float *>(raw);
-                tmem_fence_after();
-                tmem_ld64(s_at, raw);
-                if ((t + 1) * kTile > e.s.ctx) {
-                    const uint64_t bits = active ? seen(p, e, node, t) : 0;
-#pragma unroll
-                    for (int c = 0; c < kTile; c++)
-                        s[c] = bits >> c & 1 ? s[c] : -INFINITY;
+            if (mask) {                 /* V of a tile with fed nodes */
+                bool any = false;
+                for (uint32_t c = 0; c < p.columns; c++)
+                    at.next();
+                Turn<S::kSlots> v = at;
+                for (uint32_t c = 0; c < p.columns; c++, v.next()) {
+                    if (!wait_warp(sh, d.error, &sh.full[v.slot], v.lap & 1))
+                        return;
+                    any |= set_aside<T>(p, e, t, ring + v.slot * kSlotBytes, d.head_dim - c * kColumn);
                 }
-                float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int c = 4; c < kTile; c++)
-                    top[c & 3] = fmaxf(top[c & 3], s[c]);
-                const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * s2;
+                at = v;
+                if (any)
+                    sh.spoilt[piece % 4] = piece + 1;
+                fence_async_proxy();
+            } else {
+                for (uint32_t c = 0; c < 2 * p.columns; c++)
+                    at.next();
+            }
+            if (work) {
+                uint32_t raw[64], w[32];
+                float *s = reinterpret_cast<float *>(raw);
+                uint64_t low = 0, high = 0;
+                if (mask && active) {
+                    low = seen(p, e, node, t * kTile);
+                    high = seen(p, e, node, t * kTile + 64);
+                }
+                /* the maximum first, then the scores again: a thread holds 64 of them */
+                tmem_fence_after();
+                scores64(s_at, raw, mask, low);
+                float now = max64(s);
+                scores64(s_at + 64, raw, mask, high);
+                now = fmaxf(now, max64(s)) * s2;
                 const bool raise = active && now > m + Type<T>::kLazy;
                 if (t == e.t0) {
                     m = now;
                 } else if (__any_sync(~0u, raise)) {
+                    /* S of this tile was issued behind O of the one before, so that is done */
                     const float f = raise ? exp2_approx(m - now) : 1.f;
                     if (raise)
                         m = now;
                     l *= f;
-                    if (!wait_warp(sh, d.error, &sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1))
-                        return;
-                    tmem_fence_after();
                     for (uint32_t c = 0; c < d.head_dim; c += 16) {
                         uint32_t o[16];
                         tmem_ld16(o_at + c, o);
@@ -828,49 +940,53 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
                     }
                 }
                 const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
-                float sum[4] = {};
-                uint32_t w[kTile / 2];
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    scores64(s_at + half * 64, raw, mask, half ? high : low);
+                    float sum[4] = {};
 #pragma unroll
-                for (int c = 0; c < kTile; c += 2) {
-                    const float a = exp2_approx(fmaf(s[c], s2, -from)), b = exp2_approx(fmaf(s[c + 1], s2, -from));
-                    sum[c & 2] += a;
-                    sum[(c & 2) + 1] += b;
-                    w[c / 2] = Type<T>::pack(a, b);
+                    for (int c = 0; c < 64; c += 2) {
+                        const float a = exp2_approx(fmaf(s[c], s2, -from)), b = exp2_approx(fmaf(s[c + 1], s2, -from));
+                        sum[c & 2] += a;
+                        sum[(c & 2) + 1] += b;
+                        w[c / 2] = Type<T>::pack(a, b);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st32(s_at + half * 32, w);     /* over scores that have been read */
+                    tmem_wait_st();
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (tid % 32 == 0)
+                        mbar_arrive(&sh.p_full[half]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st32(s_at, w);
-                tmem_wait_st();
-                tmem_fence_before();
+            } else {
+                __syncwarp();
+                if (tid % 32 == 0) {
+                    mbar_arrive(&sh.p_full[0]);
+                    mbar_arrive(&sh.p_full[1]);
+                }
             }
-            if ((t + 1) * kTile > e.s.ctx) {
-                const uint32_t i = 2 * g + 1, slot = i % S::kSlots;
-                if (!wait_warp(sh, d.error, &sh.full[slot], (i / S::kSlots) & 1))
-                    return;
-                if (set_aside<T, DP>(ring + slot * S::kSlotBytes, d.head_dim))
-                    sh.spoilt[piece % 16] = piece + 1;
-            }
-            __syncwarp();
-            if (tid % 32 == 0)
-                mbar_arrive(&sh.p_full[g & 1]);
         }
         /* the piece's result, or its share of it */
-        if (!wait_warp(sh, d.error, &sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1))
+        if (!wait_warp(sh, d.error, &sh.o_done, piece & 1))
             return;
         tmem_fence_after();
         const bool whole = e.whole();
         const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
         const uint32_t slot = 2 * blockIdx.x + (piece ? 1 : 0);
         const float inv = !active ? 0.f : whole ? d.v_scale / l : 1.f;
-        T *out = static_cast<T *>(d.out) + (int64_t)(e.s.q0 + node) * d.out_stride + (int64_t)(e.h * p.group.d + sub) * d.out_head_stride;
-        float *part = p.part_o + ((uint64_t)slot * kRows + tid) * d.head_dim;
-        const bool spoilt = sh.spoilt[piece % 16] == piece + 1;
+        const bool spoilt = sh.spoilt[piece % 4] == piece + 1;
         if (__any_sync(~0u, valid)) {
+            T *out = static_cast<T *>(d.out) + (int64_t)(e.q0 + node) * d.out_stride + (int64_t)(e.h * p.group + sub) * d.out_head_stride;
+            float *part = p.part_o + ((uint64_t)slot * kRows + tid) * d.head_dim;
             for (uint32_t c = 0; c < d.head_dim; c += 16) {
                 uint32_t raw[16];
                 float *o = reinterpret_cast<float *>(raw);
                 tmem_ld16(o_at + c, raw);
                 if (spoilt && active)
-                    add_spoilt<T, F8>(p, e, node, c, o);
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        o[k] += spoilt_at<T, L == kWiden>(p, e, node, c + k);
                 if (!active)
 #pragma unroll
                     for (int k = 0; k < 16; k++)
@@ -890,16 +1006,14 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
                 }
             }
             if (tid == 0 && e.t0 == 0 && !whole)
-                p.jobs[blockIdx.x] = {min(kRows, (int32_t)(e.s.nodes * p.group.d) - e.rt * kRows),
-                                      (int32_t)(1 + (e.n - e.t1 + sh.share - 1) / sh.share), (int32_t)slot, e.s.q0, e.h, e.rt * kRows};
+                p.jobs[blockIdx.x] = {e.rows(p), (int32_t)(1 + (e.n - e.t1 + sh.share - 1) / sh.share), (int32_t)slot, e.q0 + e.node0, e.h};
             if (valid) {
                 if (!whole) {
                     float *ml = p.part_ml + ((uint64_t)slot * kRows + tid) * 2;
                     ml[0] = active ? from : -INFINITY;
                     ml[1] = active ? l : 0.f;
                 } else if (d.lse) {
-                    d.lse[(int64_t)(e.s.q0 + node) * d.num_heads + e.h * p.group.d + sub] =
-                        active ? (from + log2f(l)) * kLn2 : -INFINITY;
+                    d.lse[(int64_t)(e.q0 + node) * d.num_heads + e.h * p.group + sub] = active ? (from + log2f(l)) * kLn2 : -INFINITY;
                 }
             }
         }
@@ -913,6 +1027,7 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
 /* ------------------------------------------------------------------------
  * the line: every CTA counts the call's tiles and finds its piece of them
  * ---------------------------------------------------------------------- */
+template <int kThreads>
 __device__ int64_t block_scan(Shared &sh, int64_t v, int64_t &total)
 {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -953,7 +1068,7 @@ __device__ void void_rows(const Params &p, const Seq &s)
 /* Counts the tiles of all sequences, kThreads at a time; the CTA's share of
  * the line, and the sequence that it begins in, go to sh.line.  With more than
  * kThreads sequences the search is a second walk. */
-template <typename T>
+template <typename T, int kThreads>
 __device__ void find_line(const Params &p, Shared &sh)
 {
     const kv_attn_desc &d = p.d;
@@ -967,13 +1082,13 @@ __device__ void find_line(const Params &p, Shared &sh)
             Seq s;
             if (b < d.num_seqs) {
                 if (sequence(d, b, s)) {
-                    n = head_tiles(s, p.group);
+                    n = head_tiles(p, s);
                 } else if (walk == 0 && blockIdx.x == b % gridDim.x) {
                     atomicOr(d.error, KVATTN_ERR_SEQ);
                     void_rows<T>(p, s);
                 }
             }
-            const int64_t all = (int64_t)(n * d.num_kv_heads), upto = before + block_scan(sh, all, sum);
+            const int64_t all = (int64_t)(n * d.num_kv_heads), upto = before + block_scan<kThreads>(sh, all, sum);
             before += sum;
             if (once || (walk == 0 && b0 + kThreads >= d.num_seqs)) {
                 if (threadIdx.x == 0) {
@@ -996,35 +1111,35 @@ __device__ void find_line(const Params &p, Shared &sh)
     __syncthreads();
 }
 
-template <typename T, bool F8, int DP>
-__global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(const __grid_constant__ Params p)
+template <typename T, Load L, int DP>
+__global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_attn_kernel(const __grid_constant__ Params p)
 {
-    using S = Shape<DP>;
+    using S = Shape<L, DP>;
     extern __shared__ __align__(1024) uint8_t smem[];
+    constexpr int kThreads = Roles<L>::kThreads;
     uint8_t *q_smem = smem, *ring = smem + S::kQBytes;
-    Shared &sh = *reinterpret_cast<Shared *>(smem + S::kQBytes + S::kSlots * S::kSlotBytes);
+    Shared &sh = *reinterpret_cast<Shared *>(smem + S::kShared);
     const uint32_t warp = threadIdx.x >> 5;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int k = 0; k < S::kSlots; k++) {
-            mbar_init(&sh.full[k], kLoaders);
+            mbar_init(&sh.full[k], L == kTma ? 1 : Roles<L>::kLoaders);
             mbar_init(&sh.empty[k], 1);
         }
-        for (int k = 0; k < 2; k++) {
-            mbar_init(&sh.s_full[k], 1);
-            mbar_init(&sh.o_done[k], 1);
-            mbar_init(&sh.p_full[k], kSoftmax / 32);
-        }
+        mbar_init(&sh.s_full, 1);
+        mbar_init(&sh.p_full[0], kSoftmax / 32);
+        mbar_init(&sh.p_full[1], kSoftmax / 32);
+        mbar_init(&sh.o_done, 1);
         mbar_init(&sh.o_free, kSoftmax / 32);
-        mbar_init(&sh.q_full, kLoaders);
+        mbar_init(&sh.q_full, 1);
         mbar_init(&sh.q_empty, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.dead = 0;
-        for (int k = 0; k < 16; k++)
+        for (int k = 0; k < 4; k++)
             sh.spoilt[k] = 0;
     }
-    find_line<T>(p, sh);
+    find_line<T, kThreads>(p, sh);
     if (threadIdx.x == 0)
         p.jobs[blockIdx.x].rows = 0;
     if (sh.line.x >= sh.line.hi)
@@ -1039,22 +1154,25 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(con
     const Line line = sh.line;
     if (smem_u32(smem) % 1024 == 0) {
         if (warp < kSoftmax / 32) {
-            softmax<T, F8, DP>(p, sh, ring, line);
-        } else if (warp < (kSoftmax + kLoaders) / 32) {
-            Loader<T, F8, DP> load(p, sh, q_smem, ring);
-            if constexpr (F8)
-                load.run8(line);
+            softmax<T, L, DP>(p, sh, ring, line);
+        } else if (warp < kThreads / 32 - 1) {
+            Loader<T, L, DP> load(p, sh, ring);
+            if constexpr (L == kTma)
+                load.run_tma(line);
+            else if constexpr (L == kWiden)
+                load.run_widen(line);
             else
-                load.run16(line);
+                load.run_copy(line);
             copy_wait_all();
         } else {
-            if ((threadIdx.x & 31) == 0)
-                products<T, DP>(p, sh, q_smem, ring, line);
-            __syncwarp();
+            products<T, L, DP>(p, sh, q_smem, ring, line);
         }
     } else if (threadIdx.x == 0) {
         atomicOr(p.d.error, KVATTN_ERR_TIMEOUT);
     }
+    if (sh.dead)
+        for (int k = 0; k < 1000; k++)          /* what is in flight lands before the CTA leaves */
+            __nanosleep(1000);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -1063,52 +1181,88 @@ __global__ void __launch_bounds__(kThreads, Shape<DP>::kCtas) kv_attn_kernel(con
 }
 
 /* ------------------------------------------------------------------------
- * join: the pieces of a row tile that lies across CTAs, in their order.
+ * join: the pieces of a row tile that lies across CTAs, in an order that only
+ * the sizes set.
  * ---------------------------------------------------------------------- */
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid_constant__ Params p)
 {
+    __shared__ float2 ml[kJoinRows][kJoinPieces];       /* maxima and sums of some pieces; then weights */
+    __shared__ float4 other[kJoinThreads];
     const kv_attn_desc &d = p.d;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Job job = p.jobs[blockIdx.x];
-    const int32_t r0 = blockIdx.y * kJoinRows;
-    if (r0 >= job.rows)
-        return;
-    const uint32_t quads = d.head_dim / 4;
-    for (uint32_t x = threadIdx.x; x < kJoinRows * quads; x += kJoinThreads) {
-        const int32_t r = r0 + (int32_t)(x / quads);
-        const uint32_t c = x % quads * 4;
-        if (r >= job.rows)
-            return;
-        /* piece k's row: the first piece's slot, then slot 0 of the CTAs behind */
-        auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (blockIdx.x + k) : (uint32_t)job.slot) * kRows + r; };
-        float m = -INFINITY, l = 0;
+    const int32_t quads = d.head_dim / 4, tid = threadIdx.x;
+    for (int32_t r0 = blockIdx.y * kJoinRows; r0 < job.rows; r0 += gridDim.y * kJoinRows) {
+        const int32_t rows = min(kJoinRows, job.rows - r0), lanes = rows * quads;
+        /* a thread has four dimensions of a row; where that leaves threads
+         * over, `groups` of them share the pieces */
+        const int32_t groups = max(1, kJoinThreads / lanes);
+        for (int32_t base = 0; base < lanes; base += kJoinThreads) {
+            const int32_t lane = groups > 1 ? tid % lanes : base + tid, group = groups > 1 ? tid / lanes : 0;
+            const bool on = lane < lanes && group < groups;
+            const int32_t r = on ? lane / quads : 0, c = lane % quads * 4;
+            float m = -INFINITY, l = 0;
+            float4 o = make_float4(0, 0, 0, 0);
+            for (int32_t k0 = 0; k0 < job.ctas; k0 += kJoinPieces) {
+                const int32_t n = min(kJoinPieces, job.ctas - k0);
+                /* piece k's rows: the first piece's slot, then slot 0 of the CTAs behind */
+                auto at = [&](int32_t k) { return (uint64_t)(k0 + k ? 2 * (blockIdx.x + k0 + k) : (uint32_t)job.slot) * kRows + r0; };
+                __syncthreads();
+                for (int32_t x = tid; x < rows * n; x += kJoinThreads) {
+                    const float2 v = *reinterpret_cast<const float2 *>(p.part_ml + (at(x % n) + x / n) * 2);
+                    ml[x / n][x % n] = v.y == 0 ? make_float2(-INFINITY, 0) : v;    /* sees nothing there */
+                }
+                __syncthreads();
+                float top = m;
+                for (int32_t k = 0; k < n; k++)
+                    top = fmaxf(top, ml[r][k].x);
+                if (!on || top == -INFINITY)
+                    continue;
+                const float keep = exp2f(m - top);
+                m = top;
+                l *= keep;
+                o.x *= keep;
+                o.y *= keep;
+                o.z *= keep;
+                o.w *= keep;
+                for (int32_t k = 0; group == 0 && k < n; k++)
+                    l += exp2f(ml[r][k].x - m) * ml[r][k].y;
 #pragma unroll 4
-        for (int32_t k = 0; k < job.ctas; k++) {
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(k) * 2);
-            m = fmaxf(m, ml.y == 0 ? -INFINITY : ml.x);
+                for (int32_t k = group; k < n; k += groups) {
+                    if (ml[r][k].x == -INFINITY)
+                        continue;           /* its sums were not written */
+                    const float f = exp2f(ml[r][k].x - m);
+                    const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (at(k) + r) * d.head_dim + c);
+                    o.x += f * v.x;
+                    o.y += f * v.y;
+                    o.z += f * v.z;
+                    o.w += f * v.w;
+                }
+            }
+            if (groups > 1) {
+                __syncthreads();
+                other[tid] = o;
+                __syncthreads();
+                if (!on || group)
+                    continue;
+                for (int32_t g = 1; g < groups; g++) {
+                    const float4 v = other[tid + g * lanes];
+                    o.x += v.x;
+                    o.y += v.y;
+                    o.z += v.z;
+                    o.w += v.w;
+                }
+            }
+            if (!on)
+                continue;
+            const int32_t node = (r0 + r) / (int32_t)p.group, sub = (r0 + r) % (int32_t)p.group;
+            const float inv = l == 0 ? 0.f : d.v_scale / l;
+            T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
+            *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
+            if (c == 0 && d.lse)
+                d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
         }
-        float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int32_t k = 0; k < job.ctas; k++) {
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + at(k) * 2);
-            if (ml.y == 0)
-                continue;               /* sees nothing there: its sums were not written */
-            const float f = exp2f(ml.x - m);
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at(k) * d.head_dim + c);
-            l += f * ml.y;
-            o.x += f * v.x;
-            o.y += f * v.y;
-            o.z += f * v.z;
-            o.w += f * v.w;
-        }
-        const uint32_t q = job.row0 + r;
-        const int32_t node = (int32_t)fdiv(q, p.group), sub = (int32_t)(q - node * p.group.d);
-        const float inv = l == 0 ? 0.f : d.v_scale / l;
-        T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group.d + sub) * d.out_head_stride;
-        *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
-        if (c == 0 && d.lse)
-            d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group.d + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
     }
 }
 
@@ -1117,7 +1271,7 @@ bool desc_ok(const kv_attn_desc *d)
 {
     if (!d || !d->num_heads || !d->num_kv_heads || d->num_heads % d->num_kv_heads || d->num_heads > 65535 ||
         !d->head_dim || d->head_dim % 16 || d->head_dim > KVATTN_MAX_HEAD_DIM || !d->block_size || d->block_size > INT32_MAX ||
-        !d->num_pages || d->num_pages > INT32_MAX || !d->width || d->table_stride < (int64_t)d->width || !d->num_rows ||
+        !d->num_pages || d->num_pages > INT32_MAX || d->num_heads / d->num_kv_heads > kRows || !d->width || d->table_stride < (int64_t)d->width || !d->num_rows ||
         d->total_q > INT32_MAX || (d->q_type != KVATTN_BF16 && d->q_type != KVATTN_FP16) ||
         (d->kv_type != d->q_type && d->kv_type != KVATTN_E4M3) || d->device < 0 || d->device >= 64)
         return false;
@@ -1157,28 +1311,79 @@ Work workspace(const kv_attn_desc *d)
     return w;
 }
 
-template <typename T, bool F8, int DP>
+/* cuTensorMapEncodeTiled, from the driver that is loaded */
+using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                            const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder()
+{
+    static Encode f;
+    static std::once_flag once;
+    std::call_once(once, [&] {
+        void *at = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &at, cudaEnableDefault, &found) == cudaSuccess &&
+            found == cudaDriverEntryPointSuccess)
+            f = reinterpret_cast<Encode>(at);
+    });
+    return f;
+}
+
+bool encode_map(const Params &p, CUtensorMap *map, int rank, const void *base, const cuuint64_t *size, const cuuint64_t *stride,
+                const cuuint32_t *box)
+{
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    const Encode encode = encoder();
+    return encode && encode(map, p.d.q_type == KVATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            rank, const_cast<void *>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+/* a plane as the TMA sees it, token-major or head-major alike */
+bool plane_map(const Params &p, const void *plane, CUtensorMap *map)
+{
+    const kv_attn_desc &d = p.d;
+    const uint64_t row = d.head_dim * 2ull;
+    const cuuint64_t size[4] = {d.head_dim, d.block_size, d.num_kv_heads, d.num_pages};
+    const cuuint64_t stride[3] = {row * (d.head_major ? 1 : d.num_kv_heads), row * (d.head_major ? d.block_size : 1), p.stride};
+    const cuuint32_t box[4] = {kColumn, p.box, 1, 1};
+    return encode_map(p, map, 4, plane, size, stride, box);
+}
+
+/* the rows of a tile, whole nodes, as one box */
+bool query_map(const Params &p, CUtensorMap *map)
+{
+    const kv_attn_desc &d = p.d;
+    const cuuint64_t size[3] = {d.head_dim, d.num_heads, d.total_q};
+    const cuuint64_t stride[2] = {2ull * d.q_head_stride, 2ull * d.q_stride};
+    const cuuint32_t box[3] = {kColumn, p.group, p.nodes.d};
+    return encode_map(p, map, 3, d.q, size, stride, box);
+}
+
+template <typename T, Load L, int DP>
 int launch(const Params &p, cudaStream_t stream)
 {
     static std::once_flag once[64];
     static cudaError_t err[64];
     const int dev = p.d.device;
     std::call_once(once[dev], [&] {
-        err[dev] = cudaFuncSetAttribute(kv_attn_kernel<T, F8, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem);
+        err[dev] = cudaFuncSetAttribute(kv_attn_kernel<T, L, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<L, DP>::kSmem);
         if (err[dev] != cudaSuccess)
             cudaGetLastError();
     });
     if (err[dev] != cudaSuccess)
         return -EIO;
     const unsigned grid = (unsigned)grid_of(&p.d);
-    kv_attn_kernel<T, F8, DP><<<grid, kThreads, Shape<DP>::kSmem, stream>>>(p);
+    kv_attn_kernel<T, L, DP><<<grid, Roles<L>::kThreads, Shape<L, DP>::kSmem, stream>>>(p);
     g_cc_kernel_launches.fetch_add(1, std::memory_order_relaxed);
     if (cudaPeekAtLastError() != cudaSuccess)
         return -EIO;
     /* started while the first kernel drains; it waits for its results on the device */
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(grid, kRows / kJoinRows);
+    cfg.gridDim = dim3(grid, p.join_ctas);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1193,14 +1398,31 @@ int launch(const Params &p, cudaStream_t stream)
     return 0;
 }
 
-template <typename T, bool F8>
+template <typename T, Load L>
 int launch_dim(const Params &p, cudaStream_t stream)
 {
     if (p.d.head_dim <= 64)
-        return launch<T, F8, 64>(p, stream);
+        return launch<T, L, 64>(p, stream);
     if (p.d.head_dim <= 128)
-        return launch<T, F8, 128>(p, stream);
-    return launch<T, F8, 256>(p, stream);
+        return launch<T, L, 128>(p, stream);
+    return launch<T, L, 256>(p, stream);
+}
+
+template <typename T>
+int launch_load(Params &p, cudaStream_t stream)
+{
+    if (!query_map(p, &p.q_map))
+        return -EIO;
+    if (p.d.kv_type == KVATTN_E4M3)
+        return launch_dim<T, kWiden>(p, stream);
+    const uint32_t bs = p.d.block_size;
+    p.box = bs < (uint32_t)kTile ? bs : kTile;
+    /* a tile is whole boxes of one page each, which start on the swizzle's eight rows */
+    if (p.box % 8 || kTile % p.box || bs % p.box)
+        return launch_dim<T, kCopy>(p, stream);
+    if (!plane_map(p, p.d.k, &p.k_map) || !plane_map(p, p.d.v, &p.v_map))
+        return -EIO;
+    return launch_dim<T, kTma>(p, stream);
 }
 
 }  // namespace
@@ -1222,7 +1444,7 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
         return 0;
     if (!d->q || !d->out || !d->k || !d->v || !d->table || !d->lens || !d->q_offsets || !d->error || !d->workspace ||
         ((uintptr_t)d->q | (uintptr_t)d->out | (uintptr_t)d->k | (uintptr_t)d->v) % 16 || (uintptr_t)d->workspace % 256 ||
-        (d->q_stride | d->q_head_stride | d->out_stride | d->out_head_stride) % 8)
+        (d->q_stride | d->q_head_stride | d->out_stride | d->out_head_stride) % 8 || d->q_stride <= 0 || d->q_head_stride <= 0)
         return -EINVAL;
     DeviceGuard on(d->device);
     if (!on.ok)
@@ -1234,20 +1456,21 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
     p.d = *d;
     p.stride = d->block_stride ? d->block_stride
                                : (uint64_t)d->block_size * d->num_kv_heads * d->head_dim * (d->kv_type == KVATTN_E4M3 ? 1 : 2);
-    p.group = make_fastdiv(d->num_heads / d->num_kv_heads);
+    p.group = d->num_heads / d->num_kv_heads;
+    p.nodes = make_fastdiv(kRows / p.group);
+    p.columns = (d->head_dim + kColumn - 1) / kColumn;
     p.block = make_fastdiv(d->block_size);
     /* a piece's sums, written and read, are 8 bytes a row and dimension against
-     * 256 bytes a dimension of a 16-bit tile: a CTA takes enough tiles to be
+     * 512 bytes a dimension of a 16-bit tile: a CTA takes enough tiles to be
      * worth that */
-    const uint64_t rows = (uint64_t)d->total_q * p.group.d / d->num_seqs;
-    p.min_share = 1 + (uint32_t)((rows < kRows ? rows : kRows) / 32);
+    const uint64_t mean = ((uint64_t)d->total_q * p.group + d->num_seqs - 1) / d->num_seqs;
+    const uint32_t rows = (uint32_t)(mean < kRows ? mean : kRows);
+    p.min_share = 1 + rows / 64;
+    p.join_ctas = (rows + kJoinRows - 1) / kJoinRows;
     char *base = static_cast<char *>(d->workspace);
     p.jobs = reinterpret_cast<Job *>(base + w.jobs);
     p.part_ml = reinterpret_cast<float *>(base + w.ml);
     p.part_o = reinterpret_cast<float *>(base + w.o);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool e4m3 = d->kv_type == KVATTN_E4M3;
-    if (d->q_type == KVATTN_BF16)
-        return e4m3 ? launch_dim<__nv_bfloat16, true>(p, st) : launch_dim<__nv_bfloat16, false>(p, st);
-    return e4m3 ? launch_dim<__half, true>(p, st) : launch_dim<__half, false>(p, st);
+    return d->q_type == KVATTN_BF16 ? launch_load<__nv_bfloat16>(p, st) : launch_load<__half>(p, st);
 }

@@ -64,7 +64,7 @@ struct kv_attn_desc {
     uint64_t workspace_bytes;
     uint64_t block_stride;       /* bytes from page to page, 0 = block_size * num_kv_heads * head_dim * element */
     int64_t table_stride;
-    int64_t q_stride, q_head_stride;      /* in elements, multiples of 8; head_dim is contiguous */
+    int64_t q_stride, q_head_stride;      /* in elements, multiples of 8 above 0; head_dim is contiguous */
     int64_t out_stride, out_head_stride;
     uint32_t width;              /* entries of a table row */
     uint32_t num_rows;           /* rows of the table */
@@ -72,7 +72,7 @@ struct kv_attn_desc {
     uint32_t total_q;
     uint32_t num_pages;
     uint32_t block_size;
-    uint32_t num_heads;
+    uint32_t num_heads;          /* at most 128 per K/V head */
     uint32_t num_kv_heads;
     uint32_t head_dim;           /* a multiple of 16, <= KVATTN_MAX_HEAD_DIM */
     uint32_t head_major;         /* pages are [kv heads][block_size][head_dim] */

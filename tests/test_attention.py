@@ -27,13 +27,13 @@ def desc(**k):
 
 
 SHAPES = [dict(num_heads=0), dict(num_kv_heads=0), dict(num_kv_heads=3), dict(head_dim=0), dict(head_dim=120),
-          dict(head_dim=272), dict(block_size=0), dict(num_pages=0), dict(num_pages=1 << 31), dict(width=0),
+          dict(head_dim=272), dict(num_heads=258), dict(block_size=0), dict(num_pages=0), dict(num_pages=1 << 31), dict(width=0),
           dict(table_stride=7), dict(num_rows=0), dict(q_type=KVATTN_E4M3), dict(q_type=5), dict(kv_type=KVATTN_FP16),
           dict(block_stride=4096), dict(block_stride=8200), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
           dict(k_scale=0.0), dict(k_scale=math.inf), dict(v_scale=math.nan), dict(device=-1), dict(device=64)]
 POINTERS = [dict(q=None), dict(out=None), dict(k=None), dict(v=None), dict(table=None), dict(lens=None),
             dict(q_offsets=None), dict(error=None), dict(q=X + 8), dict(out=X + 2), dict(k=X + 8), dict(v=X + 4),
-            dict(q_stride=1020), dict(q_head_stride=4), dict(out_stride=1001), dict(out_head_stride=130)]
+            dict(q_stride=1020), dict(q_head_stride=4), dict(q_stride=0), dict(q_head_stride=-128), dict(out_stride=1001), dict(out_head_stride=130)]
 
 
 @pytest.mark.parametrize("bad", SHAPES, ids=str)
@@ -70,6 +70,7 @@ def layout(**k):
     (lambda: TreeAttention(layout(), [X, X], [X], 8, 2), "one pointer"),
     (lambda: TreeAttention(layout(), [X], [X], 8, 3), "must divide"),
     (lambda: TreeAttention(layout(), [X], [X], 8, 0), "must divide"),
+    (lambda: TreeAttention(layout(), [X], [X], 258, 2), "at most 128"),
     (lambda: TreeAttention(layout(hidden_dim_size=240), [X], [X], 8, 2), "multiple of 16"),
     (lambda: TreeAttention(layout(hidden_dim_size=1024), [X], [X], 8, 2), "multiple of 16"),
     (lambda: TreeAttention(layout(element_size=4), [X], [X], 8, 2), "1 or 2-byte"),

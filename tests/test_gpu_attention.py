@@ -177,6 +177,25 @@ def test_masked_infinities_stay_masked(bad, kvt):
     close(out, lse, clean)
 
 
+@pytest.mark.parametrize("kvt", [BF16, E4M3], ids=["16bit", "8bit"])
+@pytest.mark.parametrize("block", [16, 24], ids=["block16", "block24"])
+def test_a_value_of_the_context_that_is_not_finite_reaches_every_row(kvt, block):
+    """beside the nodes, in their tile, and in an earlier one"""
+    for pos in (3, 85, 190, 199):
+        b = Batch([90, 210], [4, 10], seed=15, dim=64, kvt=kvt, block=block).tree(15)
+        r = 0 if pos < 86 else 1
+        clean = b.expected()
+        b.view[:, 1, int(b.table[r, pos // block]), pos % block, :, 3] = torch.full((), math.nan, device="cuda").to(kvt)
+        args, parents = b.args()
+        out, lse = b.attention()(*args, parents=parents, return_lse=True)
+        hit = torch.zeros(14, dtype=torch.bool)
+        hit[b.off[r]:b.off[r + 1]] = True
+        spoiled = ~torch.isfinite(out[:, :, 3]).cpu()
+        assert torch.equal(spoiled.all(1), hit) and torch.equal(spoiled.any(1), hit), pos
+        out[:, :, 3] = clean[0][:, :, 3].to(out.dtype)
+        close(out, lse, clean)
+
+
 def test_large_scores():
     """rows whose maximum climbs through the whole context, and scores that
     only a running maximum survives"""
