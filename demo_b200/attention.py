@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Sequence
 
 import torch
@@ -16,8 +17,10 @@ import torch
 from . import _lib
 from ._lib import KvAttnDesc, lib
 from .cache import CacheError, KVLayout
-from .pages import _int32
+from .pages import _current_stream, _int32
 
+# struct kv_attn_desc in one go: 12 pointers, 8 64-bit numbers, 12 32-bit ones, three floats, the device
+_DESC = struct.Struct("@12PQQqqqqq10I2i3fi")
 _TYPES = {torch.bfloat16: _lib.KVATTN_BF16, torch.float16: _lib.KVATTN_FP16}
 
 _ERRORS = ((_lib.KVATTN_ERR_PAGE, "a page id outside the cache"),
@@ -60,11 +63,19 @@ class TreeAttention:
             raise ValueError("scale and k_scale must be finite and above 0, v_scale finite")
         self.layout, self.num_heads, self.num_kv_heads, self.head_dim = layout, num_heads, num_kv_heads, dim
         self._k, self._v = [int(p) for p in k_ptrs], [int(p) for p in v_ptrs]
-        self._errors: dict[int, torch.Tensor] = {}
-        self._desc = KvAttnDesc(
-            block_stride=layout.block_stride, num_pages=layout.num_blocks, block_size=layout.block_size,
-            num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=dim, head_major=1 if layout.head_bytes else 0,
-            scale=scale, k_scale=k_scale, v_scale=v_scale)
+        self._devices: dict[int, tuple[torch.Tensor, int, int]] = {}     # error bits, their address, workspace bytes
+        self._shape = (layout.num_blocks, layout.block_size, num_heads, num_kv_heads, dim, 1 if layout.head_bytes else 0)
+        self._scales = (scale, float(k_scale), float(v_scale))
+
+    def _device(self, index: int) -> tuple[torch.Tensor, int, int]:
+        d = KvAttnDesc(table_stride=1, width=1, num_rows=1, device=index, scale=self._scales[0], k_scale=self._scales[1])
+        d.num_pages, d.block_size, d.num_heads, d.num_kv_heads, d.head_dim, d.head_major = self._shape
+        need = lib.kv_attn_workspace_bytes(C.addressof(d))
+        if need < 0:
+            raise CacheError("kv_attn_workspace_bytes", need)
+        error = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        self._devices[index] = found = error, error.data_ptr(), need
+        return found
 
     def __call__(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                  q_offsets: torch.Tensor, parents: torch.Tensor | None = None, rows: torch.Tensor | None = None,
@@ -81,58 +92,50 @@ class TreeAttention:
 
         Runs on `stream`, by default the current stream of q's device.
         """
-        if q.dim() != 3 or q.dtype not in _TYPES or q.device.type != "cuda" or q.shape[1] != self.num_heads or \
-                q.shape[2] != self.head_dim or q.stride(2) != 1:
+        index, kind = q.get_device(), _TYPES.get(q.dtype)
+        if index < 0 or kind is None or q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or \
+                q.stride(2) != 1:
             raise ValueError(f"q: expected a bfloat16 or float16 CUDA tensor [total, {self.num_heads}, {self.head_dim}]")
-        dev, total = q.device, q.shape[0]
-        if 0 in q.stride():                             # an expanded tensor
+        total = q.shape[0]
+        q_strides = q.stride()
+        if 0 in q_strides:                              # an expanded tensor
             q = q.contiguous()
-        if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.device != dev or \
+            q_strides = q.stride()
+        if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.get_device() != index or \
                 block_table.shape[1] < 1 or block_table.stride(1) != 1:
-            raise ValueError(f"block_table: expected an int32 tensor [rows, width] on {dev} with contiguous rows")
+            raise ValueError(f"block_table: expected an int32 tensor [rows, width] on cuda:{index} with contiguous rows")
         n_rows, width = block_table.shape
         seqs = q_offsets.numel() - 1
         if seqs < 0 or (rows is None and seqs > n_rows):
             raise ValueError("q_offsets: expected one offset per sequence and the end")
         if out is None:
-            out = torch.empty((total, self.num_heads, self.head_dim), dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+            out = torch.empty((total, self.num_heads, self.head_dim), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or out.stride(2) != 1:
             raise ValueError("out: expected a tensor like q")
-        lse = torch.empty((total, self.num_heads), dtype=torch.float32, device=dev) if return_lse else None
-        index = dev.index
-        error = self._errors.get(index)
-        if error is None:
-            error = self._errors[index] = torch.zeros(1, dtype=torch.int32, device=dev)
-        d = KvAttnDesc.from_buffer_copy(self._desc)     # calls from several threads share nothing
-        d.q, d.out, d.k, d.v = q.data_ptr(), out.data_ptr(), self._k[layer], self._v[layer]
-        d.lse = lse.data_ptr() if return_lse else None
-        d.table, d.lens = block_table.data_ptr(), _int32("seq_lens", seq_lens, dev, n_rows)
-        d.rows = _int32("rows", rows, dev, seqs) if rows is not None else None
-        d.q_offsets = _int32("q_offsets", q_offsets, dev)
-        d.parents = _int32("parents", parents, dev, total) if parents is not None else None
-        d.error = error.data_ptr()
-        d.table_stride = block_table.stride(0) if n_rows > 1 else width
-        row = self.num_heads * self.head_dim            # a stride of one row or one head means nothing
-        d.q_stride, d.out_stride = (q.stride(0), out.stride(0)) if total > 1 else (row, row)
-        d.q_head_stride, d.out_head_stride = (q.stride(1), out.stride(1)) if self.num_heads > 1 else (row, row)
-        d.width, d.num_rows, d.num_seqs, d.total_q = width, n_rows, seqs, total
-        d.q_type = _TYPES[q.dtype]
-        d.kv_type = _lib.KVATTN_E4M3 if self.layout.element_size == 1 else d.q_type
-        d.device = index
-        p = C.addressof(d)
-        need = lib.kv_attn_workspace_bytes(p)
-        if need < 0:
-            raise CacheError("kv_attn_workspace_bytes", need)
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        out_strides = out.stride()
+        lse = torch.empty((total, self.num_heads), dtype=torch.float32, device=q.device) if return_lse else None
+        _, error, need = self._devices.get(index) or self._device(index)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)    # of this call alone, also where graphs are captured
         if stream is None:
-            st = torch.cuda.current_stream(dev).cuda_stream
+            st = _current_stream(index)
         else:
             st = stream.cuda_stream
             for t in (out, lse, work):      # the allocator frees them for the current stream otherwise
                 if t is not None:
                     t.record_stream(stream)
-        d.workspace, d.workspace_bytes = work.data_ptr(), need
-        ret = lib.kv_attn_launch(p, st)
+        row = self.num_heads * self.head_dim            # a stride of one row or one head means nothing
+        pages, block, heads, kv_heads, dim, head_major = self._shape
+        desc = _DESC.pack(
+            q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, self._k[layer], self._v[layer],
+            block_table.data_ptr(), _int32("seq_lens", seq_lens, index, n_rows),
+            _int32("rows", rows, index, seqs) if rows is not None else 0, _int32("q_offsets", q_offsets, index),
+            _int32("parents", parents, index, total) if parents is not None else 0, error, work.data_ptr(),
+            need, self.layout.block_stride, block_table.stride(0) if n_rows > 1 else width,
+            q_strides[0] if total > 1 else row, q_strides[1] if heads > 1 else row,
+            out_strides[0] if total > 1 else row, out_strides[1] if heads > 1 else row,
+            width, n_rows, seqs, total, pages, block, heads, kv_heads, dim, head_major, kind,
+            _lib.KVATTN_E4M3 if self.layout.element_size == 1 else kind, *self._scales, index)
+        ret = lib.kv_attn_launch(desc, st)
         if ret:
             raise CacheError("kv_attn_launch", ret)
         return (out, lse) if return_lse else out
@@ -140,7 +143,7 @@ class TreeAttention:
     def check(self) -> None:
         """Wait for the device and raise ValueError for what the calls since
         the last check() found wrong in their arguments."""
-        for error in self._errors.values():
+        for error, _, _ in self._devices.values():
             bits = int(error.item())
             if bits:
                 error.zero_()

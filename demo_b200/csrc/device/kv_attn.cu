@@ -3,24 +3,25 @@
  * (include/kvattn.h), sm_100a.
  *
  * A K/V head of a sequence serves nodes x (query heads per K/V head) query
- * rows, in tiles of whole nodes, at most 128 rows.  Per 128 positions of the
+ * rows, in tiles of whole nodes, at most 128 rows.  Per 64 positions of the
  * context a CTA computes
  *
- *   S = Q K^T        128 x 128, tcgen05.mma, Q and K in shared memory, S in TMEM
+ *   S = Q K^T        128 x 64, tcgen05.mma, Q and K in shared memory, S in TMEM
  *   P = exp2(S - m)  one thread per row, the running maximum and sum in 32 bits
  *   O += P V         128 x dim, tcgen05.mma, P in TMEM (where S was), V in shared
  *
- * Bound: with up to about 200 rows, reading K and V once from HBM: a tile of
- * 128 positions is 64 KiB at 16 bits and dim 128, about 2800 cycles of an SM's
- * share of the bandwidth, while its products take 1024 cycles of the tensor
+ * Bound: with up to about 200 rows, reading K and V once from HBM: a tile of 64
+ * positions is 32 KiB at 16 bits and dim 128, about 1400 cycles of an SM's
+ * share of the bandwidth, while its products take some 640 cycles of the tensor
  * cores even if only one of the 128 rows is a query, and its exponentials at
- * most as long.  So one form serves single tokens and trees alike.  Two CTAs
- * share an SM: one's softmax runs beside the other's products and loads.
+ * most 512.  So one form serves single tokens and trees alike.  What is left to
+ * hide is latency, from the load to the product, the softmax and the next
+ * product: two CTAs share an SM, and in each S is held twice, so that S of the
+ * next tile is computed under the softmax of this one.
  *
  * Warps 0-3 are the softmax (a thread owns a TMEM lane, a row), then come the
  * loaders, the last warp issues the products.  They meet at mbarriers: a ring
- * of slots of 128 positions x 64 values of K or V, S and P, and O.  Every wait
- * is bounded.
+ * of tiles of K and one of V, S and P, and O.  Every wait is bounded.
  *
  * The (sequence, K/V head, row tile, position tile) quadruples of a call lie on
  * one line, and each CTA takes an equal part of it, wherever that ends inside a
@@ -47,9 +48,9 @@
 namespace {
 
 constexpr int kRows = 128;          /* query rows of a tile: TMEM lanes */
-constexpr int kTile = 128;          /* positions of a tile */
-constexpr int kColumn = 64;         /* values of a row in a slot: 128 bytes, the swizzle's width */
-constexpr int kSlotBytes = kTile * kColumn * 2;
+constexpr int kTile = 64;           /* positions of a tile */
+constexpr int kColumn = 64;         /* Q, K and V stand in columns of 64 values: 128 bytes, the swizzle's width */
+constexpr int kColumnBytes = kTile * kColumn * 2;   /* of K and V */
 constexpr int kSoftmax = 128;       /* threads of the softmax */
 
 /* how K and V come: by TMA (16-bit caches whose pages divide into boxes of 8 or
@@ -57,27 +58,28 @@ constexpr int kSoftmax = 128;       /* threads of the softmax */
  * 16-byte copies that are widened (8-bit caches) */
 enum Load { kTma, kCopy, kWiden };
 template <Load L> struct Roles {
-    static constexpr int kLoaders = L == kTma ? 32 : 128;
+    static constexpr int kLoaders = L == kTma ? 64 : 128;           /* kTma: a warp for K and one for V */
     static constexpr int kThreads = kSoftmax + kLoaders + 32;
 };
-constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 16;       /* rows of one joining CTA */
-constexpr int kJoinPieces = 64;     /* pieces that it looks at together */
+constexpr int kJoinThreads = 128;
+constexpr int kJoinPieces = 4;      /* pieces whose loads are in flight together */
 constexpr uint32_t kSpinLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-/* DP: head_dim rounded up to whole columns, of which K, V and Q are made */
+/* DP: head_dim rounded up to whole columns.  K of the next tile is used a
+ * softmax earlier than V of this one: its ring is the longer one. */
 template <Load L, int DP> struct Shape {
     static constexpr int kCtas = DP <= 128 ? 2 : 1;                 /* per SM */
-    static constexpr int kRaw = L == kWiden ? 4 : 0;                /* slots of 8-bit values on their way */
-    static constexpr int kSlots = DP == 64 ? (kRaw ? 4 : 6) : DP == 128 ? (kRaw ? 3 : 5) : (kRaw ? 8 : 10);
+    static constexpr int kRaw = L == kWiden ? 4 : 0;                /* 8-bit tiles on their way */
+    static constexpr int kSlotsK = kRaw ? 2 : DP == 64 ? 5 : 3;
+    static constexpr int kSlotsV = kRaw ? 1 : DP == 64 ? 4 : 2;
+    static constexpr int kSlotBytes = DP / kColumn * kColumnBytes;
     static constexpr int kQBytes = kRows * DP * 2;
-    static constexpr int kTmem = DP <= 128 ? 256 : 512;             /* columns: 128 of S, then O */
-    static constexpr int kShared = kQBytes + kSlots * kSlotBytes + kRaw * kSlotBytes / 2;   /* where struct Shared stands */
+    static constexpr int kTmem = DP <= 128 ? 256 : 512;             /* columns: 2 x 64 of S, then O */
+    static constexpr int kShared = kQBytes + (kSlotsK + kSlotsV) * kSlotBytes + kRaw * kSlotBytes / 2;  /* of struct Shared */
     static constexpr int kSmem = kShared + 1024;
-    static_assert(kSlots > DP / kColumn, "V of a tile, and one more");
     static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "the CTAs of an SM share its shared memory");
-    static_assert(kTile + DP <= kTmem && kCtas * kTmem <= 512, "and its TMEM");
+    static_assert(2 * kTile + DP <= kTmem && kCtas * kTmem <= 512, "and its TMEM");
 };
 
 /* a row tile that lies across CTAs: its first piece is the last of CTA c (in
@@ -98,6 +100,7 @@ struct Params {
     uint32_t box;
     uint32_t min_share;     /* tiles that a CTA takes at least */
     uint32_t join_ctas;     /* that join a row tile */
+    uint32_t wide_out;      /* rows of out start on 32 bytes */
     Job *jobs;              /* workspace: [CTAs] row tiles to be joined, by the CTA that has their first tiles */
     float *part_ml;         /* [2 * CTAs][128][2] maximum and sum of a piece */
     float *part_o;          /* [2 * CTAs][128][dim] */
@@ -168,7 +171,7 @@ struct Line {
     uint32_t b;
     Seq s;                          /* sequence b, its tiles per K/V head, and the tiles before it */
 
-    __device__ bool next(const Params &p, Piece &e)
+    __device__ __noinline__ bool next(const Params &p, Piece &e)
     {
         if (x >= hi)
             return false;
@@ -213,20 +216,20 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar)
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\t"
                  "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
                  "selp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
 
 struct Shared {
-    uint64_t full[10], empty[10];   /* slots */
-    uint64_t s_full, p_full[2];     /* S of a tile; P of its first and second 64 positions */
-    uint64_t o_done, o_free;        /* O of a piece is complete; has been read */
+    uint64_t k_full[5], k_empty[5], v_full[4], v_empty[4];
+    uint64_t s_full[2], p_full[2];  /* of tiles in turn */
+    uint64_t o_done[2], o_free;     /* O of a tile is complete; O of a piece has been read */
     uint64_t q_full, q_empty;
     uint32_t tmem;
     volatile uint32_t dead;         /* a wait ran out: every role leaves */
@@ -236,12 +239,14 @@ struct Shared {
 };
 static_assert(sizeof(Shared) <= 1024, "the last KiB of the dynamic shared memory");
 
-/* waits for the phase of `parity`, about a second at most */
-__device__ bool wait(Shared &sh, int32_t *error, uint64_t *bar, uint32_t parity)
+/* Waits for the phase of `parity`, about a second at most.  A parity tells a
+ * phase from the one before and the one after only.  Softmax does not wait for
+ * every O: O is done at two barriers in turn, so that where it waits for one,
+ * the one before at that barrier is known to be done (S of a tile is issued
+ * behind O of the tile two before) and the one after is not yet issued. */
+__device__ __noinline__ bool wait_long(Shared &sh, int32_t *error, uint32_t bar, uint32_t parity)
 {
-    for (uint32_t i = 0;; i++) {
-        if (mbar_try_wait(bar, parity))
-            return true;
+    for (uint32_t i = 0; !mbar_try_wait(bar, parity); i++) {
         if (sh.dead)
             return false;
         if (i >= kSpinLimit) {
@@ -249,15 +254,26 @@ __device__ bool wait(Shared &sh, int32_t *error, uint64_t *bar, uint32_t parity)
             atomicOr(error, KVATTN_ERR_TIMEOUT);
             return false;
         }
-        if (i > 256)
-            __nanosleep(64);
+        if (i > 64)
+            __nanosleep(32);
     }
+    return true;
+}
+
+__device__ __forceinline__ bool wait(Shared &sh, int32_t *error, uint32_t bar, uint32_t parity)
+{
+    return mbar_try_wait(bar, parity) || wait_long(sh, error, bar, parity);
 }
 
 /* the same for a whole warp, whose lanes go on together or not at all */
-__device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint64_t *bar, uint32_t parity)
+__device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint32_t bar, uint32_t parity)
 {
     return __all_sync(~0u, wait(sh, error, bar, parity));
+}
+
+__device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint64_t *bar, uint32_t parity)
+{
+    return wait_warp(sh, error, smem_u32(bar), parity);
 }
 
 /* One lane of a converged warp.  What the tensor cores and the TMA are given
@@ -271,7 +287,7 @@ __device__ __forceinline__ bool elect()
     return one != 0;
 }
 
-__device__ __forceinline__ int32_t uniform(int32_t x) { return __shfl_sync(~0u, x, 0); }
+template <typename I> __device__ __forceinline__ I uniform(I x) { return (I)__shfl_sync(~0u, (int32_t)x, 0); }
 
 /* shared-memory matrix descriptor, 128-byte swizzle: the low word (where it
  * starts, and the bytes between 64-value columns of an operand stored row by
@@ -327,14 +343,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t *a)
                  : R8(a, 0), R8(a, 8) : "r"(addr) : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t *a)
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *a)
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-                 "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
                  "tcgen05.wait::ld.sync.aligned;"
-                 : R8(a, 0), R8(a, 8), R8(a, 16), R8(a, 24), R8(a, 32), R8(a, 40), R8(a, 48), R8(a, 56) : "r"(addr) : "memory");
+                 : R8(a, 0), R8(a, 8), R8(a, 16), R8(a, 24) : "r"(addr) : "memory");
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *a)
@@ -343,18 +357,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *a)
                  ::W8(a, 0), W8(a, 8), "r"(addr) : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *a)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
-                 ::W8(a, 0), W8(a, 8), W8(a, 16), W8(a, 24), "r"(addr) : "memory");
-}
-
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+/* 32 bytes, one sector: a row's lane fills sectors of its own */
+__device__ __forceinline__ void store32(void *to, const uint32_t *w)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
 /* ---- 16-bit types ---- */
@@ -411,21 +425,21 @@ __device__ __forceinline__ void copy_arrive(uint64_t *bar)
 /* what this thread has written to shared memory, or seen written, comes before the products behind it */
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes)
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes)
 {
-    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint64_t *bar)
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint32_t bar)
 {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t *bar)
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, int32_t w, uint32_t bar)
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
 
 /* where chunk c (16 bytes) of row r stands in a slot */
@@ -435,9 +449,9 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c)
 }
 
 /* ------------------------------------------------------------------------
- * loaders: for each tile the columns of K, then those of V, a slot each.
+ * loaders: a ring of tiles of K, one of tiles of V.
  * ---------------------------------------------------------------------- */
-/* a place in the ring, and how often the ring has been gone around */
+/* a place in a ring, and how often the ring has been gone around */
 template <int N> struct Turn {
     uint32_t slot = 0, lap = 0;
     __device__ __forceinline__ void next()
@@ -453,61 +467,83 @@ template <typename T, Load L, int DP> struct Loader {
     using S = Shape<L, DP>;
     static constexpr bool F8 = L == kWiden;
     enum : uint64_t { kNone = ~0ull };
-    static constexpr int kChunks = F8 ? 4 : 8;                  /* 16-byte loads of a row of a slot */
+    static constexpr int kChunks = F8 ? 4 : 8;                  /* 16-byte loads of a row of a column */
     static constexpr int kPass = 128 / kChunks;                 /* rows of one pass */
     static constexpr int kPasses = kTile / kPass;
     static constexpr int kWarpRows = kPass / 4;                 /* of them a warp's */
-    static_assert(kPasses * kWarpRows == 32, "a lane looks after one of the warp's rows");
+    static_assert(kPasses * kWarpRows == 16, "a lane of each half warp looks after one of the warp's rows");
 
     const Params &p;
     Shared &sh;
-    uint8_t *ring;
-    Turn<S::kSlots> at;
+    uint8_t *ring;                      /* K's slots, then V's, then the 8-bit ones */
+    Turn<S::kSlotsK> at_k;
+    Turn<S::kSlotsV> at_v;
 
     __device__ Loader(const Params &p_, Shared &sh_, uint8_t *ring_) : p(p_), sh(sh_), ring(ring_) {}
 
-    __device__ __forceinline__ uint8_t *slot() const { return ring + at.slot * kSlotBytes; }
+    /* the slot of the next tile of V or K may be written; the lanes go on together or not at all */
+    __device__ __forceinline__ bool acquire(bool v)
+    {
+        return wait_warp(sh, p.d.error, v ? &sh.v_empty[at_v.slot] : &sh.k_empty[at_k.slot], (v ? at_v.lap : at_k.lap) & 1 ^ 1);
+    }
+    __device__ __forceinline__ uint8_t *slot(bool v) const
+    {
+        return ring + (v ? S::kSlotsK + at_v.slot : at_k.slot) * S::kSlotBytes;
+    }
+    __device__ __forceinline__ uint64_t *full(bool v) const { return v ? &sh.v_full[at_v.slot] : &sh.k_full[at_k.slot]; }
+    __device__ __forceinline__ void advance(bool v)
+    {
+        if (v)
+            at_v.next();
+        else
+            at_k.next();
+    }
 
-    /* the slot may be written; the lanes go on together or not at all */
-    __device__ __forceinline__ bool acquire() { return wait_warp(sh, p.d.error, &sh.empty[at.slot], at.lap & 1 ^ 1); }
-
-    /* Boxes of a page's rows by a column; a lane looks up its box's page.  Rows behind the end, and those of padding nodes, hold
-     * anything: their scores are masked, and softmax makes their values finite.
-     * A page id out of range is out of the map: zeros. */
-    __device__ void run_tma(Line line)
+    /* Boxes of a page's rows by a column; a lane looks up its box's page.  Rows
+     * behind the end, and those of padding nodes, hold anything: their scores are
+     * masked, and softmax makes their values finite.  A page id out of range is
+     * out of the map: zeros.  One warp brings K, another V. */
+    __device__ void run_tma(Line line, bool v)
     {
         const uint32_t lane = threadIdx.x % 32, boxes = kTile / p.box, box_bytes = p.box * (kColumn * 2);
+        const uint32_t slots = uniform(v ? S::kSlotsV : S::kSlotsK), base = uniform(smem_u32(slot(v)));
+        const uint32_t bars = uniform(smem_u32(v ? sh.v_full : sh.k_full)), frees = uniform(smem_u32(v ? sh.v_empty : sh.k_empty));
+        const CUtensorMap *map = v ? &p.v_map : &p.k_map;
+        uint32_t at = 0, parity = 1;
         Piece e;
         while (line.next(p, e)) {
             const int32_t *tab = p.d.table + (int64_t)e.row * p.d.table_stride;
             const int32_t t1 = uniform(e.t1), end = uniform(e.end), h = uniform(e.h);
             int32_t pos = e.t0 * kTile + (int32_t)(lane * p.box);
-            int32_t next = lane < boxes && pos < e.end ? tab[fdiv(pos, p.block)] : 0;
+            int32_t next = lane < boxes && pos < end ? tab[fdiv(pos, p.block)] : 0;
             for (int32_t t = uniform(e.t0); t < t1; t++) {
                 const int32_t page = next;
-                /* a page of more than 128 rows holds several tiles */
+                /* a page of more than 64 rows holds several tiles */
                 const int32_t first = uniform(boxes == 1 ? pos - (int32_t)(fdiv(pos, p.block) * p.block.d) : 0);
                 const uint32_t n = min(boxes, (end - t * kTile + p.box - 1) / p.box);
                 if (lane < n && (uint32_t)page >= p.d.num_pages)
                     atomicOr(p.d.error, KVATTN_ERR_PAGE);
                 pos += kTile;
                 if (t + 1 < t1)
-                    next = lane < boxes && pos < e.end ? tab[fdiv(pos, p.block)] : 0;   /* in flight while the tile is loaded */
-                for (uint32_t x = 0; x < 2 * p.columns; x++, at.next()) {
-                    if (!acquire())
-                        return;
-                    uint64_t *bar = &sh.full[at.slot];
-                    const CUtensorMap *map = x < p.columns ? &p.k_map : &p.v_map;
-                    const int32_t column = (int32_t)(x < p.columns ? x : x - p.columns) * kColumn;
-                    uint32_t to = smem_u32(slot());
+                    next = lane < boxes && pos < end ? tab[fdiv(pos, p.block)] : 0;     /* in flight while the tile is loaded */
+                if (!wait_warp(sh, p.d.error, frees + at * 8, parity))
+                    return;
+                const uint32_t bar = bars + at * 8;
+                uint32_t to = base + at * S::kSlotBytes;
+                if (elect())
+                    mbar_expect(bar, n * box_bytes * p.columns);
+                __syncwarp();
+                for (uint32_t b = 0; b < n; b++, to += box_bytes) {
+                    const int32_t id = __shfl_sync(~0u, page, b);
                     if (elect())
-                        mbar_expect(bar, n * box_bytes);
-                    __syncwarp();
-                    for (uint32_t b = 0; b < n; b++, to += box_bytes) {
-                        const int32_t id = __shfl_sync(~0u, page, b);
-                        if (elect())
-                            tma_load(to, map, column, first, h, id, bar);
-                    }
+#pragma unroll
+                        for (uint32_t c = 0; c < DP / kColumn; c++)
+                            if (c < p.columns)
+                                tma_load(to + c * kColumnBytes, map, c * kColumn, first, h, id, bar);
+                }
+                if (++at == slots) {
+                    at = 0;
+                    parity ^= 1;
                 }
             }
         }
@@ -523,7 +559,7 @@ template <typename T, Load L, int DP> struct Loader {
         const uint32_t t = threadIdx.x - kSoftmax, lane = t % 32, warp = t / 32;
         chunk = t % kChunks;
         row = t / kChunks;
-        own_row = lane / kWarpRows * kPass + warp * kWarpRows + lane % kWarpRows;
+        own_row = lane % 16 / kWarpRows * kPass + warp * kWarpRows + lane % kWarpRows;
     }
 
     /* the page of this lane's row of tile t: a load that waits for nothing */
@@ -556,16 +592,18 @@ template <typename T, Load L, int DP> struct Loader {
             off[i] = __shfl_sync(~0u, own, i * kWarpRows + from);
     }
 
-    /* this thread's share of column c of K (v = 0) or V, asynchronously, row r of a pass going to at(pass) */
-    template <typename F> __device__ __forceinline__ void copy_column(uint32_t v, uint32_t c, F place)
+    /* this thread's share of K or V, asynchronously; chunk c's row of pass i goes to place(c, i) */
+    template <typename F> __device__ __forceinline__ void copy_tile(bool v, F place)
     {
-        const uint32_t x = c * (F8 ? kColumn : kColumn * 2) + chunk * 16;
         const char *plane = static_cast<const char *>(v ? p.d.v : p.d.k);
-        if (x >= p.d.head_dim * (F8 ? 1 : 2))
-            return;
 #pragma unroll
-        for (int i = 0; i < kPasses; i++)
-            copy16(place(i), plane + (off[i] == kNone ? 0 : off[i] + x), off[i] != kNone);
+        for (uint32_t c = 0; c < DP / kColumn; c++) {
+            const uint32_t x = c * (F8 ? kColumn : kColumn * 2) + chunk * 16;
+            if (x < p.d.head_dim * (F8 ? 1 : 2))
+#pragma unroll
+                for (int i = 0; i < kPasses; i++)
+                    copy16(place(c, i), plane + (off[i] == kNone ? 0 : off[i] + x), off[i] != kNone);
+        }
     }
 
     __device__ void run_copy(Line line)
@@ -573,49 +611,55 @@ template <typename T, Load L, int DP> struct Loader {
         take_rows();
         Piece e;
         while (line.next(p, e)) {
+            const int32_t t1 = e.t1;
             int32_t page = look_up(e, e.t0);
-            for (int32_t t = e.t0; t < e.t1; t++) {
+            for (int32_t t = e.t0; t < t1; t++) {
                 places(e, t, page);
-                if (t + 1 < e.t1)
+                if (t + 1 < t1)
                     page = look_up(e, t + 1);       /* in flight while the tile is copied */
-                for (uint32_t x = 0; x < 2 * p.columns; x++, at.next()) {
-                    if (!acquire())
+                for (int v = 0; v < 2; v++) {
+                    if (!acquire(v))
                         return;
-                    const uint32_t to = smem_u32(slot());
-                    copy_column(x >= p.columns, x < p.columns ? x : x - p.columns,
-                                [&](int i) { return to + swizzled(row + i * kPass, chunk); });
-                    copy_arrive(&sh.full[at.slot]);
+                    const uint32_t to = smem_u32(slot(v));
+                    copy_tile(v, [&](uint32_t c, int i) { return to + c * kColumnBytes + swizzled(row + i * kPass, chunk); });
+                    copy_arrive(full(v));
+                    advance(v);
                 }
             }
         }
     }
 
-    /* 8-bit caches: copied as they are, kRaw - 1 slots ahead, to places in
-     * shared memory that only the copying thread uses; that thread widens them
-     * into the ring. */
-    __device__ __forceinline__ uint8_t *raw(uint32_t k, int i) const
+    /* 8-bit caches: copied as they are, kRaw - 1 tiles of K or V ahead, to
+     * places in shared memory that only the copying thread uses; that thread
+     * widens them into the rings. */
+    __device__ __forceinline__ uint8_t *raw(uint32_t k, uint32_t c, int i) const
     {
-        return ring + S::kSlots * kSlotBytes + (k % S::kRaw) * (kSlotBytes / 2) + i * (128 * 16) + (threadIdx.x - kSoftmax) * 16;
+        return ring + (S::kSlotsK + S::kSlotsV) * S::kSlotBytes + (k % S::kRaw) * (S::kSlotBytes / 2) +
+               (c * kPasses + i) * (128 * 16) + (threadIdx.x - kSoftmax) * 16;
     }
 
-    __device__ bool widen(uint32_t k, uint32_t c)
+    __device__ bool widen(uint32_t k)
     {
-        if (!acquire())
+        const bool v = k & 1;
+        if (!acquire(v))
             return false;
-        if (c * kColumn + chunk * 16 < p.d.head_dim)
 #pragma unroll
-            for (int i = 0; i < kPasses; i++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(raw(k, i));
-                const uint32_t r = row + i * kPass;
-                *reinterpret_cast<uint4 *>(slot() + swizzled(r, 2 * chunk)) =
-                    make_uint4(Type<T>::widen((uint16_t)w.x), Type<T>::widen((uint16_t)(w.x >> 16)),
-                               Type<T>::widen((uint16_t)w.y), Type<T>::widen((uint16_t)(w.y >> 16)));
-                *reinterpret_cast<uint4 *>(slot() + swizzled(r, 2 * chunk + 1)) =
-                    make_uint4(Type<T>::widen((uint16_t)w.z), Type<T>::widen((uint16_t)(w.z >> 16)),
-                               Type<T>::widen((uint16_t)w.w), Type<T>::widen((uint16_t)(w.w >> 16)));
-            }
-        mbar_arrive(&sh.full[at.slot]);
-        at.next();
+        for (uint32_t c = 0; c < DP / kColumn; c++)
+            if (c * kColumn + chunk * 16 < p.d.head_dim)
+#pragma unroll
+                for (int i = 0; i < kPasses; i++) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(raw(k, c, i));
+                    const uint32_t r = row + i * kPass;
+                    uint8_t *to = slot(v) + c * kColumnBytes;
+                    *reinterpret_cast<uint4 *>(to + swizzled(r, 2 * chunk)) =
+                        make_uint4(Type<T>::widen((uint16_t)w.x), Type<T>::widen((uint16_t)(w.x >> 16)),
+                                   Type<T>::widen((uint16_t)w.y), Type<T>::widen((uint16_t)(w.y >> 16)));
+                    *reinterpret_cast<uint4 *>(to + swizzled(r, 2 * chunk + 1)) =
+                        make_uint4(Type<T>::widen((uint16_t)w.z), Type<T>::widen((uint16_t)(w.z >> 16)),
+                                   Type<T>::widen((uint16_t)w.w), Type<T>::widen((uint16_t)(w.w >> 16)));
+                }
+        mbar_arrive(full(v));
+        advance(v);
         return true;
     }
 
@@ -623,25 +667,21 @@ template <typename T, Load L, int DP> struct Loader {
     {
         constexpr uint32_t kAhead = S::kRaw > 0 ? S::kRaw - 1 : 0;
         take_rows();
-        uint32_t k = 0, done = 0, c = 0;    /* slots fetched, widened, and the column of the next to be widened */
+        uint32_t k = 0, done = 0;           /* tiles of K and V, in turn: fetched, widened */
         Piece e;
-        auto finish = [&] {
-            const uint32_t mine = c;
-            c = c + 1 == p.columns ? 0 : c + 1;
-            return widen(done++, mine);
-        };
         while (line.next(p, e)) {
+            const int32_t t1 = e.t1;
             int32_t page = look_up(e, e.t0);
-            for (int32_t t = e.t0; t < e.t1; t++) {
+            for (int32_t t = e.t0; t < t1; t++) {
                 places(e, t, page);
-                if (t + 1 < e.t1)
+                if (t + 1 < t1)
                     page = look_up(e, t + 1);
-                for (uint32_t x = 0; x < 2 * p.columns; x++, k++) {
-                    copy_column(x >= p.columns, x < p.columns ? x : x - p.columns, [&](int i) { return smem_u32(raw(k, i)); });
+                for (int v = 0; v < 2; v++, k++) {
+                    copy_tile(v, [&](uint32_t c, int i) { return smem_u32(raw(k, c, i)); });
                     copy_commit();
                     if (k >= kAhead) {
                         copy_wait_but<kAhead>();
-                        if (!finish())
+                        if (!widen(done++))
                             return;
                     }
                 }
@@ -649,14 +689,15 @@ template <typename T, Load L, int DP> struct Loader {
         }
         copy_wait_all();
         while (done < k)
-            if (!finish())
+            if (!widen(done++))
                 return;
     }
 };
 
 /* ------------------------------------------------------------------------
- * products.  Those of a CTA run in the order in which they were issued, so S of
- * the next tile may overwrite the P that O += P V before it reads.  The same
+ * products.  S of tile g + 1 is issued before O += P V of tile g, to be computed
+ * under the softmax of g.  Those of a CTA run in the order in which they were
+ * issued, so S may overwrite a buffer whose P an earlier one reads.  The same
  * warp has Q loaded: of the next piece as soon as the last S of this one is
  * done, under its softmax.
  * ---------------------------------------------------------------------- */
@@ -664,9 +705,10 @@ __device__ __forceinline__ void load_q(const Params &p, Shared &sh, uint8_t *q_s
 {
     const int32_t head = uniform(e.h * (int32_t)p.group), q = uniform(e.q0 + e.node0);
     if (elect()) {
-        mbar_expect(&sh.q_full, p.columns * p.nodes.d * p.group * (kColumn * 2));
+        const uint32_t bar = smem_u32(&sh.q_full);
+        mbar_expect(bar, p.columns * p.nodes.d * p.group * (kColumn * 2));
         for (uint32_t c = 0; c < p.columns; c++)    /* rows behind the sequence's are another's, and not used */
-            tma_load(smem_u32(q_smem) + c * (kRows * kColumn * 2), &p.q_map, c * kColumn, head, q, &sh.q_full);
+            tma_load(smem_u32(q_smem) + c * (kRows * kColumn * 2), &p.q_map, c * kColumn, head, q, bar);
     }
     __syncwarp();
 }
@@ -675,42 +717,47 @@ template <typename T, Load L, int DP>
 __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *ring, Line line)
 {
     using S = Shape<L, DP>;
-    constexpr uint32_t kSteps = kColumn / 16;           /* of 16 values or positions */
-    const uint32_t dim = p.d.head_dim, s = uniform(sh.tmem), o = s + kTile;
-    const uint32_t inst_s = instruction(Type<T>::kBf16, kTile, 0);
-    const uint32_t q0 = matrix(smem_u32(q_smem), kNoLead), r0 = matrix(smem_u32(ring), kNoLead);
-    Turn<S::kSlots> at;
+    const uint32_t dim = p.d.head_dim, s = uniform(sh.tmem), o = s + 2 * kTile;
+    const uint32_t inst_s = instruction(Type<T>::kBf16, kTile, 0), inst_o = instruction(Type<T>::kBf16, dim, 1);
+    const uint32_t q0 = matrix(smem_u32(q_smem), kNoLead), k0 = matrix(smem_u32(ring), kNoLead),
+                   v0 = matrix(smem_u32(ring) + S::kSlotsK * S::kSlotBytes, kColumnBytes);
+    Turn<S::kSlotsK> at_k;
+    Turn<S::kSlotsV> at_v;
     uint32_t g = 0, piece = 0;
     Piece e;
     bool more = line.next(p, e);
+    /* S of a tile; the last of its piece also releases Q */
+    auto scores = [&](uint32_t tile, bool last) {
+        if (!wait_warp(sh, p.d.error, &sh.k_full[at_k.slot], at_k.lap & 1))
+            return false;
+        if (L != kTma)
+            fence_async_proxy();
+        tmem_fence_after();
+        const uint32_t b = k0 + at_k.slot * (S::kSlotBytes >> 4), to = s + (tile & 1) * kTile;
+        if (elect()) {
+#pragma unroll
+            for (uint32_t x = 0; x < DP / 16; x++)
+                if (x * 16 < dim)
+                    mma_ss(to, q0 + ((x >> 2) * (kRows * kColumn * 2 >> 4) + (x & 3) * 2), b + ((x >> 2) * (kColumnBytes >> 4) + (x & 3) * 2),
+                           inst_s, x > 0);
+            mma_commit(&sh.k_empty[at_k.slot]);
+            mma_commit(&sh.s_full[tile & 1]);
+            if (last)
+                mma_commit(&sh.q_empty);
+        }
+        __syncwarp();
+        at_k.next();
+        return true;
+    };
     if (more)
         load_q(p, sh, q_smem, e);
     for (; uniform(more); piece++) {
-        if (!wait_warp(sh, p.d.error, &sh.q_full, piece & 1))
-            return;
         const int32_t n = uniform(e.t1 - e.t0);
+        if (!wait_warp(sh, p.d.error, &sh.q_full, piece & 1) || !scores(g, n == 1))
+            return;
         for (int32_t k = 0; k < n; k++, g++) {
-            for (uint32_t c = 0; c < p.columns; c++, at.next()) {
-                if (!wait_warp(sh, p.d.error, &sh.full[at.slot], at.lap & 1))
-                    return;
-                if (L != kTma)
-                    fence_async_proxy();
-                tmem_fence_after();
-                const uint32_t a = q0 + c * (kRows * kColumn * 2 >> 4), b = r0 + at.slot * (kSlotBytes >> 4);
-                if (elect()) {
-#pragma unroll
-                    for (uint32_t x = 0; x < kSteps; x++)
-                        if (c * kColumn + x * 16 < dim)
-                            mma_ss(s, a + x * 2, b + x * 2, inst_s, c > 0 || x > 0);
-                    mma_commit(&sh.empty[at.slot]);
-                    if (c + 1 == p.columns) {
-                        mma_commit(&sh.s_full);
-                        if (k + 1 == n)
-                            mma_commit(&sh.q_empty);
-                    }
-                }
-                __syncwarp();
-            }
+            if (k + 1 < n && !scores(g + 1, k + 2 == n))
+                return;
             if (k + 1 == n) {
                 more = line.next(p, e);
                 if (!wait_warp(sh, p.d.error, &sh.q_empty, piece & 1))
@@ -720,34 +767,22 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
             }
             if (k == 0 && piece && !wait_warp(sh, p.d.error, &sh.o_free, (piece - 1) & 1))
                 return;
-            for (uint32_t half = 0; half < 2; half++) {
-                if (!wait_warp(sh, p.d.error, &sh.p_full[half], g & 1))
-                    return;
-                Turn<S::kSlots> v = at;
-                for (uint32_t c = 0; c < p.columns; c++, v.next()) {
-                    if (half == 0 && !wait_warp(sh, p.d.error, &sh.full[v.slot], v.lap & 1))
-                        return;
-                    if (L != kTma)
-                        fence_async_proxy();
-                    tmem_fence_after();
-                    const uint32_t b = r0 + v.slot * (kSlotBytes >> 4) + half * (64 * kColumn * 2 >> 4);
-                    const uint32_t inst_o = instruction(Type<T>::kBf16, min(dim - c * kColumn, (uint32_t)kColumn), 1);
-                    if (elect()) {
+            if (!wait_warp(sh, p.d.error, &sh.v_full[at_v.slot], at_v.lap & 1) ||
+                !wait_warp(sh, p.d.error, &sh.p_full[g & 1], (g >> 1) & 1))
+                return;
+            if (L != kTma)
+                fence_async_proxy();
+            tmem_fence_after();
+            const uint32_t b = v0 + at_v.slot * (S::kSlotBytes >> 4), a = s + (g & 1) * kTile;
+            if (elect()) {
 #pragma unroll
-                        for (uint32_t x = 0; x < kSteps; x++)
-                            mma_ts(o + c * kColumn, s + half * 32 + x * 8, b + x * (16 * kColumn * 2 >> 4), inst_o,
-                                   k > 0 || half > 0 || x > 0);
-                        if (half) {
-                            mma_commit(&sh.empty[v.slot]);
-                            if (k + 1 == n && c + 1 == p.columns)
-                                mma_commit(&sh.o_done);
-                        }
-                    }
-                    __syncwarp();
-                }
-                if (half)
-                    at = v;
+                for (uint32_t x = 0; x < kTile / 16; x++)
+                    mma_ts(o, a + x * 8, b + x * (16 * kColumn * 2 >> 4), inst_o, k > 0 || x > 0);
+                mma_commit(&sh.v_empty[at_v.slot]);
+                mma_commit(&sh.o_done[g & 1]);
             }
+            __syncwarp();
+            at_v.next();
         }
     }
 }
@@ -778,34 +813,42 @@ __device__ uint64_t seen(const Params &p, const Piece &e, int32_t j, int32_t p0)
     return bits;
 }
 
-/* what was set aside of dimension x of the values that node j sees in tiles t0 .. t1 */
+/* Adds to O what was set aside of the values that node j sees in the piece's
+ * tiles; the warp's rows that are not `active` add nothing.  Rare, and kept out
+ * of the loops' way: inlined, it pushed them out of the instruction cache. */
 template <typename T, bool F8>
-__device__ __noinline__ float spoilt_at(const Params &p, const Piece &e, int32_t j, uint32_t x)
+__device__ __noinline__ void add_spoilt(const Params &p, const Piece &e, int32_t j, bool active, uint32_t o_at)
 {
     const kv_attn_desc &d = p.d;
     const int32_t *par = d.parents ? d.parents + e.q0 : nullptr;
     const int32_t *tab = d.table + (int64_t)e.row * d.table_stride;
-    float sum = 0;
-    for (int32_t a = j; a >= 0;) {
-        const int32_t pos = e.ctx + a;
-        if (pos < e.t0 * kTile)
-            break;
-        const int32_t page = tab[fdiv(pos, p.block)];
-        if (pos < e.t1 * kTile && page >= 0 && (uint32_t)page < d.num_pages) {
-            const uint64_t at = ((uint64_t)(pos - fdiv(pos, p.block) * p.block.d) * (d.head_major ? 1 : d.num_kv_heads) +
-                                 (uint64_t)(d.head_major ? d.block_size : 1) * e.h) * d.head_dim + x;
-            const char *base = static_cast<const char *>(d.v) + (uint64_t)page * p.stride;
-            const uint32_t w = F8 ? Type<T>::widen(reinterpret_cast<const uint8_t *>(base)[at])
-                                  : reinterpret_cast<const uint16_t *>(base)[at];
-            if (!Type<T>::finite(w))
-                sum += Type<T>::value(w & 0xffff);
+#pragma unroll 1
+    for (uint32_t c = 0; c < d.head_dim; c += 16) {
+        uint32_t raw[16];
+        tmem_ld16(o_at + c, raw);
+#pragma unroll 1
+        for (int32_t a = active ? j : -1; a >= 0 && e.ctx + a >= e.t0 * kTile;) {
+            const uint32_t pos = e.ctx + a, b = fdiv(pos, p.block);
+            const int32_t page = tab[b];
+            if ((int32_t)pos < e.t1 * kTile && page >= 0 && (uint32_t)page < d.num_pages) {
+                const uint64_t at = ((uint64_t)(pos - b * p.block.d) * (d.head_major ? 1 : d.num_kv_heads) +
+                                     (uint64_t)(d.head_major ? d.block_size : 1) * e.h) * d.head_dim + c;
+                const char *base = static_cast<const char *>(d.v) + (uint64_t)page * p.stride;
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const uint32_t w = F8 ? Type<T>::widen(reinterpret_cast<const uint8_t *>(base)[at + x])
+                                          : reinterpret_cast<const uint16_t *>(base)[at + x];
+                    if (!Type<T>::finite(w))
+                        raw[x] = __float_as_uint(__uint_as_float(raw[x]) + Type<T>::value(w & 0xffff));
+                }
+            }
+            const int32_t u = par ? par[a] : a - 1;
+            a = u < 0 || (par && !node_ok(par, u)) ? -1 : u;
         }
-        const int32_t u = par ? par[a] : a - 1;
-        if (u < 0 || (par && !node_ok(par, u)))
-            break;
-        a = u;
+        __syncwarp();
+        tmem_st16(o_at + c, raw);
     }
-    return sum;
+    tmem_wait_st();
 }
 
 /* Rows first .. of a slot of V, behind the cached context: the softmax threads
@@ -817,10 +860,12 @@ template <typename T>
 __device__ bool set_aside(const Params &p, const Piece &e, int32_t t, uint8_t *slot, uint32_t values)
 {
     bool any = false;
-    for (uint32_t x = threadIdx.x; x < kSlotBytes / 16; x += kSoftmax) {
+    const int32_t skip = max(0, e.ctx - t * kTile);     /* the context's */
+#pragma unroll 4
+    for (uint32_t x = skip * 8 + threadIdx.x; x < kColumnBytes / 16; x += kSoftmax) {
         const int32_t j = t * kTile + (int32_t)(x / 8) - e.ctx;
-        if (j < 0 || ((x ^ x >> 3) & 7) * 8 >= values)
-            continue;                   /* the context's, or behind the head's dimensions */
+        if (((x ^ x >> 3) & 7) * 8 >= values)
+            continue;                   /* behind the head's dimensions */
         uint4 v = *reinterpret_cast<uint4 *>(slot + x * 16);
         uint32_t *w = reinterpret_cast<uint32_t *>(&v);
         bool here = false;
@@ -843,23 +888,12 @@ __device__ bool set_aside(const Params &p, const Piece &e, int32_t t, uint8_t *s
     return any;
 }
 
-/* 64 scores of a row, those that are not seen being -inf */
-__device__ __forceinline__ void scores64(uint32_t addr, uint32_t *raw, bool mask, uint64_t bits)
+/* -inf for the scores whose bit is off */
+__device__ __forceinline__ void hide(float *s, uint32_t bits)
 {
-    tmem_ld64(addr, raw);
-    if (mask)
 #pragma unroll
-        for (int c = 0; c < 64; c++)
-            raw[c] = bits >> c & 1 ? raw[c] : 0xff800000u;
-}
-
-__device__ __forceinline__ float max64(const float *s)
-{
-    float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-    for (int c = 4; c < 64; c++)
-        top[c & 3] = fmaxf(top[c & 3], s[c]);
-    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    for (int c = 0; c < 32; c++)
+        s[c] = bits >> c & 1 ? s[c] : -INFINITY;
 }
 
 template <typename T, Load L, int DP>
@@ -868,11 +902,11 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
     using S = Shape<L, DP>;
     const kv_attn_desc &d = p.d;
     const uint32_t tid = threadIdx.x, lanes = (tid / 32 * 32) << 16;
-    const uint32_t s_at = sh.tmem + lanes, o_at = s_at + kTile;
+    const uint32_t tmem = sh.tmem + lanes, o_at = tmem + 2 * kTile;
     const float s2 = d.scale * d.k_scale * kLog2e;
     const int32_t my_node = (int32_t)(tid / p.group), sub = (int32_t)(tid % p.group);
     uint32_t g = 0, piece = 0;
-    Turn<S::kSlots> at;                 /* K of the tile */
+    Turn<S::kSlotsV> at_v;
     Piece e;
     for (; line.next(p, e); piece++) {
         const bool valid = (int32_t)tid < e.rows(p);
@@ -884,125 +918,124 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
                 atomicOr(d.error, KVATTN_ERR_PARENT);
         }
         const bool work = __any_sync(~0u, active);
+        const int32_t t0 = e.t0, t1 = e.t1, ctx = e.ctx;
         float m = -INFINITY, l = 0;
-        for (int32_t t = e.t0; t < e.t1; t++, g++) {
-            const bool mask = (t + 1) * kTile > e.ctx;
-            if (!wait_warp(sh, d.error, &sh.s_full, g & 1))
+        for (int32_t t = t0; t < t1; t++, g++, at_v.next()) {
+            const uint32_t s_at = tmem + (g & 1) * kTile;
+            const bool mask = (t + 1) * kTile > ctx;
+            uint64_t bits = 0;
+            if (mask && active)
+                bits = seen(p, e, node, t * kTile);
+            if (!wait_warp(sh, d.error, &sh.s_full[g & 1], (g >> 1) & 1))
                 return;
-            if (mask) {                 /* V of a tile with fed nodes */
-                bool any = false;
-                for (uint32_t c = 0; c < p.columns; c++)
-                    at.next();
-                Turn<S::kSlots> v = at;
-                for (uint32_t c = 0; c < p.columns; c++, v.next()) {
-                    if (!wait_warp(sh, d.error, &sh.full[v.slot], v.lap & 1))
-                        return;
-                    any |= set_aside<T>(p, e, t, ring + v.slot * kSlotBytes, d.head_dim - c * kColumn);
-                }
-                at = v;
-                if (any)
-                    sh.spoilt[piece % 4] = piece + 1;
-                fence_async_proxy();
-            } else {
-                for (uint32_t c = 0; c < 2 * p.columns; c++)
-                    at.next();
-            }
             if (work) {
-                uint32_t raw[64], w[32];
+                /* The maximum first, then the scores again, 32 at a time: the
+                 * second reading is cheap, and a short loop stays in the
+                 * instruction cache beside the other roles'. */
+                uint32_t raw[32];
                 float *s = reinterpret_cast<float *>(raw);
-                uint64_t low = 0, high = 0;
-                if (mask && active) {
-                    low = seen(p, e, node, t * kTile);
-                    high = seen(p, e, node, t * kTile + 64);
-                }
-                /* the maximum first, then the scores again: a thread holds 64 of them */
+                float now = -INFINITY;
                 tmem_fence_after();
-                scores64(s_at, raw, mask, low);
-                float now = max64(s);
-                scores64(s_at + 64, raw, mask, high);
-                now = fmaxf(now, max64(s)) * s2;
+#pragma unroll 1
+                for (int half = 0; half < kTile; half += 32) {
+                    tmem_ld32(s_at + half, raw);
+                    if (mask)
+                        hide(s, (uint32_t)(bits >> half));
+                    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c < 32; c++)
+                        top[c & 3] = fmaxf(top[c & 3], s[c]);
+                    now = fmaxf(now, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                }
+                now *= s2;
                 const bool raise = active && now > m + Type<T>::kLazy;
-                if (t == e.t0) {
+                if (t == t0) {
                     m = now;
                 } else if (__any_sync(~0u, raise)) {
-                    /* S of this tile was issued behind O of the one before, so that is done */
                     const float f = raise ? exp2_approx(m - now) : 1.f;
                     if (raise)
                         m = now;
                     l *= f;
+                    if (!wait_warp(sh, d.error, &sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1))
+                        return;
+                    tmem_fence_after();
+#pragma unroll 1
                     for (uint32_t c = 0; c < d.head_dim; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(o_at + c, o);
+                        tmem_ld16(o_at + c, raw);
 #pragma unroll
                         for (int k = 0; k < 16; k++)
-                            o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                        tmem_st16(o_at + c, o);
+                            s[k] *= f;
+                        tmem_st16(o_at + c, raw);
                     }
                 }
                 const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
 #pragma unroll 1
-                for (int half = 0; half < 2; half++) {
-                    scores64(s_at + half * 64, raw, mask, half ? high : low);
+                for (int half = 0; half < kTile; half += 32) {
+                    tmem_ld32(s_at + half, raw);
+                    if (mask)
+                        hide(s, (uint32_t)(bits >> half));
                     float sum[4] = {};
+                    uint32_t w[16];
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) {
+                    for (int c = 0; c < 32; c += 2) {
                         const float a = exp2_approx(fmaf(s[c], s2, -from)), b = exp2_approx(fmaf(s[c + 1], s2, -from));
                         sum[c & 2] += a;
                         sum[(c & 2) + 1] += b;
                         w[c / 2] = Type<T>::pack(a, b);
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st32(s_at + half * 32, w);     /* over scores that have been read */
-                    tmem_wait_st();
-                    tmem_fence_before();
-                    __syncwarp();
-                    if (tid % 32 == 0)
-                        mbar_arrive(&sh.p_full[half]);
+                    tmem_st16(s_at + half / 2, w);      /* over scores that have been read */
                 }
-            } else {
-                __syncwarp();
-                if (tid % 32 == 0) {
-                    mbar_arrive(&sh.p_full[0]);
-                    mbar_arrive(&sh.p_full[1]);
-                }
+                tmem_wait_st();
+                tmem_fence_before();
             }
+            if (mask) {                 /* V of a tile with fed nodes */
+                if (!wait_warp(sh, d.error, &sh.v_full[at_v.slot], at_v.lap & 1))
+                    return;
+                bool any = false;
+                for (uint32_t c = 0; c < p.columns; c++)
+                    any |= set_aside<T>(p, e, t, ring + (S::kSlotsK + at_v.slot) * S::kSlotBytes + c * kColumnBytes,
+                                        d.head_dim - c * kColumn);
+                if (any)
+                    sh.spoilt[piece % 4] = piece + 1;
+                fence_async_proxy();
+            }
+            __syncwarp();
+            if (tid % 32 == 0)
+                mbar_arrive(&sh.p_full[g & 1]);
         }
         /* the piece's result, or its share of it */
-        if (!wait_warp(sh, d.error, &sh.o_done, piece & 1))
+        if (!wait_warp(sh, d.error, &sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1))
             return;
         tmem_fence_after();
         const bool whole = e.whole();
         const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
         const uint32_t slot = 2 * blockIdx.x + (piece ? 1 : 0);
         const float inv = !active ? 0.f : whole ? d.v_scale / l : 1.f;
-        const bool spoilt = sh.spoilt[piece % 4] == piece + 1;
+        const bool spoilt = __any_sync(~0u, sh.spoilt[piece % 4] == piece + 1);
         if (__any_sync(~0u, valid)) {
+            if (spoilt)
+                add_spoilt<T, L == kWiden>(p, e, node, active, o_at);
             T *out = static_cast<T *>(d.out) + (int64_t)(e.q0 + node) * d.out_stride + (int64_t)(e.h * p.group + sub) * d.out_head_stride;
             float *part = p.part_o + ((uint64_t)slot * kRows + tid) * d.head_dim;
+#pragma unroll 1
             for (uint32_t c = 0; c < d.head_dim; c += 16) {
-                uint32_t raw[16];
-                float *o = reinterpret_cast<float *>(raw);
+                uint32_t raw[16], w[8];
+                const float *o = reinterpret_cast<const float *>(raw);
                 tmem_ld16(o_at + c, raw);
-                if (spoilt && active)
-#pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        o[k] += spoilt_at<T, L == kWiden>(p, e, node, c + k);
-                if (!active)
-#pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        o[k] = 0.f;
                 if (whole && valid) {
-                    uint4 v[2];
-                    uint32_t *w = reinterpret_cast<uint32_t *>(v);
 #pragma unroll
                     for (int k = 0; k < 8; k++)
-                        w[k] = Type<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv);
-                    *reinterpret_cast<uint4 *>(out + c) = v[0];
-                    *reinterpret_cast<uint4 *>(out + c + 8) = v[1];
+                        w[k] = active ? Type<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0;
+                    if (p.wide_out) {
+                        store32(out + c, w);
+                    } else {
+                        *reinterpret_cast<uint4 *>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4 *>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
                 } else if (active) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        *reinterpret_cast<float4 *>(part + c + 4 * k) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    store32(part + c, raw);
+                    store32(part + c + 8, raw + 8);
                 }
             }
             if (tid == 0 && e.t0 == 0 && !whole)
@@ -1052,7 +1085,7 @@ __device__ int64_t block_scan(Shared &sh, int64_t v, int64_t &total)
 }
 
 template <typename T>
-__device__ void void_rows(const Params &p, const Seq &s)
+__device__ __noinline__ void void_rows(const Params &p, const Seq &s)
 {
     const kv_attn_desc &d = p.d;
     for (int64_t x = 0; x < (int64_t)s.nodes * d.num_heads; x++) {
@@ -1123,14 +1156,19 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int k = 0; k < S::kSlots; k++) {
-            mbar_init(&sh.full[k], L == kTma ? 1 : Roles<L>::kLoaders);
-            mbar_init(&sh.empty[k], 1);
+        for (int k = 0; k < S::kSlotsK; k++) {
+            mbar_init(&sh.k_full[k], L == kTma ? 1 : Roles<L>::kLoaders);
+            mbar_init(&sh.k_empty[k], 1);
         }
-        mbar_init(&sh.s_full, 1);
-        mbar_init(&sh.p_full[0], kSoftmax / 32);
-        mbar_init(&sh.p_full[1], kSoftmax / 32);
-        mbar_init(&sh.o_done, 1);
+        for (int k = 0; k < S::kSlotsV; k++) {
+            mbar_init(&sh.v_full[k], L == kTma ? 1 : Roles<L>::kLoaders);
+            mbar_init(&sh.v_empty[k], 1);
+        }
+        for (int k = 0; k < 2; k++) {
+            mbar_init(&sh.s_full[k], 1);
+            mbar_init(&sh.p_full[k], kSoftmax / 32);
+            mbar_init(&sh.o_done[k], 1);
+        }
         mbar_init(&sh.o_free, kSoftmax / 32);
         mbar_init(&sh.q_full, 1);
         mbar_init(&sh.q_empty, 1);
@@ -1157,9 +1195,9 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
             softmax<T, L, DP>(p, sh, ring, line);
         } else if (warp < kThreads / 32 - 1) {
             Loader<T, L, DP> load(p, sh, ring);
-            if constexpr (L == kTma)
-                load.run_tma(line);
-            else if constexpr (L == kWiden)
+            if constexpr (L == kTma) {
+                load.run_tma(line, warp != kSoftmax / 32);
+            } else if constexpr (L == kWiden)
                 load.run_widen(line);
             else
                 load.run_copy(line);
@@ -1187,82 +1225,52 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid_constant__ Params p)
 {
-    __shared__ float2 ml[kJoinRows][kJoinPieces];       /* maxima and sums of some pieces; then weights */
-    __shared__ float4 other[kJoinThreads];
     const kv_attn_desc &d = p.d;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Job job = p.jobs[blockIdx.x];
-    const int32_t quads = d.head_dim / 4, tid = threadIdx.x;
-    for (int32_t r0 = blockIdx.y * kJoinRows; r0 < job.rows; r0 += gridDim.y * kJoinRows) {
-        const int32_t rows = min(kJoinRows, job.rows - r0), lanes = rows * quads;
-        /* a thread has four dimensions of a row; where that leaves threads
-         * over, `groups` of them share the pieces */
-        const int32_t groups = max(1, kJoinThreads / lanes);
-        for (int32_t base = 0; base < lanes; base += kJoinThreads) {
-            const int32_t lane = groups > 1 ? tid % lanes : base + tid, group = groups > 1 ? tid / lanes : 0;
-            const bool on = lane < lanes && group < groups;
-            const int32_t r = on ? lane / quads : 0, c = lane % quads * 4;
-            float m = -INFINITY, l = 0;
-            float4 o = make_float4(0, 0, 0, 0);
-            for (int32_t k0 = 0; k0 < job.ctas; k0 += kJoinPieces) {
-                const int32_t n = min(kJoinPieces, job.ctas - k0);
-                /* piece k's rows: the first piece's slot, then slot 0 of the CTAs behind */
-                auto at = [&](int32_t k) { return (uint64_t)(k0 + k ? 2 * (blockIdx.x + k0 + k) : (uint32_t)job.slot) * kRows + r0; };
-                __syncthreads();
-                for (int32_t x = tid; x < rows * n; x += kJoinThreads) {
-                    const float2 v = *reinterpret_cast<const float2 *>(p.part_ml + (at(x % n) + x / n) * 2);
-                    ml[x / n][x % n] = v.y == 0 ? make_float2(-INFINITY, 0) : v;    /* sees nothing there */
-                }
-                __syncthreads();
-                float top = m;
-                for (int32_t k = 0; k < n; k++)
-                    top = fmaxf(top, ml[r][k].x);
-                if (!on || top == -INFINITY)
-                    continue;
-                const float keep = exp2f(m - top);
-                m = top;
-                l *= keep;
-                o.x *= keep;
-                o.y *= keep;
-                o.z *= keep;
-                o.w *= keep;
-                for (int32_t k = 0; group == 0 && k < n; k++)
-                    l += exp2f(ml[r][k].x - m) * ml[r][k].y;
-#pragma unroll 4
-                for (int32_t k = group; k < n; k += groups) {
-                    if (ml[r][k].x == -INFINITY)
-                        continue;           /* its sums were not written */
-                    const float f = exp2f(ml[r][k].x - m);
-                    const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (at(k) + r) * d.head_dim + c);
-                    o.x += f * v.x;
-                    o.y += f * v.y;
-                    o.z += f * v.z;
-                    o.w += f * v.w;
-                }
+    const int32_t quads = d.head_dim / 4;
+    /* a thread has four dimensions of a row */
+    for (int32_t x = blockIdx.y * kJoinThreads + threadIdx.x; x < job.rows * quads; x += gridDim.y * kJoinThreads) {
+        const int32_t r = x / quads, c = (x - r * quads) * 4;
+        /* piece k's row: the first piece's slot, then slot 0 of the CTAs behind */
+        auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (blockIdx.x + k) : (uint32_t)job.slot) * kRows + r; };
+        float m = -INFINITY, l = 0;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int32_t k0 = 0; k0 < job.ctas; k0 += kJoinPieces) {
+            float2 ml[kJoinPieces];
+            float4 v[kJoinPieces];
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < kJoinPieces; k++) {     /* all loads first */
+                const bool on = k0 + k < job.ctas;
+                ml[k] = on ? *reinterpret_cast<const float2 *>(p.part_ml + at(k0 + k) * 2) : make_float2(0, 0);
+                v[k] = on ? *reinterpret_cast<const float4 *>(p.part_o + at(k0 + k) * d.head_dim + c) : make_float4(0, 0, 0, 0);
             }
-            if (groups > 1) {
-                __syncthreads();
-                other[tid] = o;
-                __syncthreads();
-                if (!on || group)
-                    continue;
-                for (int32_t g = 1; g < groups; g++) {
-                    const float4 v = other[tid + g * lanes];
-                    o.x += v.x;
-                    o.y += v.y;
-                    o.z += v.z;
-                    o.w += v.w;
-                }
-            }
-            if (!on)
+#pragma unroll
+            for (int k = 0; k < kJoinPieces; k++)
+                if (ml[k].y != 0)                       /* else it sees nothing there, and its sums were not written */
+                    top = fmaxf(top, ml[k].x);
+            if (top == -INFINITY)
                 continue;
-            const int32_t node = (r0 + r) / (int32_t)p.group, sub = (r0 + r) % (int32_t)p.group;
-            const float inv = l == 0 ? 0.f : d.v_scale / l;
-            T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
-            *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
-            if (c == 0 && d.lse)
-                d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
+            const float keep = exp2f(m - top);
+            m = top;
+            l *= keep;
+            o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+            for (int k = 0; k < kJoinPieces; k++) {
+                if (ml[k].y == 0)
+                    continue;
+                const float f = exp2f(ml[k].x - m);
+                l += f * ml[k].y;
+                o = make_float4(o.x + f * v[k].x, o.y + f * v[k].y, o.z + f * v[k].z, o.w + f * v[k].w);
+            }
         }
+        const int32_t node = r / (int32_t)p.group, sub = r - node * (int32_t)p.group;
+        const float inv = l == 0 ? 0.f : d.v_scale / l;
+        T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
+        *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
+        if (c == 0 && d.lse)
+            d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
     }
 }
 
@@ -1461,12 +1469,13 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
     p.columns = (d->head_dim + kColumn - 1) / kColumn;
     p.block = make_fastdiv(d->block_size);
     /* a piece's sums, written and read, are 8 bytes a row and dimension against
-     * 512 bytes a dimension of a 16-bit tile: a CTA takes enough tiles to be
+     * 256 bytes a dimension of a 16-bit tile: a CTA takes enough tiles to be
      * worth that */
     const uint64_t mean = ((uint64_t)d->total_q * p.group + d->num_seqs - 1) / d->num_seqs;
     const uint32_t rows = (uint32_t)(mean < kRows ? mean : kRows);
-    p.min_share = 1 + rows / 64;
-    p.join_ctas = (rows + kJoinRows - 1) / kJoinRows;
+    p.min_share = 1 + rows / 32;
+    p.join_ctas = (rows * d->head_dim / 4 + 2 * kJoinThreads - 1) / (2 * kJoinThreads);    /* two of a thread's shares each */
+    p.wide_out = (uintptr_t)d->out % 32 == 0 && (d->out_stride | d->out_head_stride) % 16 == 0;
     char *base = static_cast<char *>(d->workspace);
     p.jobs = reinterpret_cast<Job *>(base + w.jobs);
     p.part_ml = reinterpret_cast<float *>(base + w.ml);

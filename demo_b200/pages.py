@@ -29,10 +29,16 @@ _ERRORS = ((_lib.KVPAGE_ERR_PAGE, "a page id outside the cache"),
 OK, NO_PAGES, INVALID = _lib.KVPAGE_OK, _lib.KVPAGE_NO_PAGES, _lib.KVPAGE_INVALID
 
 
-def _int32(name: str, t: torch.Tensor, device: torch.device, numel: int | None = None) -> int:
-    """data pointer of a contiguous int32 tensor on `device`; ValueError otherwise"""
-    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous int32 tensor on {device}")
+# The calls are short on the GPU too: the helpers ask a tensor for its device's
+# number and torch for the stream's handle, which costs a tenth of the objects.
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _int32(name: str, t: torch.Tensor, index: int, numel: int | None = None) -> int:
+    """data pointer of a contiguous int32 tensor on CUDA device `index` (-1:
+    the CPU); ValueError otherwise"""
+    if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor on {f'cuda:{index}' if index >= 0 else 'the CPU'}")
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name}: expected {numel} values, got {t.numel()}")
     return t.data_ptr()
@@ -98,11 +104,11 @@ class PagePool:
         self.error = torch.zeros(1, dtype=torch.int32, device=dev)
         self._marks = torch.zeros(n, dtype=torch.int32, device=dev)
         self._k, self._v, align = plane_bases(layout, k_ptrs, v_ptrs, dev)
-        self._index = dev.index if dev.index is not None else torch.cuda.current_device()
+        self._index = index = dev.index
         self._state = KvPageState(
-            table=block_table.data_ptr(), lens=_int32("seq_lens", seq_lens, dev, rows),
-            refs=_int32("refs", refs, dev, n), free_list=_int32("free_list", free_list, dev, n),
-            free_count=_int32("free_count", free_count, dev, 1), marks=self._marks.data_ptr(),
+            table=block_table.data_ptr(), lens=_int32("seq_lens", seq_lens, index, rows),
+            refs=_int32("refs", refs, index, n), free_list=_int32("free_list", free_list, index, n),
+            free_count=_int32("free_count", free_count, index, 1), marks=self._marks.data_ptr(),
             error=self.error.data_ptr(), table_stride=block_table.stride(0) if rows > 1 else width, width=width,
             num_rows=rows, num_pages=n, block_size=layout.block_size, device=self._index)
         self._cache = KvPageCache(
@@ -116,7 +122,7 @@ class PagePool:
         """n results and `scratch` values behind them, and the stream's handle"""
         out = torch.empty(n + scratch, dtype=torch.int32, device=self.device)
         if stream is None:
-            return out, torch.cuda.current_stream(self.device).cuda_stream
+            return out, _current_stream(self._index)
         out.record_stream(stream)           # the allocator frees it for the current stream otherwise
         return out, stream.cuda_stream
 
@@ -126,8 +132,8 @@ class PagePool:
         order of the call.  Returns each row's result."""
         n = rows.numel()
         status, st = self._results(n, 0, stream)
-        ret = lib.kv_page_resize_launch(self._state_p, _int32("rows", rows, self.device),
-                                        _int32("lens", lens, self.device, n), n, status.data_ptr(), st)
+        ret = lib.kv_page_resize_launch(self._state_p, _int32("rows", rows, self._index),
+                                        _int32("lens", lens, self._index, n), n, status.data_ptr(), st)
         if ret:
             raise CacheError("kv_page_resize_launch", ret)
         return status
@@ -138,9 +144,9 @@ class PagePool:
         tokens[i] tokens, with tokens).  Destinations are distinct and not
         among the sources."""
         n = src.numel()
-        st = (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream
-        ret = lib.kv_page_copy_launch(self._cache_p, _int32("src", src, self.device), _int32("dst", dst, self.device, n),
-                                      _int32("tokens", tokens, self.device, n) if tokens is not None else None, n, st)
+        st = _current_stream(self._index) if stream is None else stream.cuda_stream
+        ret = lib.kv_page_copy_launch(self._cache_p, _int32("src", src, self._index), _int32("dst", dst, self._index, n),
+                                      _int32("tokens", tokens, self._index, n) if tokens is not None else None, n, st)
         if ret:
             raise CacheError("kv_page_copy_launch", ret)
 
@@ -151,8 +157,8 @@ class PagePool:
         each child's result."""
         n = parents.numel()
         out, st = self._results(n, 3 * n, stream)
-        ret = lib.kv_page_fork_launch(self._cache_p, self._state_p, _int32("parents", parents, self.device),
-                                      _int32("children", children, self.device, n), n, out.data_ptr() + 4 * n,
+        ret = lib.kv_page_fork_launch(self._cache_p, self._state_p, _int32("parents", parents, self._index),
+                                      _int32("children", children, self._index, n), n, out.data_ptr() + 4 * n,
                                       out.data_ptr(), st)
         if ret:
             raise CacheError("kv_page_fork_launch", ret)
@@ -166,9 +172,9 @@ class PagePool:
         left over are given back.  Returns each row's result."""
         n = rows.numel()
         out, st = self._results(n, n, stream)
-        ret = lib.kv_page_compact_launch(self._cache_p, self._state_p, _int32("rows", rows, self.device),
-                                         _int32("start", start, self.device, n), _int32("keep", keep, self.device),
-                                         _int32("offsets", offsets, self.device, n + 1), keep.numel(), n,
+        ret = lib.kv_page_compact_launch(self._cache_p, self._state_p, _int32("rows", rows, self._index),
+                                         _int32("start", start, self._index, n), _int32("keep", keep, self._index),
+                                         _int32("offsets", offsets, self._index, n + 1), keep.numel(), n,
                                          out.data_ptr() + 4 * n, out.data_ptr(), st)
         if ret:
             raise CacheError("kv_page_compact_launch", ret)

@@ -116,6 +116,16 @@ def test_struct_layout(tmp_path):
         assert (getattr(KvAttnDesc, field).offset if field else C.sizeof(KvAttnDesc)) == int(val), field
 
 
+def test_packed_descriptor():
+    """the descriptor that a call packs is the struct"""
+    from demo_b200.attention import _DESC
+
+    values = [*range(1, 13), *range(101, 108), *range(201, 211), 1, 2, 0.5, 0.25, 2.0, 7]
+    d = KvAttnDesc.from_buffer_copy(_DESC.pack(*values))
+    assert _DESC.size == C.sizeof(KvAttnDesc)
+    assert [getattr(d, name) for name, _ in KvAttnDesc._fields_] == values
+
+
 def test_the_oracle_on_a_case_worked_by_hand():
     """scores 0 everywhere: the mean of the values seen"""
     q = torch.zeros(4, 2, 16, dtype=torch.bfloat16)

@@ -91,11 +91,11 @@ def test_pool_refuses_tensors_it_cannot_use():
     with pytest.raises(ValueError, match="block_table"):
         pg.PagePool(lay, [X], [X], table, lens)                       # not on a CUDA device
     with pytest.raises(ValueError, match="contiguous int32"):
-        pg._int32("x", lens.long(), lens.device)
+        pg._int32("x", lens.long(), -1)
     with pytest.raises(ValueError, match="contiguous int32"):
-        pg._int32("x", torch.zeros(4, dtype=torch.int32)[::2], lens.device)
+        pg._int32("x", torch.zeros(4, dtype=torch.int32)[::2], -1)
     with pytest.raises(ValueError, match="expected 3 values"):
-        pg._int32("x", lens, lens.device, 3)
+        pg._int32("x", lens, -1, 3)
     with pytest.raises(ValueError, match="one pointer per layer"):
         pg.plane_bases(lay, [X, X], [X], lens.device)
     with pytest.raises(ValueError, match="kv must be 1"):
