@@ -20,8 +20,9 @@
  * next tile is computed under the softmax of this one.
  *
  * Warps 0-3 are the softmax (a thread owns a TMEM lane, a row), then come the
- * loaders, the last warp issues the products.  They meet at mbarriers: a ring
- * of tiles of K and one of V, S and P, and O.  Every wait is bounded.
+ * loaders, a warp that issues the products, and one that finds the next pieces
+ * of work for all of them.  They meet at mbarriers: pieces, a ring of tiles of
+ * K and one of V, S and P, and O.  Every wait is bounded.
  *
  * The (sequence, K/V head, row tile, position tile) quadruples of a call lie on
  * one line, and each CTA takes an equal part of it, wherever that ends inside a
@@ -59,8 +60,9 @@ constexpr int kSoftmax = 128;       /* threads of the softmax */
 enum Load { kTma, kCopy, kWiden };
 template <Load L> struct Roles {
     static constexpr int kLoaders = L == kTma ? 64 : 128;           /* kTma: a warp for K and one for V */
-    static constexpr int kThreads = kSoftmax + kLoaders + 32;
+    static constexpr int kThreads = kSoftmax + kLoaders + 64;       /* a warp for the products, one that plans */
 };
+constexpr int kPlanned = 4;         /* pieces that the planning warp is ahead */
 constexpr int kJoinThreads = 128;
 constexpr int kJoinPieces = 4;      /* pieces whose loads are in flight together */
 constexpr uint32_t kSpinLimit = 1u << 20;
@@ -171,7 +173,7 @@ struct Line {
     uint32_t b;
     Seq s;                          /* sequence b, its tiles per K/V head, and the tiles before it */
 
-    __device__ __noinline__ bool next(const Params &p, Piece &e)
+    __device__ bool next(const Params &p, Piece &e)
     {
         if (x >= hi)
             return false;
@@ -231,6 +233,8 @@ struct Shared {
     uint64_t s_full[2], p_full[2];  /* of tiles in turn */
     uint64_t o_done[2], o_free;     /* O of a tile is complete; O of a piece has been read */
     uint64_t q_full, q_empty;
+    uint64_t planned[kPlanned], taken[kPlanned];
+    Piece pieces[kPlanned];         /* one without tiles ends the work */
     uint32_t tmem;
     volatile uint32_t dead;         /* a wait ran out: every role leaves */
     volatile uint32_t spoilt[4];    /* [piece % 4] == piece + 1: values of its fed nodes that are not finite were set aside */
@@ -274,6 +278,38 @@ __device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint32_t b
 __device__ __forceinline__ bool wait_warp(Shared &sh, int32_t *error, uint64_t *bar, uint32_t parity)
 {
     return wait_warp(sh, error, smem_u32(bar), parity);
+}
+
+/* piece number `piece` of the CTA, for a whole warp; false behind the last one */
+__device__ __forceinline__ bool take(const Params &p, Shared &sh, uint32_t piece, Piece &e)
+{
+    const uint32_t k = piece % kPlanned;
+    if (!wait_warp(sh, p.d.error, &sh.planned[k], piece / kPlanned & 1))
+        return false;
+    e = sh.pieces[k];
+    __syncwarp();
+    if (threadIdx.x % 32 == 0)
+        mbar_arrive(&sh.taken[k]);
+    return e.t1 > e.t0;
+}
+
+/* the planning warp: finding a piece is a chain of loads and divisions, which
+ * the others would wait for (7000 cycles a piece when each did it itself) */
+__device__ __forceinline__ void plan(const Params &p, Shared &sh, Line line)
+{
+    Piece e;
+    for (uint32_t piece = 0, more = 1; more; piece++) {
+        const uint32_t k = piece % kPlanned;
+        more = line.next(p, e);
+        if (!more)
+            e.t0 = e.t1 = 0;
+        if (!wait_warp(sh, p.d.error, &sh.taken[k], piece / kPlanned & 1 ^ 1))
+            return;
+        if (threadIdx.x % 32 == 0) {
+            sh.pieces[k] = e;
+            mbar_arrive(&sh.planned[k]);
+        }
+    }
 }
 
 /* One lane of a converged warp.  What the tensor cores and the TMA are given
@@ -503,7 +539,7 @@ template <typename T, Load L, int DP> struct Loader {
      * behind the end, and those of padding nodes, hold anything: their scores are
      * masked, and softmax makes their values finite.  A page id out of range is
      * out of the map: zeros.  One warp brings K, another V. */
-    __device__ void run_tma(Line line, bool v)
+    __device__ void run_tma(bool v)
     {
         const uint32_t lane = threadIdx.x % 32, boxes = kTile / p.box, box_bytes = p.box * (kColumn * 2);
         const uint32_t slots = uniform(v ? S::kSlotsV : S::kSlotsK), base = uniform(smem_u32(slot(v)));
@@ -511,7 +547,7 @@ template <typename T, Load L, int DP> struct Loader {
         const CUtensorMap *map = v ? &p.v_map : &p.k_map;
         uint32_t at = 0, parity = 1;
         Piece e;
-        while (line.next(p, e)) {
+        for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
             const int32_t *tab = p.d.table + (int64_t)e.row * p.d.table_stride;
             const int32_t t1 = uniform(e.t1), end = uniform(e.end), h = uniform(e.h);
             int32_t pos = e.t0 * kTile + (int32_t)(lane * p.box);
@@ -606,11 +642,11 @@ template <typename T, Load L, int DP> struct Loader {
         }
     }
 
-    __device__ void run_copy(Line line)
+    __device__ void run_copy()
     {
         take_rows();
         Piece e;
-        while (line.next(p, e)) {
+        for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
             const int32_t t1 = e.t1;
             int32_t page = look_up(e, e.t0);
             for (int32_t t = e.t0; t < t1; t++) {
@@ -638,9 +674,8 @@ template <typename T, Load L, int DP> struct Loader {
                (c * kPasses + i) * (128 * 16) + (threadIdx.x - kSoftmax) * 16;
     }
 
-    __device__ bool widen(uint32_t k)
+    __device__ bool widen(uint32_t k, bool v)
     {
-        const bool v = k & 1;
         if (!acquire(v))
             return false;
 #pragma unroll
@@ -663,33 +698,52 @@ template <typename T, Load L, int DP> struct Loader {
         return true;
     }
 
-    __device__ void run_widen(Line line)
+    /* K of a tile comes before V of the tile before: S is needed a softmax
+     * earlier than O, and V's one slot is free only when that O is done */
+    __device__ void run_widen()
     {
         constexpr uint32_t kAhead = S::kRaw > 0 ? S::kRaw - 1 : 0;
         take_rows();
-        uint32_t k = 0, done = 0;           /* tiles of K and V, in turn: fetched, widened */
+        uint32_t k = 0, done = 0;           /* tiles fetched, widened: K, K, V, K, V .. V */
+        uint64_t last[kPasses];
         Piece e;
-        while (line.next(p, e)) {
+        auto fetch = [&](bool v) {
+            copy_tile(v, [&](uint32_t c, int i) { return smem_u32(raw(k, c, i)); });
+            copy_commit();
+            if (k++ < kAhead)
+                return true;
+            copy_wait_but<kAhead>();
+            done++;
+            return widen(done - 1, done > 1 && (done & 1));
+        };
+        auto swap = [&] {
+#pragma unroll
+            for (int i = 0; i < kPasses; i++) {
+                const uint64_t o = off[i];
+                off[i] = last[i];
+                last[i] = o;
+            }
+        };
+        for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
             const int32_t t1 = e.t1;
             int32_t page = look_up(e, e.t0);
             for (int32_t t = e.t0; t < t1; t++) {
                 places(e, t, page);
                 if (t + 1 < t1)
                     page = look_up(e, t + 1);
-                for (int v = 0; v < 2; v++, k++) {
-                    copy_tile(v, [&](uint32_t c, int i) { return smem_u32(raw(k, c, i)); });
-                    copy_commit();
-                    if (k >= kAhead) {
-                        copy_wait_but<kAhead>();
-                        if (!widen(done++))
-                            return;
-                    }
-                }
+                if (!fetch(false))
+                    return;
+                swap();
+                if (k > 1 && !fetch(true))
+                    return;
             }
         }
+        swap();                             /* V of the last tile */
+        if (k && !fetch(true))
+            return;
         copy_wait_all();
-        while (done < k)
-            if (!widen(done++))
+        for (; done < k; done++)
+            if (!widen(done, done > 0 && (!(done & 1) || done + 1 == k)))
                 return;
     }
 };
@@ -714,7 +768,7 @@ __device__ __forceinline__ void load_q(const Params &p, Shared &sh, uint8_t *q_s
 }
 
 template <typename T, Load L, int DP>
-__device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *ring, Line line)
+__device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *ring)
 {
     using S = Shape<L, DP>;
     const uint32_t dim = p.d.head_dim, s = uniform(sh.tmem), o = s + 2 * kTile;
@@ -725,7 +779,7 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
     Turn<S::kSlotsV> at_v;
     uint32_t g = 0, piece = 0;
     Piece e;
-    bool more = line.next(p, e);
+    bool more = take(p, sh, 0, e);
     /* S of a tile; the last of its piece also releases Q */
     auto scores = [&](uint32_t tile, bool last) {
         if (!wait_warp(sh, p.d.error, &sh.k_full[at_k.slot], at_k.lap & 1))
@@ -759,7 +813,7 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
             if (k + 1 < n && !scores(g + 1, k + 2 == n))
                 return;
             if (k + 1 == n) {
-                more = line.next(p, e);
+                more = take(p, sh, piece + 1, e);
                 if (!wait_warp(sh, p.d.error, &sh.q_empty, piece & 1))
                     return;
                 if (uniform(more))
@@ -897,7 +951,7 @@ __device__ __forceinline__ void hide(float *s, uint32_t bits)
 }
 
 template <typename T, Load L, int DP>
-__device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
+__device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
 {
     using S = Shape<L, DP>;
     const kv_attn_desc &d = p.d;
@@ -908,7 +962,7 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring, Line line)
     uint32_t g = 0, piece = 0;
     Turn<S::kSlotsV> at_v;
     Piece e;
-    for (; line.next(p, e); piece++) {
+    for (; take(p, sh, piece, e); piece++) {
         const bool valid = (int32_t)tid < e.rows(p);
         const int32_t node = valid ? e.node0 + my_node : 0;
         bool active = valid;
@@ -1169,6 +1223,10 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
             mbar_init(&sh.p_full[k], kSoftmax / 32);
             mbar_init(&sh.o_done[k], 1);
         }
+        for (int k = 0; k < kPlanned; k++) {
+            mbar_init(&sh.planned[k], 1);
+            mbar_init(&sh.taken[k], kThreads / 32 - 1);
+        }
         mbar_init(&sh.o_free, kSoftmax / 32);
         mbar_init(&sh.q_full, 1);
         mbar_init(&sh.q_empty, 1);
@@ -1189,21 +1247,22 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const Line line = sh.line;
     if (smem_u32(smem) % 1024 == 0) {
         if (warp < kSoftmax / 32) {
-            softmax<T, L, DP>(p, sh, ring, line);
-        } else if (warp < kThreads / 32 - 1) {
+            softmax<T, L, DP>(p, sh, ring);
+        } else if (warp < kThreads / 32 - 2) {
             Loader<T, L, DP> load(p, sh, ring);
             if constexpr (L == kTma) {
-                load.run_tma(line, warp != kSoftmax / 32);
+                load.run_tma(warp != kSoftmax / 32);
             } else if constexpr (L == kWiden)
-                load.run_widen(line);
+                load.run_widen();
             else
-                load.run_copy(line);
+                load.run_copy();
             copy_wait_all();
+        } else if (warp == kThreads / 32 - 2) {
+            products<T, L, DP>(p, sh, q_smem, ring);
         } else {
-            products<T, L, DP>(p, sh, q_smem, ring, line);
+            plan(p, sh, sh.line);
         }
     } else if (threadIdx.x == 0) {
         atomicOr(p.d.error, KVATTN_ERR_TIMEOUT);
@@ -1474,7 +1533,7 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
     const uint64_t mean = ((uint64_t)d->total_q * p.group + d->num_seqs - 1) / d->num_seqs;
     const uint32_t rows = (uint32_t)(mean < kRows ? mean : kRows);
     p.min_share = 1 + rows / 32;
-    p.join_ctas = (rows * d->head_dim / 4 + 2 * kJoinThreads - 1) / (2 * kJoinThreads);    /* two of a thread's shares each */
+    p.join_ctas = (rows * d->head_dim / 4 + 4 * kJoinThreads - 1) / (4 * kJoinThreads);    /* four of a thread's shares each */
     p.wide_out = (uintptr_t)d->out % 32 == 0 && (d->out_stride | d->out_head_stride) % 16 == 0;
     char *base = static_cast<char *>(d->workspace);
     p.jobs = reinterpret_cast<Job *>(base + w.jobs);
