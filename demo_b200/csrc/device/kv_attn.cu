@@ -63,8 +63,8 @@ template <Load L> struct Roles {
     static constexpr int kThreads = kSoftmax + kLoaders + 64;       /* a warp for the products, one that plans */
 };
 constexpr int kPlanned = 4;         /* pieces that the planning warp is ahead */
-constexpr int kJoinThreads = 128;
-constexpr int kJoinPieces = 4;      /* pieces whose loads are in flight together */
+constexpr int kJoinThreads = 256;
+constexpr int kMaxCtas = 512;       /* of the first kernel */
 constexpr uint32_t kSpinLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -101,7 +101,6 @@ struct Params {
     uint32_t columns;       /* of Q, K and V */
     uint32_t box;
     uint32_t min_share;     /* tiles that a CTA takes at least */
-    uint32_t join_ctas;     /* that join a row tile */
     uint32_t wide_out;      /* rows of out start on 32 bytes */
     Job *jobs;              /* workspace: [CTAs] row tiles to be joined, by the CTA that has their first tiles */
     float *part_ml;         /* [2 * CTAs][128][2] maximum and sum of a piece */
@@ -1278,58 +1277,140 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
 }
 
 /* ------------------------------------------------------------------------
- * join: the pieces of a row tile that lies across CTAs, in an order that only
- * the sizes set.
+ * join: the pieces of the row tiles that lie across CTAs, in their order.  The
+ * tiles' rows, however many each has, are dealt evenly to the grid's warps; a
+ * lane has four dimensions of a row, and eight loads are in flight.
+ * (Joining in the first kernel, by the CTA that finishes a row tile last, takes
+ * no second launch but left long joins to a few CTAs: 424 us instead of 98 for
+ * 8 contexts in 37 pieces each.)
  * ---------------------------------------------------------------------- */
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid_constant__ Params p)
+/* rows r0 .. r1 of a job, R rows and P pieces in flight together */
+template <typename T, int R, int P>
+__device__ __forceinline__ void join_rows(const Params &p, const Job &job, uint32_t cta, int32_t r0, int32_t r1, uint32_t lane)
 {
     const kv_attn_desc &d = p.d;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Job job = p.jobs[blockIdx.x];
-    const int32_t quads = d.head_dim / 4;
-    /* a thread has four dimensions of a row */
-    for (int32_t x = blockIdx.y * kJoinThreads + threadIdx.x; x < job.rows * quads; x += gridDim.y * kJoinThreads) {
-        const int32_t r = x / quads, c = (x - r * quads) * 4;
-        /* piece k's row: the first piece's slot, then slot 0 of the CTAs behind */
-        auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (blockIdx.x + k) : (uint32_t)job.slot) * kRows + r; };
-        float m = -INFINITY, l = 0;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int32_t k0 = 0; k0 < job.ctas; k0 += kJoinPieces) {
-            float2 ml[kJoinPieces];
-            float4 v[kJoinPieces];
-            float top = m;
+    /* piece k's rows: the first piece's slot, then slot 0 of the CTAs behind */
+    auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (cta + k) : (uint32_t)job.slot) * kRows; };
+    for (uint32_t c = lane * 4; c < d.head_dim; c += 128)
+#pragma unroll 1
+        for (int32_t r = r0; r < r1; r += R) {
+            float m[R], l[R];
+            float4 o[R];
 #pragma unroll
-            for (int k = 0; k < kJoinPieces; k++) {     /* all loads first */
-                const bool on = k0 + k < job.ctas;
-                ml[k] = on ? *reinterpret_cast<const float2 *>(p.part_ml + at(k0 + k) * 2) : make_float2(0, 0);
-                v[k] = on ? *reinterpret_cast<const float4 *>(p.part_o + at(k0 + k) * d.head_dim + c) : make_float4(0, 0, 0, 0);
+            for (int i = 0; i < R; i++) {
+                m[i] = -INFINITY;
+                l[i] = 0;
+                o[i] = make_float4(0, 0, 0, 0);
+            }
+#pragma unroll 1
+            for (int32_t k0 = 0; k0 < job.ctas; k0 += P) {
+                float2 ml[R][P];
+                float4 v[R][P];
+#pragma unroll
+                for (int k = 0; k < P; k++)
+#pragma unroll
+                    for (int i = 0; i < R; i++) {
+                        const bool on = k0 + k < job.ctas && r + i < r1;
+                        const uint64_t row = at(k0 + k) + r + i;
+                        ml[i][k] = on ? *reinterpret_cast<const float2 *>(p.part_ml + row * 2) : make_float2(0, 0);
+                        v[i][k] = on ? *reinterpret_cast<const float4 *>(p.part_o + row * d.head_dim + c) : make_float4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    float top = m[i];
+#pragma unroll
+                    for (int k = 0; k < P; k++)
+                        if (ml[i][k].y != 0)    /* else it sees nothing there, and its sums were not written */
+                            top = fmaxf(top, ml[i][k].x);
+                    if (top == -INFINITY)
+                        continue;
+                    const float keep = exp2_approx(m[i] - top);
+                    m[i] = top;
+                    l[i] *= keep;
+                    o[i] = make_float4(o[i].x * keep, o[i].y * keep, o[i].z * keep, o[i].w * keep);
+#pragma unroll
+                    for (int k = 0; k < P; k++) {
+                        if (ml[i][k].y == 0)
+                            continue;
+                        const float f = exp2_approx(ml[i][k].x - top);
+                        l[i] += f * ml[i][k].y;
+                        o[i] = make_float4(o[i].x + f * v[i][k].x, o[i].y + f * v[i][k].y, o[i].z + f * v[i][k].z, o[i].w + f * v[i][k].w);
+                    }
+                }
             }
 #pragma unroll
-            for (int k = 0; k < kJoinPieces; k++)
-                if (ml[k].y != 0)                       /* else it sees nothing there, and its sums were not written */
-                    top = fmaxf(top, ml[k].x);
-            if (top == -INFINITY)
-                continue;
-            const float keep = exp2f(m - top);
-            m = top;
-            l *= keep;
-            o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-#pragma unroll
-            for (int k = 0; k < kJoinPieces; k++) {
-                if (ml[k].y == 0)
-                    continue;
-                const float f = exp2f(ml[k].x - m);
-                l += f * ml[k].y;
-                o = make_float4(o.x + f * v[k].x, o.y + f * v[k].y, o.z + f * v[k].z, o.w + f * v[k].w);
+            for (int i = 0; i < R; i++) {
+                if (r + i >= r1)
+                    break;
+                const int32_t node = (r + i) / (int32_t)p.group, sub = r + i - node * (int32_t)p.group;
+                const float inv = l[i] == 0 ? 0.f : d.v_scale / l[i];
+                T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
+                *reinterpret_cast<uint2 *>(out + c) =
+                    make_uint2(Type<T>::pack(o[i].x * inv, o[i].y * inv), Type<T>::pack(o[i].z * inv, o[i].w * inv));
+                if (c == 0 && d.lse)
+                    d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] =
+                        l[i] == 0 ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
             }
         }
-        const int32_t node = r / (int32_t)p.group, sub = r - node * (int32_t)p.group;
-        const float inv = l == 0 ? 0.f : d.v_scale / l;
-        T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
-        *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(o.x * inv, o.y * inv), Type<T>::pack(o.z * inv, o.w * inv));
-        if (c == 0 && d.lse)
-            d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] = l == 0 ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid_constant__ Params p, uint32_t ctas)
+{
+    __shared__ int32_t upto[kMaxCtas], warp_sum[kJoinThreads / 32];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    /* rows before and with each job's */
+    constexpr int kEach = kMaxCtas / kJoinThreads;
+    int32_t rows[kEach], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const uint32_t c = threadIdx.x * kEach + k;
+        rows[k] = c < ctas ? p.jobs[c].rows : 0;
+        sum += rows[k];
+    }
+    int32_t inc = sum;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+        const int32_t u = __shfl_up_sync(~0u, inc, k);
+        if (lane >= (uint32_t)k)
+            inc += u;
+    }
+    if (lane == 31)
+        warp_sum[warp] = inc;
+    __syncthreads();
+    int32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kJoinThreads / 32; k++) {
+        if (k < (int)warp)
+            inc += warp_sum[k];
+        total += warp_sum[k];
+    }
+    inc -= sum;
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        upto[threadIdx.x * kEach + k] = inc += rows[k];
+    __syncthreads();
+    const int32_t warps = gridDim.x * (kJoinThreads / 32), each = (total + warps - 1) / warps;
+    int32_t u = (blockIdx.x * (kJoinThreads / 32) + warp) * each;
+    const int32_t end = min(total, u + each);
+    while (u < end) {
+        uint32_t lo = 0, hi = ctas - 1;         /* the job whose rows go past u */
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (upto[mid] > u)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        const Job job = p.jobs[lo];
+        const int32_t r0 = u - (upto[lo] - job.rows), r1 = min(job.rows, r0 + end - u);
+        /* most have two pieces: then four rows together */
+        if (job.ctas == 2)
+            join_rows<T, 4, 2>(p, job, lo, r0, r1, lane);
+        else
+            join_rows<T, 1, 8>(p, job, lo, r0, r1, lane);
+        u += r1 - r0;
     }
 }
 
@@ -1357,7 +1438,7 @@ int grid_of(const kv_attn_desc *d)
         int n = 0;
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d->device) != cudaSuccess)
             cudaGetLastError();
-        sms[d->device] = n > 0 ? n : 148;
+        sms[d->device] = n > 0 ? (n < kMaxCtas / 2 ? n : kMaxCtas / 2) : 148;
     });
     return sms[d->device] * (d->head_dim <= 128 ? 2 : 1);
 }
@@ -1450,14 +1531,14 @@ int launch(const Params &p, cudaStream_t stream)
     /* started while the first kernel drains; it waits for its results on the device */
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(grid, p.join_ctas);
+    cfg.gridDim = dim3(2 * grid);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<T>, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, kv_attn_join_kernel<T>, p, grid) != cudaSuccess) {
         cudaGetLastError();
         return -EIO;
     }
@@ -1533,7 +1614,6 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
     const uint64_t mean = ((uint64_t)d->total_q * p.group + d->num_seqs - 1) / d->num_seqs;
     const uint32_t rows = (uint32_t)(mean < kRows ? mean : kRows);
     p.min_share = 1 + rows / 32;
-    p.join_ctas = (rows * d->head_dim / 4 + 4 * kJoinThreads - 1) / (4 * kJoinThreads);    /* four of a thread's shares each */
     p.wide_out = (uintptr_t)d->out % 32 == 0 && (d->out_stride | d->out_head_stride) % 16 == 0;
     char *base = static_cast<char *>(d->workspace);
     p.jobs = reinterpret_cast<Job *>(base + w.jobs);
