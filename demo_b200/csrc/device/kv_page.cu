@@ -14,6 +14,7 @@
 #include "kvpage.h"
 #include "adaptor.h"
 #include "device_guard.h"
+#include "fastdiv.h"
 
 #include <cuda_runtime.h>
 
@@ -23,9 +24,10 @@
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanThreads = 1024;          /* at most; 256 for small calls, whose time is barriers and loads */
 constexpr uint32_t kPlanCluster = 8;
+constexpr uint32_t kUnit = 128;             /* table entries that a warp takes together, four to a lane */
+constexpr uint32_t kMaxUnits = 2 * KVPAGE_MAX_CALL;
 constexpr int32_t kRefused = INT32_MIN;     /* compact's length for resize of a row that it has refused and reported */
 
 /* ---- the cluster's barrier and shared memory ---- */
@@ -56,51 +58,47 @@ __device__ __forceinline__ void store_cluster(int32_t *p, uint32_t rank, int32_t
     asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(b), "r"(v) : "memory");
 }
 
-/* exclusive prefix sum of a[0 .. n) in place, n <= KVPAGE_MAX_CALL; returns
- * the total to every thread.  Each thread sums 4 consecutive values. */
-__device__ int32_t block_scan(int32_t *a, uint32_t n)
+/* Exclusive prefix sums of K arrays of n values each in place, n <= kMaxUnits;
+ * total[k] is array k's sum.  A thread sums consecutive values. */
+template <int K> __device__ __noinline__ void block_scan(int32_t *const *a, uint32_t n, int32_t *total)
 {
-    __shared__ int32_t warp_sum[kPlanWarps];
-    static_assert(KVPAGE_MAX_CALL == 4 * kPlanThreads, "four values per thread");
-    const uint32_t i0 = threadIdx.x * 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int32_t v[4], sum = 0;
+    __shared__ int32_t warp_sum[K][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const uint32_t each = (n + blockDim.x - 1) / blockDim.x, i0 = min(n, threadIdx.x * each), i1 = min(n, i0 + each);
+    int32_t sum[K], inc[K];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        v[k] = i0 + k < n ? a[i0 + k] : 0;
-        sum += v[k];
+    for (int k = 0; k < K; k++) {
+        sum[k] = 0;
+        for (uint32_t i = i0; i < i1; i++)
+            sum[k] += a[k][i];
+        inc[k] = sum[k];
     }
-    int32_t inc = sum;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        int32_t o = __shfl_up_sync(~0u, inc, d);
-        if (lane >= d)
-            inc += o;
-    }
-    if (lane == 31)
-        warp_sum[warp] = inc;
-    __syncthreads();
-    if (warp == 0) {
-        int32_t w = warp_sum[lane];
+    for (int d = 1; d < 32; d <<= 1)
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            int32_t o = __shfl_up_sync(~0u, w, d);
+        for (int k = 0; k < K; k++) {
+            const int32_t o = __shfl_up_sync(~0u, inc[k], d);
             if (lane >= d)
-                w += o;
+                inc[k] += o;
         }
-        warp_sum[lane] = w;
-    }
-    __syncthreads();
-    int32_t run = inc - sum + (warp ? warp_sum[warp - 1] : 0);
-    const int32_t total = warp_sum[kPlanWarps - 1];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        if (i0 + k < n)
-            a[i0 + k] = run;
-        run += v[k];
+    for (int k = 0; k < K; k++)
+        if (lane == 31)
+            warp_sum[k][warp] = inc[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int32_t w = lane < warps ? warp_sum[k][lane] : 0;
+        int32_t run = inc[k] - sum[k] + __reduce_add_sync(~0u, lane < warp ? w : 0);
+        total[k] = __reduce_add_sync(~0u, w);
+        for (uint32_t i = i0; i < i1; i++) {
+            const int32_t v = a[k][i];
+            a[k][i] = run;
+            run += v;
+        }
     }
     __syncthreads();
-    return total;
 }
 
 /* sets bit r; true if it was set already */
@@ -126,54 +124,74 @@ __device__ __forceinline__ int32_t free_pages(const kv_page_state &s)
     return min(max(c, 0), (int32_t)s.num_pages);
 }
 
+/* the row that unit u of the prefix sums `first` belongs to */
+__device__ __forceinline__ uint32_t row_of(const int32_t *first, uint32_t n, int32_t u)
+{
+    uint32_t lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (first[mid] <= u)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
 /* ------------------------------------------------------------------------
  * resize.  Entry k of the call's row i has the number i * width + k, and a
  * dropped page's place in the push order is its highest number:
  *   A  every dropped entry takes one reference off its page and raises the
  *      page's mark to its number + 1 (both commute: any order, same result)
  *   B  the entry whose number the mark holds, of a page without references,
- *      stands for the page; warps count these row by row, the counts go to
+ *      stands for the page; warps count these unit by unit, the counts go to
  *      every CTA's shared memory, and each CTA scans them
  *   C  those entries push their pages
  *   D  growing rows pop, marks go back to zero, lengths and counts are written
- * with a cluster barrier between phases.  A warp owns a row.  A reference is
- * taken back where a page had none left, so a page freed twice is neither
- * pushed twice nor left negative.
+ * with a cluster barrier between phases.  What is dropped or taken is cut into
+ * units of 128 entries of a row (more where that would be too many units), so
+ * that a lane has four loads or atomics in flight and long rows are shared by
+ * warps: with a warp per row and an entry per lane, replacing 256 rows of 170
+ * pages took 44 us.  A reference is taken back where a page had none left, so a
+ * page freed twice is neither pushed twice nor left negative.
  * ---------------------------------------------------------------------- */
 __global__ void __launch_bounds__(kPlanThreads, 1)
 kv_page_resize_kernel(const kv_page_state s, const int32_t *__restrict__ rows, const int32_t *__restrict__ lens,
                       uint32_t n, int32_t *__restrict__ status)
 {
     extern __shared__ int32_t sm[];
-    int32_t *row = sm, *old_p = sm + n, *new_p = sm + 2 * n, *need = sm + 3 * n, *gone = sm + 4 * n;
+    int32_t *row = sm, *old_p = sm + n, *new_p = sm + 2 * n, *need = sm + 3 * n;
+    int32_t *drops = sm + 4 * n, *takes = sm + 5 * n;       /* units of the rows before */
     const uint32_t words = (s.num_rows + 31) / 32;
-    uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 5 * n), *twice = seen + words;
-    __shared__ int32_t served;
+    uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 6 * n), *twice = seen + words;
+    int32_t *gone = sm + 6 * n + 2 * words;                 /* pages pushed by the units before */
+    __shared__ int32_t served, all_drop, all_take;
     const uint32_t rank = cluster_rank(), ctas = cluster_size();
-    const uint32_t lane = threadIdx.x & 31, warp0 = rank * kPlanWarps + (threadIdx.x >> 5), warps = ctas * kPlanWarps;
+    const uint32_t lane = threadIdx.x & 31, warp0 = rank * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = ctas * (blockDim.x >> 5);
 
-    for (uint32_t i = threadIdx.x; i < 2 * words; i += kPlanThreads)
+    for (uint32_t i = threadIdx.x; i < 2 * words; i += blockDim.x)
         seen[i] = 0;
     if (threadIdx.x == 0)
-        served = 0;
+        served = all_drop = all_take = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const int32_t r = rows[i];
         row[i] = r;
         if (r >= 0 && (uint32_t)r < s.num_rows && test_and_set(seen, r))
             test_and_set(twice, r);
     }
+    const int32_t count = free_pages(s);
     __syncthreads();
-    bool drop = false;
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    int32_t drop = 0, take = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const int32_t r = row[i], to = lens[i];
-        bool ok = r >= 0 && (uint32_t)r < s.num_rows && !test_bit(twice, r) && to >= 0;
+        bool ok = r >= 0 && (uint32_t)r < s.num_rows && to >= 0;
         uint32_t a = 0, b = 0;
         if (ok) {
             const int32_t from = s.lens[r];
             a = pages_of(max(from, 0), s.block_size);
             b = pages_of(to, s.block_size);
-            ok = from >= 0 && a <= s.width && b <= s.width;
+            ok = !test_bit(twice, r) && from >= 0 && a <= s.width && b <= s.width;
         }
         if (!ok) {
             if (rank == 0 && to != kRefused)
@@ -184,113 +202,225 @@ kv_page_resize_kernel(const kv_page_state s, const int32_t *__restrict__ rows, c
         old_p[i] = a;
         new_p[i] = b;
         need[i] = b > a ? b - a : 0;
-        gone[i] = 0;
-        drop |= b < a;
+        drop += a > b ? a - b : 0;
+        take += need[i];
     }
-    const int32_t count = free_pages(s);
-    drop = __syncthreads_or(drop);
-    int32_t pushed = 0;
-    if (drop) {
-        for (uint32_t i = warp0; i < n; i += warps) {
-            const int32_t *t = s.table + (int64_t)max(row[i], 0) * s.table_stride;
-            for (int32_t k = new_p[i] + (int32_t)lane; k < old_p[i]; k += 32) {
-                const int32_t p = t[k];
-                if (p < 0 || (uint32_t)p >= s.num_pages) {
-                    atomicOr(s.error, KVPAGE_ERR_PAGE);
+    if (drop)
+        atomicAdd(&all_drop, drop);
+    if (take)
+        atomicAdd(&all_take, take);
+    __syncthreads();
+    /* entries of a unit: at most as many units of n rows as kMaxUnits holds */
+    uint32_t unit = kUnit;
+    while ((uint32_t)max(all_drop, all_take) / unit > kMaxUnits - KVPAGE_MAX_CALL)
+        unit *= 2;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const int32_t d = old_p[i] - new_p[i];
+        drops[i] = d > 0 ? (d + unit - 1) / unit : 0;
+        takes[i] = (need[i] + unit - 1) / unit;
+    }
+    int32_t total[3], pushed = 0;
+    {
+        int32_t *arrays[3] = {drops, takes, need};
+        block_scan<3>(arrays, n, total);
+    }
+    const int32_t drop_units = total[0], take_units = total[1];
+    if (drop_units > 0 && drop_units <= (int32_t)warps && unit == kUnit) {
+        /* a unit per warp: its pages stay in registers from phase to phase */
+        const bool mine = warp0 < (uint32_t)drop_units;
+        int32_t page[4], number = 0, c = 0;
+        uint32_t on = 0, stands = 0;
+        if (mine) {
+            const uint32_t i = row_of(drops, n, warp0);
+            const int32_t k = new_p[i] + (warp0 - drops[i]) * (int32_t)kUnit + (int32_t)lane;
+            const int32_t *t = s.table + (int64_t)row[i] * s.table_stride;
+            number = (int32_t)(i * s.width) + k + 1;
+            int32_t had[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                page[j] = k + 32 * j < old_p[i] ? t[k + 32 * j] : 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (k + 32 * j >= old_p[i])
                     continue;
-                }
-                if (atomicSub(&s.refs[p], 1) >= 1) {
-                    atomicMax(&s.marks[p], (int32_t)(i * s.width) + k + 1);
+                if (page[j] >= 0 && (uint32_t)page[j] < s.num_pages) {
+                    on |= 1u << j;
+                    had[j] = atomicSub(&s.refs[page[j]], 1);
                 } else {
-                    atomicAdd(&s.refs[p], 1);
+                    atomicOr(s.error, KVPAGE_ERR_PAGE);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (!(on >> j & 1))
+                    continue;
+                if (had[j] >= 1) {
+                    atomicMax(&s.marks[page[j]], number + 32 * j);
+                } else {
+                    atomicAdd(&s.refs[page[j]], 1);
                     atomicOr(s.error, KVPAGE_ERR_REFS);
                 }
             }
         }
         cluster_sync();
-        auto stands = [&](uint32_t i, int32_t k, const int32_t *t, int32_t &p) {
-            if (k >= old_p[i])
-                return false;
-            p = t[k];
-            return p >= 0 && (uint32_t)p < s.num_pages && __ldcg(&s.marks[p]) == (int32_t)(i * s.width) + k + 1 &&
-                   __ldcg(&s.refs[p]) == 0;
-        };
-        for (uint32_t i = warp0; i < n; i += warps) {
-            if (new_p[i] >= old_p[i])
-                continue;
-            const int32_t *t = s.table + (int64_t)row[i] * s.table_stride;
-            int32_t c = 0, p;
-            for (int32_t k = new_p[i] + (int32_t)lane; k - (int32_t)lane < old_p[i]; k += 32)
-                c += stands(i, k, t, p);
-            c = __reduce_add_sync(~0u, c);
+        if (mine) {
+            int32_t mark[4], refs[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                mark[j] = on >> j & 1 ? __ldcg(&s.marks[page[j]]) : 0;
+                refs[j] = on >> j & 1 ? __ldcg(&s.refs[page[j]]) : 1;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                stands |= (uint32_t)(mark[j] == number + 32 * j && refs[j] == 0) << j;
+            c = __reduce_add_sync(~0u, __popc(stands));
             if (lane < ctas)
-                store_cluster(&gone[i], lane, c);
+                store_cluster(&gone[warp0], lane, c);
         }
         cluster_sync();
-        pushed = block_scan(gone, n);
-        for (uint32_t i = warp0; i < n; i += warps) {
-            if (new_p[i] >= old_p[i])
-                continue;
-            const int32_t *t = s.table + (int64_t)row[i] * s.table_stride;
-            int32_t at = count + gone[i];
-            for (int32_t k = new_p[i] + (int32_t)lane; k - (int32_t)lane < old_p[i]; k += 32) {
-                int32_t p = 0;
-                const bool mine = stands(i, k, t, p);
-                const uint32_t m = __ballot_sync(~0u, mine);
-                const int32_t place = at + __popc(m & ((1u << lane) - 1));
-                if (mine && (uint32_t)place < s.num_pages)
-                    s.free_list[place] = p;
-                at += __popc(m);
+        {
+            int32_t *arrays[1] = {gone};
+            block_scan<1>(arrays, drop_units, &pushed);
+        }
+        if (mine) {
+            int32_t place = count + gone[warp0];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t m = __ballot_sync(~0u, stands >> j & 1);
+                const int32_t at = place + __popc(m & ((1u << lane) - 1));
+                if ((stands >> j & 1) && (uint32_t)at < s.num_pages)
+                    s.free_list[at] = page[j];
+                place += __popc(m);
             }
         }
+        cluster_sync();
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (on >> j & 1)
+                s.marks[page[j]] = 0;
+    } else if (drop_units) {
+        /* the same in one loop over the warp's units for the four phases */
+#pragma unroll 1
+        for (int phase = 0; phase < 4; phase++) {
+            if (phase)
+                cluster_sync();
+            if (phase == 2) {
+                int32_t *arrays[1] = {gone};
+                block_scan<1>(arrays, drop_units, &pushed);
+            }
+#pragma unroll 1
+            for (int32_t u = warp0; u < drop_units; u += warps) {
+                const uint32_t i = row_of(drops, n, u);
+                const int32_t *t = s.table + (int64_t)row[i] * s.table_stride;
+                const int32_t k0 = new_p[i] + (u - drops[i]) * (int32_t)unit, k1 = min(old_p[i], k0 + (int32_t)unit);
+                int32_t c = 0;
+#pragma unroll 1
+                for (int32_t k = k0 + lane; k - (int32_t)lane < k1; k += kUnit) {
+                    const int32_t number = (int32_t)(i * s.width) + k + 1;
+                    int32_t page[4], mark[4], refs[4];
+                    bool on[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        page[j] = k + 32 * j < k1 ? t[k + 32 * j] : 0;
+                        on[j] = k + 32 * j < k1 && page[j] >= 0 && (uint32_t)page[j] < s.num_pages;
+                    }
+                    if (phase == 0) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if (on[j])
+                                refs[j] = atomicSub(&s.refs[page[j]], 1);
+                            else if (k + 32 * j < k1)
+                                atomicOr(s.error, KVPAGE_ERR_PAGE);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if (!on[j])
+                                continue;
+                            if (refs[j] >= 1) {
+                                atomicMax(&s.marks[page[j]], number + 32 * j);
+                            } else {
+                                atomicAdd(&s.refs[page[j]], 1);
+                                atomicOr(s.error, KVPAGE_ERR_REFS);
+                            }
+                        }
+                    } else if (phase == 3) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (on[j])
+                                s.marks[page[j]] = 0;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            mark[j] = on[j] ? __ldcg(&s.marks[page[j]]) : 0;
+                            refs[j] = on[j] ? __ldcg(&s.refs[page[j]]) : 1;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const bool stands = mark[j] == number + 32 * j && refs[j] == 0;
+                            const uint32_t m = __ballot_sync(~0u, stands);
+                            if (phase == 2) {
+                                const int32_t place = count + gone[u] + c + __popc(m & ((1u << lane) - 1));
+                                if (stands && (uint32_t)place < s.num_pages)
+                                    s.free_list[place] = page[j];
+                            }
+                            c += __popc(m);
+                        }
+                    }
+                }
+                if (phase == 1 && lane < ctas)
+                    store_cluster(&gone[u], lane, c);
+            }
+        }
+    } else {
+        cluster_sync();             /* every CTA has read the lengths and the count */
     }
     const int32_t have = min(count + pushed, (int32_t)s.num_pages);
-    block_scan(need, n);
-    cluster_sync();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
-        const int32_t want = new_p[i] - old_p[i];
-        if (want > 0 && need[i] + want <= have)
-            atomicMax(&served, need[i] + want);
-    }
-    for (uint32_t i = warp0; i < n; i += warps) {
-        const int32_t r = row[i];
-        if (r < 0) {
-            if (lane == 0 && status)
-                status[i] = KVPAGE_INVALID;
-            continue;
-        }
-        int32_t *t = s.table + (int64_t)r * s.table_stride;
-        const int32_t want = new_p[i] - old_p[i];
-        const bool fits = want <= 0 || need[i] + want <= have;
-        for (int32_t k = new_p[i] + (int32_t)lane; k < old_p[i]; k += 32) {
-            const int32_t p = t[k];
-            if (p >= 0 && (uint32_t)p < s.num_pages)
-                s.marks[p] = 0;
-        }
-        if (fits)
-            for (int32_t k = lane; k < want; k += 32) {
-                const int32_t p = __ldcg(&s.free_list[have - 1 - need[i] - k]);
-                t[old_p[i] + k] = p;
-                if (p >= 0 && (uint32_t)p < s.num_pages)
-                    s.refs[p] = 1;
-                else
-                    atomicOr(s.error, KVPAGE_ERR_PAGE);
+    {
+#pragma unroll 1
+        for (int32_t u = warp0; u < take_units; u += warps) {
+            const uint32_t i = row_of(takes, n, u);
+            const int32_t want = new_p[i] - old_p[i], k0 = (u - takes[i]) * (int32_t)unit, k1 = min(want, k0 + (int32_t)unit);
+            if (need[i] + want > have)
+                continue;
+            int32_t *t = s.table + (int64_t)row[i] * s.table_stride + old_p[i];
+#pragma unroll 1
+            for (int32_t k = k0 + lane; k < k1; k += kUnit) {
+                int32_t page[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    page[j] = k + 32 * j < k1 ? __ldcg(&s.free_list[have - 1 - need[i] - k - 32 * j]) : 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (k + 32 * j < k1) {
+                        t[k + 32 * j] = page[j];
+                        if (page[j] >= 0 && (uint32_t)page[j] < s.num_pages)
+                            s.refs[page[j]] = 1;
+                        else
+                            atomicOr(s.error, KVPAGE_ERR_PAGE);
+                    }
             }
-        if (lane == 0) {
-            if (fits)
-                s.lens[r] = lens[i];
-            if (status)
-                status[i] = fits ? KVPAGE_OK : KVPAGE_NO_PAGES;
         }
+    }
+    if (rank)
+        return;
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const int32_t r = row[i], want = new_p[i] - old_p[i];
+        const bool fits = want <= 0 || need[i] + want <= have;
+        if (want > 0 && fits)
+            atomicMax(&served, need[i] + want);
+        if (r >= 0 && fits)
+            s.lens[r] = lens[i];
+        if (status)
+            status[i] = r < 0 ? KVPAGE_INVALID : fits ? KVPAGE_OK : KVPAGE_NO_PAGES;
     }
     __syncthreads();
-    if (rank == 0 && threadIdx.x == 0)
+    if (threadIdx.x == 0)
         *s.free_count = have - served;
 }
 
 /* ------------------------------------------------------------------------
  * fork's plan: what each child gets, the tables and the references; the pages
- * to copy go to pairs[3 * i] = (source, destination, tokens), source -1 where
+ * to copy go to pairs[3 * i] = (source, destination, tokens), 0 tokens where
  * there is nothing to copy.  One cluster, a warp per child.
  * ---------------------------------------------------------------------- */
 __global__ void __launch_bounds__(kPlanThreads, 1)
@@ -303,14 +433,14 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
     uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 4 * n), *twice = seen + words, *parent = seen + 2 * words;
     __shared__ int32_t served;
     const uint32_t rank = cluster_rank(), ctas = cluster_size();
-    const uint32_t lane = threadIdx.x & 31, warp0 = rank * kPlanWarps + (threadIdx.x >> 5), warps = ctas * kPlanWarps;
+    const uint32_t lane = threadIdx.x & 31, warp0 = rank * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = ctas * (blockDim.x >> 5);
 
-    for (uint32_t i = threadIdx.x; i < 3 * words; i += kPlanThreads)
+    for (uint32_t i = threadIdx.x; i < 3 * words; i += blockDim.x)
         seen[i] = 0;
     if (threadIdx.x == 0)
         served = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const int32_t p = parents[i], c = children[i];
         from[i] = p;
         child[i] = c;
@@ -320,7 +450,7 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
             test_and_set(twice, c);
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const int32_t p = from[i], c = child[i];
         bool ok = p >= 0 && (uint32_t)p < s.num_rows && c >= 0 && (uint32_t)c < s.num_rows && !test_bit(twice, c) &&
                   !test_bit(parent, c);
@@ -339,9 +469,11 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
         need[i] = len % (int32_t)s.block_size != 0;
     }
     const int32_t have = free_pages(s);
-    block_scan(need, n);
+    int32_t wanted;
+    int32_t *arrays[1] = {need};
+    block_scan<1>(arrays, n, &wanted);
     cluster_sync();                 /* every CTA has read the lengths and the count */
-    for (uint32_t i = threadIdx.x; i < n; i += kPlanThreads)
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
         if (length[i] % (int32_t)s.block_size && need[i] < have)
             atomicMax(&served, need[i] + 1);
     for (uint32_t i = warp0; i < n; i += warps) {
@@ -352,13 +484,22 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
         if (fits) {
             const int32_t *tp = s.table + (int64_t)from[i] * s.table_stride;
             int32_t *tc = s.table + (int64_t)c * s.table_stride;
-            for (int32_t k = lane; k < full; k += 32) {
-                const int32_t p = tp[k];
-                tc[k] = p;
-                if (p >= 0 && (uint32_t)p < s.num_pages)
-                    atomicAdd(&s.refs[p], 1);
-                else
-                    atomicOr(s.error, KVPAGE_ERR_PAGE);
+#pragma unroll 1
+            for (int32_t k = lane; k < full; k += kUnit) {
+                int32_t page[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    page[j] = k + 32 * j < full ? tp[k + 32 * j] : 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (k + 32 * j >= full)
+                        break;
+                    tc[k + 32 * j] = page[j];
+                    if (page[j] >= 0 && (uint32_t)page[j] < s.num_pages)
+                        atomicAdd(&s.refs[page[j]], 1);
+                    else
+                        atomicOr(s.error, KVPAGE_ERR_PAGE);
+                }
             }
             if (tail && lane == 0) {
                 src = tp[full];
@@ -451,28 +592,35 @@ __device__ __forceinline__ uint8_t *plane(const Planes &p, uint32_t lk)
 }
 
 /* ------------------------------------------------------------------------
- * copy.  A CTA moves up to kCopyVectors vectors of one page in one plane: a
- * page is one run of bytes in every geometry, so consecutive threads move
- * consecutive vectors.  With a token count, token-major pages stop early and
- * head-major ones skip the tokens behind it.  `pack` is the
- * distance between the entries of the lists: 1, or 3 for fork's pairs.
+ * copy.  A page in a plane is one run of vectors in every geometry.  Where a run
+ * fills CTAs of 2048 vectors, a CTA moves that much of one run.  Shorter runs
+ * (4 KiB: one head, 16 tokens) of all planes and pages lie on one line, of which
+ * a CTA takes 2048 vectors, so that a thread still has eight loads in flight:
+ * 256 half pages of 160 such planes took 95 us with a CTA per run, 40 like this;
+ * four pages of 64 planes of 32 KiB 3.6 us with CTAs per run, 5.0 on the line.
+ * With a token count, a token-major page stops early and a head-major one skips
+ * the tokens behind it.  `pack` is the distance between the entries of the
+ * lists: 1, or 3 for fork's pairs.
  * ---------------------------------------------------------------------- */
 constexpr int kMoveThreads = 256;
 constexpr int kMoveUnroll = 8;
 constexpr uint32_t kMoveVectors = kMoveThreads * kMoveUnroll;
 
+struct Copy {
+    const int32_t *src, *dst, *tokens;
+    uint32_t pack, n, planes_per_grid;  /* planes of one grid row */
+    FastDiv run, per_head, per_token;   /* vectors of a page, of a head, of a token of one */
+    FastDiv pairs;          /* pages; for long runs, CTAs of one */
+};
+
+/* grid: (pages x CTAs of a run, planes) */
 template <int VEC>
-__global__ void __launch_bounds__(kMoveThreads)
-kv_page_copy_kernel(const Planes p, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
-                    const int32_t *__restrict__ tokens, uint32_t pack, uint32_t n, uint32_t chunks)
+__global__ void __launch_bounds__(kMoveThreads) kv_page_copy_run_kernel(const Planes p, const __grid_constant__ Copy c)
 {
     using T = typename VecOf<VEC>::T;
-    const uint32_t lk = blockIdx.y;
-    const uint32_t i = blockIdx.x / chunks, chunk = blockIdx.x - i * chunks;
-    const int32_t a = src[(uint64_t)i * pack], b = dst[(uint64_t)i * pack];
-    int32_t keep = (int32_t)p.bs;
-    if (tokens)
-        keep = min(max(tokens[(uint64_t)i * pack], 0), keep);
+    const uint32_t i = fdiv(blockIdx.x, c.pairs), x0 = (blockIdx.x - i * c.pairs.d) * kMoveVectors + threadIdx.x;
+    const int32_t a = c.src[(uint64_t)i * c.pack], b = c.dst[(uint64_t)i * c.pack];
+    const int32_t keep = c.tokens ? min(max(c.tokens[(uint64_t)i * c.pack], 0), (int32_t)p.bs) : (int32_t)p.bs;
     if (!keep || a == b)
         return;
     if (a < 0 || (uint32_t)a >= p.pages || b < 0 || (uint32_t)b >= p.pages) {
@@ -480,27 +628,63 @@ kv_page_copy_kernel(const Planes p, const int32_t *__restrict__ src, const int32
             atomicOr(p.error, KVPAGE_ERR_PAGE);
         return;
     }
-    uint8_t *base = plane<VEC>(p, lk);
+    uint8_t *base = plane<VEC>(p, blockIdx.y);
     if (!base)
         return;
     const T *from = reinterpret_cast<const T *>(base + (uint64_t)a * p.stride);
     T *to = reinterpret_cast<T *>(base + (uint64_t)b * p.stride);
     const bool part = p.head_bytes && keep < (int32_t)p.bs;
-    const uint32_t all = (p.head_bytes ? p.bs : (uint32_t)keep) * (p.unit / VEC);
-    const uint32_t per_token = p.head_bytes / VEC, per_head = per_token * p.bs, used = per_token * keep;
+    const uint32_t all = p.head_bytes ? c.run.d : (uint32_t)keep * c.per_token.d, used = (uint32_t)keep * c.per_token.d;
     T v[kMoveUnroll];
     bool on[kMoveUnroll];
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; u++) {
-        const uint32_t x = chunk * kMoveVectors + u * kMoveThreads + threadIdx.x;
-        on[u] = x < all && !(part && x % per_head >= used);
+        const uint32_t x = x0 + u * kMoveThreads;
+        on[u] = x < all && !(part && x - fdiv(x, c.per_head) * c.per_head.d >= used);
         if (on[u])
             v[u] = from[x];
     }
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; u++)
         if (on[u])
-            to[chunk * kMoveVectors + u * kMoveThreads + threadIdx.x] = v[u];
+            to[x0 + u * kMoveThreads] = v[u];
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(kMoveThreads) kv_page_copy_kernel(const Planes p, const __grid_constant__ Copy c)
+{
+    using T = typename VecOf<VEC>::T;
+    const uint32_t lk0 = blockIdx.y * c.planes_per_grid;
+    const uint32_t items = min(c.planes_per_grid, p.layers * p.kvs - lk0) * c.n;
+    T v[kMoveUnroll];
+    T *to[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; u++) {
+        const uint32_t y = blockIdx.x * kMoveVectors + u * kMoveThreads + threadIdx.x;
+        const uint32_t item = fdiv(y, c.run), x = y - item * c.run.d;
+        to[u] = nullptr;
+        if (item >= items)
+            continue;
+        const uint32_t plane_in = fdiv(item, c.pairs), i = item - plane_in * c.n;
+        const int32_t a = c.src[(uint64_t)i * c.pack], b = c.dst[(uint64_t)i * c.pack];
+        const int32_t keep = c.tokens ? min(max(c.tokens[(uint64_t)i * c.pack], 0), (int32_t)p.bs) : (int32_t)p.bs;
+        const uint32_t head = fdiv(x, c.per_head), token = fdiv(x - head * c.per_head.d, c.per_token);
+        if ((int32_t)token >= keep || a == b)
+            continue;
+        if (a < 0 || (uint32_t)a >= p.pages || b < 0 || (uint32_t)b >= p.pages) {
+            atomicOr(p.error, KVPAGE_ERR_PAGE);
+            continue;
+        }
+        uint8_t *base = plane<VEC>(p, lk0 + plane_in);
+        if (base) {
+            v[u] = reinterpret_cast<const T *>(base + (uint64_t)a * p.stride)[x];
+            to[u] = reinterpret_cast<T *>(base + (uint64_t)b * p.stride) + x;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; u++)
+        if (to[u])
+            *to[u] = v[u];
 }
 
 /* ------------------------------------------------------------------------
@@ -650,13 +834,14 @@ int launched()
     return cudaPeekAtLastError() == cudaSuccess ? 0 : -EIO;
 }
 
-constexpr size_t kPlanSmem = (5 * KVPAGE_MAX_CALL + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
+constexpr size_t kPlanSmem = (6 * KVPAGE_MAX_CALL + kMaxUnits + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
 
-/* one cluster of `ctas` CTAs; the kernels' shared memory limit is raised once per device */
+/* one cluster; the kernels' shared memory limit is raised once per device */
 template <typename... P, typename... A>
-int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, int device, uint32_t ctas, size_t smem,
+int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, int device, uint32_t threads, size_t smem,
                 cudaStream_t stream, A... args)
 {
+    constexpr uint32_t ctas = kPlanCluster;
     std::call_once(once[device], [&] {
         err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
     });
@@ -665,7 +850,7 @@ int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, in
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kPlanThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -681,11 +866,12 @@ int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, in
     return launched();
 }
 
-/* a warp per row: one CTA has enough of them for a small call, whose time is
- * the barriers' and the loads'; larger calls use the cluster */
-uint32_t plan_ctas(uint32_t n)
+/* Threads of the cluster's CTAs: barriers of 8 warps are cheap, and a small
+ * call's units do not need more. */
+uint32_t plan_threads(const kv_page_state *s, uint32_t n)
 {
-    return n <= kPlanWarps ? 1 : kPlanCluster;
+    const uint64_t units = (uint64_t)n * ((s->width + kUnit - 1) / kUnit);
+    return units <= kPlanCluster * 8 ? 256 : kPlanThreads;
 }
 
 int resize_launch(const kv_page_state *s, const int32_t *rows, const int32_t *lens, uint32_t n, int32_t *status,
@@ -693,8 +879,9 @@ int resize_launch(const kv_page_state *s, const int32_t *rows, const int32_t *le
 {
     static std::once_flag once[64];
     static cudaError_t err[64];
-    const size_t smem = (5 * (size_t)n + 2 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
-    return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_ctas(n), smem, stream, *s, rows, lens, n, status);
+    const uint64_t units = n + (uint64_t)n * s->width / kUnit;
+    const size_t smem = (6 * (size_t)n + (units < kMaxUnits ? units : kMaxUnits) + 2 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
+    return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_threads(s, n), smem, stream, *s, rows, lens, n, status);
 }
 
 int call_ok(const kv_page_state *s, uint32_t n)
@@ -710,11 +897,36 @@ template <int VEC>
 int copy_vec(const Planes &p, const int32_t *src, const int32_t *dst, const int32_t *tokens, uint32_t pack, uint32_t n,
              cudaStream_t stream)
 {
-    const uint32_t all = p.bs * (p.unit / VEC), chunks = (all + kMoveVectors - 1) / kMoveVectors;
-    if ((uint64_t)n * chunks > INT32_MAX || p.layers * p.kvs > 65535)
+    Copy c{};
+    c.src = src;
+    c.dst = dst;
+    c.tokens = tokens;
+    c.pack = pack;
+    c.n = n;
+    const uint32_t run = p.bs * (p.unit / VEC), planes = p.layers * p.kvs;
+    c.run = make_fastdiv(run);
+    c.per_token = make_fastdiv((p.head_bytes ? p.head_bytes : p.unit) / VEC);
+    c.per_head = make_fastdiv(p.bs * c.per_token.d);
+    if (run >= kMoveVectors) {
+        c.pairs = make_fastdiv((run + kMoveVectors - 1) / kMoveVectors);
+        if ((uint64_t)n * c.pairs.d > INT32_MAX || planes > 65535)
+            return -E2BIG;
+        kv_page_copy_run_kernel<VEC><<<dim3(n * c.pairs.d, planes), kMoveThreads, 0, stream>>>(p, c);
+        return launched();
+    }
+    c.pairs = make_fastdiv(n);
+    /* 31-bit indexes: planes of all pages that fit one row of the grid */
+    const uint64_t one = (uint64_t)n * run;
+    if (one >= (1ull << 31))
         return -E2BIG;
-    kv_page_copy_kernel<VEC><<<dim3(n * chunks, p.layers * p.kvs), kMoveThreads, 0, stream>>>(p, src, dst, tokens, pack,
-                                                                                          n, chunks);
+    c.planes_per_grid = (uint32_t)(((1ull << 31) - 1) / one);
+    if (c.planes_per_grid > planes)
+        c.planes_per_grid = planes;
+    const uint32_t grid_y = (planes + c.planes_per_grid - 1) / c.planes_per_grid;
+    if (grid_y > 65535)
+        return -E2BIG;
+    const uint32_t grid_x = (uint32_t)((one * c.planes_per_grid + kMoveVectors - 1) / kMoveVectors);
+    kv_page_copy_kernel<VEC><<<dim3(grid_x, grid_y), kMoveThreads, 0, stream>>>(p, c);
     return launched();
 }
 
@@ -735,17 +947,22 @@ template <int VEC>
 int compact_vec(const Planes &p, const kv_page_state *s, const int32_t *rows, const int32_t *start, const int32_t *keep,
                 const int32_t *offsets, uint32_t num_keep, uint32_t n, int32_t *scratch, cudaStream_t stream)
 {
-    /* a slice: the most vectors that divide a token's piece, at most 32 (512
-     * bytes of a 16-byte vector), so that a pass of the CTA covers whole tokens */
+    /* a slice: the most vectors that divide a token's piece, at most 16 (256
+     * bytes of a 16-byte vector), so that a pass of the CTA covers whole tokens
+     * and long rows are cut finely */
     const uint32_t piece = (p.head_bytes ? p.head_bytes : p.unit) / VEC;
-    uint32_t vecs = piece < 32 ? piece : 32;
+    uint32_t vecs = piece < 16 ? piece : 16;
     while (piece % vecs)
         vecs--;
     const uint64_t slices = (uint64_t)(p.unit / VEC / vecs) * p.layers * p.kvs;
     if (slices > INT32_MAX)
         return -E2BIG;
-    /* enough CTAs to fill the GPU a few times over, no more: each reads its row's list */
-    uint32_t per = (uint32_t)((slices * n + 4095) / 4096);
+    /* A CTA reads and checks its row's list before it moves anything.  Where the
+     * lists are short that is most of its time, and CTAs that fill the GPU once
+     * (six to an SM) take many slices each, side by side; long lists want many
+     * CTAs, since rows differ in length. */
+    const uint64_t want = num_keep / n < kMoveVectors / 16 ? 888 : 8192;
+    uint32_t per = (uint32_t)((slices * n + want - 1) / want);
     if (per > slices)
         per = (uint32_t)slices;
     const uint32_t ctas = (uint32_t)((slices + per - 1) / per);
@@ -806,7 +1023,7 @@ extern "C" int kv_page_fork_launch(const struct kv_page_cache *c, const struct k
     static cudaError_t err[64];
     const size_t smem = (4 * (size_t)n + 3 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int ret = launch_plan(kv_page_fork_kernel, once, err, s->device, plan_ctas(n), smem, st, *s, parents, children, n,
+    const int ret = launch_plan(kv_page_fork_kernel, once, err, s->device, plan_threads(s, n), smem, st, *s, parents, children, n,
                                 pairs, status);
     if (ret)
         return ret;
