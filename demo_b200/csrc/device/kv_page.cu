@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_page_copy_kernel(const Planes
  * The first CTA of a row leaves the new length for resize, or kRefused.
  * ---------------------------------------------------------------------- */
 template <int VEC>
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kMoveThreads, 4)
 kv_page_compact_kernel(const Planes p, const kv_page_state s, const int32_t *__restrict__ rows,
                        const int32_t *__restrict__ start, const int32_t *__restrict__ keep,
                        const int32_t *__restrict__ offsets, uint32_t num_keep, uint32_t n,
