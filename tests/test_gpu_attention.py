@@ -196,6 +196,20 @@ def test_a_value_of_the_context_that_is_not_finite_reaches_every_row(kvt, block)
         close(out, lse, clean)
 
 
+@pytest.mark.parametrize("qt", [BF16, FP16], ids=["bf16", "fp16"])
+def test_every_8bit_value(qt):
+    """one visible position: the output is its value, widened exactly"""
+    b = Batch([1] * 2, [1] * 2, heads=2, kv_heads=1, dim=128, qt=qt, kvt=E4M3, order="hnd")
+    codes = torch.arange(256, dtype=torch.int32, device="cuda").to(torch.uint8).view(E4M3)
+    for r in range(2):
+        b.view[0, 1].view(torch.uint8)[int(b.table[r, 0]), 0, 0] = codes[128 * r:128 * r + 128].view(torch.uint8)
+    b.scales = (1.0, 1.0)
+    args, parents = b.args()
+    out = b.attention()(*args).double()
+    want = codes.double().view(2, 1, 128).expand(2, 2, 128)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(), want.nan_to_num())
+
+
 def test_large_scores():
     """rows whose maximum climbs through the whole context, and scores that
     only a running maximum survives"""
