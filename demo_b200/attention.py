@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import KvAttnDesc, lib
 from .cache import CacheError, KVLayout
-from .pages import _current_stream, _int32
+from .pages import _current_stream, _int32, _on_stream
 
 # struct kv_attn_desc in one go: 12 pointers, 8 64-bit numbers, 12 32-bit ones, three floats, the device
 _DESC = struct.Struct("@12PQQqqqqq10I2i3fi")
@@ -66,6 +66,8 @@ class TreeAttention:
         self._devices: dict[int, tuple[torch.Tensor, int, int]] = {}     # error bits, their address, workspace bytes
         self._shape = (layout.num_blocks, layout.block_size, num_heads, num_kv_heads, dim, 1 if layout.head_bytes else 0)
         self._scales = (scale, float(k_scale), float(v_scale))
+        if torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing():
+            self._device(torch.cuda.current_device())
 
     def _device(self, index: int) -> tuple[torch.Tensor, int, int]:
         d = KvAttnDesc(table_stride=1, width=1, num_rows=1, device=index, scale=self._scales[0], k_scale=self._scales[1])
@@ -73,7 +75,11 @@ class TreeAttention:
         need = lib.kv_attn_workspace_bytes(C.addressof(d))
         if need < 0:
             raise CacheError("kv_attn_workspace_bytes", need)
-        error = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        with torch.cuda.device(index):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError(f"the first call on cuda:{index} cannot be captured")
+            error = torch.zeros(1, dtype=torch.int32, device="cuda")
+            torch.cuda.current_stream().synchronize()   # the call may be on another stream
         self._devices[index] = found = error, error.data_ptr(), need
         return found
 
@@ -90,12 +96,17 @@ class TreeAttention:
                      ones, -2: padding); None: a chain
         rows         int32 [sequences]: their rows; None: row b
 
-        Runs on `stream`, by default the current stream of q's device.
+        Runs on `stream`, by default the current stream of q's device, to which
+        the results then belong.  May be captured, except for the first call on
+        a device that was not the current one when the object was made.
         """
         index, kind = q.get_device(), _TYPES.get(q.dtype)
         if index < 0 or kind is None or q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or \
                 q.stride(2) != 1:
             raise ValueError(f"q: expected a bfloat16 or float16 CUDA tensor [total, {self.num_heads}, {self.head_dim}]")
+        if stream is not None:
+            with _on_stream(stream, index):
+                return self(layer, q, block_table, seq_lens, q_offsets, parents, rows, out, return_lse)
         total = q.shape[0]
         q_strides = q.stride()
         if 0 in q_strides:                              # an expanded tensor
@@ -116,13 +127,6 @@ class TreeAttention:
         lse = torch.empty((total, self.num_heads), dtype=torch.float32, device=q.device) if return_lse else None
         _, error, need = self._devices.get(index) or self._device(index)
         work = torch.empty(need, dtype=torch.uint8, device=q.device)    # of this call alone, also where graphs are captured
-        if stream is None:
-            st = _current_stream(index)
-        else:
-            st = stream.cuda_stream
-            for t in (out, lse, work):      # the allocator frees them for the current stream otherwise
-                if t is not None:
-                    t.record_stream(stream)
         row = self.num_heads * self.head_dim            # a stride of one row or one head means nothing
         pages, block, heads, kv_heads, dim, head_major = self._shape
         desc = _DESC.pack(
@@ -135,7 +139,7 @@ class TreeAttention:
             out_strides[0] if total > 1 else row, out_strides[1] if heads > 1 else row,
             width, n_rows, seqs, total, pages, block, heads, kv_heads, dim, head_major, kind,
             _lib.KVATTN_E4M3 if self.layout.element_size == 1 else kind, *self._scales, index)
-        ret = lib.kv_attn_launch(desc, st)
+        ret = lib.kv_attn_launch(desc, _current_stream(index))
         if ret:
             raise CacheError("kv_attn_launch", ret)
         return (out, lse) if return_lse else out

@@ -34,6 +34,15 @@ OK, NO_PAGES, INVALID = _lib.KVPAGE_OK, _lib.KVPAGE_NO_PAGES, _lib.KVPAGE_INVALI
 _current_stream = torch._C._cuda_getCurrentRawStream
 
 
+def _on_stream(stream: torch.cuda.Stream, index: int):
+    """Context in which `stream` is the current one: what a call on it allocates
+    is then ordered with it, where memory of another stream might still be in
+    use there."""
+    if stream.device_index != index:
+        raise ValueError(f"stream: expected a stream of cuda:{index}")
+    return torch.cuda.stream(stream)
+
+
 def _int32(name: str, t: torch.Tensor, index: int, numel: int | None = None) -> int:
     """data pointer of a contiguous int32 tensor on CUDA device `index` (-1:
     the CPU); ValueError otherwise"""
@@ -76,7 +85,8 @@ class PagePool:
     The tensors are updated in place and stay readable by the engine's own
     kernels.  Calls run on `stream`, by default the current stream of the
     cache's device, in the order they are made; calls for one pool on several
-    streams have to be ordered by the caller.  The int32 results of resize,
+    streams have to be ordered by the caller, and results belong to the stream
+    of their call.  The int32 results of resize,
     fork and compact say per row pages.OK, NO_PAGES or INVALID, on the device.
     """
 
@@ -117,14 +127,17 @@ class PagePool:
             head_bytes=layout.head_bytes, block_size=layout.block_size, num_layers=layout.num_layers, num_pages=n,
             base_align=align, device=self._index)
         self._state_p, self._cache_p = C.addressof(self._state), C.addressof(self._cache)
+        torch.cuda.current_stream(dev).synchronize()    # the first call may be on any stream
 
     def _results(self, n: int, scratch: int, stream) -> tuple[torch.Tensor, int]:
         """n results and `scratch` values behind them, and the stream's handle"""
-        out = torch.empty(n + scratch, dtype=torch.int32, device=self.device)
-        if stream is None:
-            return out, _current_stream(self._index)
-        out.record_stream(stream)           # the allocator frees it for the current stream otherwise
-        return out, stream.cuda_stream
+        if stream is not None:
+            caller = torch.cuda.current_stream(self.device)
+            with _on_stream(stream, self._index):
+                out, st = self._results(n, scratch, None)
+            out.record_stream(caller)       # which may be where it is used and dropped
+            return out, st
+        return torch.empty(n + scratch, dtype=torch.int32, device=self.device), _current_stream(self._index)
 
     def resize(self, rows: torch.Tensor, lens: torch.Tensor, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """Give row rows[i] the pages of lens[i] tokens (0 frees it): rows that
@@ -144,7 +157,7 @@ class PagePool:
         tokens[i] tokens, with tokens).  Destinations are distinct and not
         among the sources."""
         n = src.numel()
-        st = _current_stream(self._index) if stream is None else stream.cuda_stream
+        st = self._results(0, 0, stream)[1] if stream is not None else _current_stream(self._index)
         ret = lib.kv_page_copy_launch(self._cache_p, _int32("src", src, self._index), _int32("dst", dst, self._index, n),
                                       _int32("tokens", tokens, self._index, n) if tokens is not None else None, n, st)
         if ret:

@@ -332,3 +332,21 @@ def test_misaligned_planes():
     pool.copy(ints([2]), ints([5]))
     pool.check()
     assert torch.equal(t, want)
+
+
+def test_results_on_a_side_stream():
+    """are not in memory that the current stream has freed but still has to
+    write"""
+    c = Case(GEOMETRIES["hnd"], 60, 4, 8)
+    rows, lens = ints([0, 1]), ints([100, 37])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    held = torch.empty(2, dtype=torch.int32, device="cuda")
+    torch.cuda._sleep(200_000_000)
+    held.fill_(7)
+    del held
+    got = c.pool.resize(rows, lens, stream=side)
+    torch.cuda.synchronize()
+    assert got.tolist() == [pg.OK, pg.OK]
+    c.model.resize([0, 1], [100, 37])
+    c.same()
