@@ -121,6 +121,8 @@ __device__ bool sequence(const kv_attn_desc &d, uint32_t b, Seq &s)
     s = {o0, 0, 0, 0};
     if (o0 < 0 || o1 < o0 || (uint32_t)o1 > d.total_q)
         return false;
+    if (o1 == o0)
+        return true;                /* nothing to do, whatever its row */
     s.nodes = o1 - o0;
     if (r < 0 || (uint32_t)r >= d.num_rows)
         return false;
@@ -484,7 +486,7 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c)
 }
 
 /* ------------------------------------------------------------------------
- * loaders: a ring of tiles of K, one of tiles of V.
+ * loaders: a ring of tiles of K, one of tiles of V; a piece's last tile first.
  * ---------------------------------------------------------------------- */
 /* a place in a ring, and how often the ring has been gone around */
 template <int N> struct Turn {
@@ -548,18 +550,18 @@ template <typename T, Load L, int DP> struct Loader {
         Piece e;
         for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
             const int32_t *tab = p.d.table + (int64_t)e.row * p.d.table_stride;
-            const int32_t t1 = uniform(e.t1), end = uniform(e.end), h = uniform(e.h);
-            int32_t pos = e.t0 * kTile + (int32_t)(lane * p.box);
+            const int32_t t0 = uniform(e.t0), end = uniform(e.end), h = uniform(e.h);
+            int32_t pos = (e.t1 - 1) * kTile + (int32_t)(lane * p.box);
             int32_t next = lane < boxes && pos < end ? tab[fdiv(pos, p.block)] : 0;
-            for (int32_t t = uniform(e.t0); t < t1; t++) {
+            for (int32_t t = uniform(e.t1) - 1; t >= t0; t--) {
                 const int32_t page = next;
                 /* a page of more than 64 rows holds several tiles */
                 const int32_t first = uniform(boxes == 1 ? pos - (int32_t)(fdiv(pos, p.block) * p.block.d) : 0);
                 const uint32_t n = min(boxes, (end - t * kTile + p.box - 1) / p.box);
                 if (lane < n && (uint32_t)page >= p.d.num_pages)
                     atomicOr(p.d.error, KVATTN_ERR_PAGE);
-                pos += kTile;
-                if (t + 1 < t1)
+                pos -= kTile;
+                if (t > t0)
                     next = lane < boxes && pos < end ? tab[fdiv(pos, p.block)] : 0;     /* in flight while the tile is loaded */
                 if (!wait_warp(sh, p.d.error, frees + at * 8, parity))
                     return;
@@ -646,12 +648,12 @@ template <typename T, Load L, int DP> struct Loader {
         take_rows();
         Piece e;
         for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
-            const int32_t t1 = e.t1;
-            int32_t page = look_up(e, e.t0);
-            for (int32_t t = e.t0; t < t1; t++) {
+            const int32_t t0 = e.t0;
+            int32_t page = look_up(e, e.t1 - 1);
+            for (int32_t t = e.t1 - 1; t >= t0; t--) {
                 places(e, t, page);
-                if (t + 1 < t1)
-                    page = look_up(e, t + 1);       /* in flight while the tile is copied */
+                if (t > t0)
+                    page = look_up(e, t - 1);       /* in flight while the tile is copied */
                 for (int v = 0; v < 2; v++) {
                     if (!acquire(v))
                         return;
@@ -724,12 +726,12 @@ template <typename T, Load L, int DP> struct Loader {
             }
         };
         for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
-            const int32_t t1 = e.t1;
-            int32_t page = look_up(e, e.t0);
-            for (int32_t t = e.t0; t < t1; t++) {
+            const int32_t t0 = e.t0;
+            int32_t page = look_up(e, e.t1 - 1);
+            for (int32_t t = e.t1 - 1; t >= t0; t--) {
                 places(e, t, page);
-                if (t + 1 < t1)
-                    page = look_up(e, t + 1);
+                if (t > t0)
+                    page = look_up(e, t - 1);
                 if (!fetch(false))
                     return;
                 swap();
@@ -845,8 +847,11 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
  * powers of two), so that O, which lives in TMEM, is rescaled rarely; the
  * result is the same quotient.
  * ---------------------------------------------------------------------- */
-/* the positions p0 .. p0 + 64 that node j sees, a bit each */
-__device__ uint64_t seen(const Params &p, const Piece &e, int32_t j, int32_t p0)
+/* The positions p0 .. p0 + 64 that a node sees, a bit each.  j is the node, or
+ * in a tree the nearest of its line (the node itself, its ancestors) that stands
+ * before p0 + 64 or not much behind it, and on return the one before p0: tiles
+ * come from the last to the first, and a piece walks a line once. */
+__device__ uint64_t seen(const Params &p, const Piece &e, int32_t &j, int32_t p0)
 {
     const int32_t before = e.ctx - p0;
     uint64_t bits = before >= 64 ? ~0ull : before > 0 ? (1ull << before) - 1 : 0;
@@ -855,13 +860,11 @@ __device__ uint64_t seen(const Params &p, const Piece &e, int32_t j, int32_t p0)
         return upto >= 64 ? ~0ull : upto > 0 ? (1ull << upto) - 1 : 0;
     }
     const int32_t *par = p.d.parents + e.q0;
-    for (int32_t a = j; before + a >= 0;) {
-        if (before + a < 64)
-            bits |= 1ull << (before + a);
-        const int32_t u = par[a];
-        if (u < 0 || !node_ok(par, u))
-            break;
-        a = u;
+    while (j >= 0 && before + j >= 0) {
+        if (before + j < 64)
+            bits |= 1ull << (before + j);
+        const int32_t u = par[j];
+        j = u >= 0 && node_ok(par, u) ? u : -1;
     }
     return bits;
 }
@@ -883,7 +886,7 @@ __device__ __noinline__ void add_spoilt(const Params &p, const Piece &e, int32_t
         for (int32_t a = active ? j : -1; a >= 0 && e.ctx + a >= e.t0 * kTile;) {
             const uint32_t pos = e.ctx + a, b = fdiv(pos, p.block);
             const int32_t page = tab[b];
-            if ((int32_t)pos < e.t1 * kTile && page >= 0 && (uint32_t)page < d.num_pages) {
+            if (pos < (uint32_t)e.t1 * kTile && page >= 0 && (uint32_t)page < d.num_pages) {
                 const uint64_t at = ((uint64_t)(pos - b * p.block.d) * (d.head_major ? 1 : d.num_kv_heads) +
                                      (uint64_t)(d.head_major ? d.block_size : 1) * e.h) * d.head_dim + c;
                 const char *base = static_cast<const char *>(d.v) + (uint64_t)page * p.stride;
@@ -973,12 +976,13 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
         const bool work = __any_sync(~0u, active);
         const int32_t t0 = e.t0, t1 = e.t1, ctx = e.ctx;
         float m = -INFINITY, l = 0;
-        for (int32_t t = t0; t < t1; t++, g++, at_v.next()) {
+        int32_t line = node;
+        for (int32_t t = t1 - 1; t >= t0; t--, g++, at_v.next()) {
             const uint32_t s_at = tmem + (g & 1) * kTile;
-            const bool mask = (t + 1) * kTile > ctx;
+            const bool mask = (uint32_t)(t + 1) * kTile > (uint32_t)ctx;
             uint64_t bits = 0;
             if (mask && active)
-                bits = seen(p, e, node, t * kTile);
+                bits = seen(p, e, line, t * kTile);
             if (!wait_warp(sh, d.error, &sh.s_full[g & 1], (g >> 1) & 1))
                 return;
             if (work) {
@@ -1002,7 +1006,7 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
                 }
                 now *= s2;
                 const bool raise = active && now > m + Type<T>::kLazy;
-                if (t == t0) {
+                if (t == t1 - 1) {
                     m = now;
                 } else if (__any_sync(~0u, raise)) {
                     const float f = raise ? exp2_approx(m - now) : 1.f;
@@ -1064,7 +1068,7 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
         const bool whole = e.whole();
         const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
         const uint32_t slot = 2 * blockIdx.x + (piece ? 1 : 0);
-        const float inv = !active ? 0.f : whole ? d.v_scale / l : 1.f;
+        const float inv = !active || l == 0 ? 0.f : whole ? d.v_scale / l : 1.f;
         const bool spoilt = __any_sync(~0u, sh.spoilt[piece % 4] == piece + 1);
         if (__any_sync(~0u, valid)) {
             if (spoilt)
@@ -1137,17 +1141,25 @@ __device__ int64_t block_scan(Shared &sh, int64_t v, int64_t &total)
     return inc;
 }
 
-template <typename T>
-__device__ __noinline__ void void_rows(const Params &p, const Seq &s)
+/* voids the rows of those of sequences b0 .. b1 that do not fit, with all threads of the grid */
+template <typename T, int kThreads>
+__device__ __noinline__ void void_rows(const Params &p, uint32_t b0, uint32_t b1)
 {
     const kv_attn_desc &d = p.d;
-    for (int64_t x = 0; x < (int64_t)s.nodes * d.num_heads; x++) {
-        const int64_t i = s.q0 + x / d.num_heads, h = x % d.num_heads;
-        T *out = static_cast<T *>(d.out) + i * d.out_stride + h * d.out_head_stride;
-        for (uint32_t c = 0; c < d.head_dim; c += 8)
-            *reinterpret_cast<uint4 *>(out + c) = make_uint4(0, 0, 0, 0);
-        if (d.lse)
-            d.lse[i * d.num_heads + h] = -INFINITY;
+    for (uint32_t b = b0; b < b1; b++) {
+        Seq s;
+        if (sequence(d, b, s))
+            continue;
+        if (blockIdx.x == 0 && threadIdx.x == 0)
+            atomicOr(d.error, KVATTN_ERR_SEQ);
+        for (int64_t x = blockIdx.x * kThreads + threadIdx.x; x < (int64_t)s.nodes * d.num_heads; x += (int64_t)gridDim.x * kThreads) {
+            const int64_t i = s.q0 + x / d.num_heads, h = x % d.num_heads;
+            T *out = static_cast<T *>(d.out) + i * d.out_stride + h * d.out_head_stride;
+            for (uint32_t c = 0; c < d.head_dim; c += 8)
+                *reinterpret_cast<uint4 *>(out + c) = make_uint4(0, 0, 0, 0);
+            if (d.lse)
+                d.lse[i * d.num_heads + h] = -INFINITY;
+        }
     }
 }
 
@@ -1166,14 +1178,11 @@ __device__ void find_line(const Params &p, Shared &sh)
             uint64_t n = 0;
             int64_t sum;
             Seq s;
-            if (b < d.num_seqs) {
-                if (sequence(d, b, s)) {
-                    n = head_tiles(p, s);
-                } else if (walk == 0 && blockIdx.x == b % gridDim.x) {
-                    atomicOr(d.error, KVATTN_ERR_SEQ);
-                    void_rows<T>(p, s);
-                }
-            }
+            const bool ok = b >= d.num_seqs || sequence(d, b, s);
+            if (ok && b < d.num_seqs)
+                n = head_tiles(p, s);
+            if (walk == 0 && __syncthreads_or(!ok))
+                void_rows<T, kThreads>(p, b0, min(b0 + kThreads, d.num_seqs));
             const int64_t all = (int64_t)(n * d.num_kv_heads), upto = before + block_scan<kThreads>(sh, all, sum);
             before += sum;
             if (once || (walk == 0 && b0 + kThreads >= d.num_seqs)) {
@@ -1592,7 +1601,8 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
         return 0;
     if (!d->q || !d->out || !d->k || !d->v || !d->table || !d->lens || !d->q_offsets || !d->error || !d->workspace ||
         ((uintptr_t)d->q | (uintptr_t)d->out | (uintptr_t)d->k | (uintptr_t)d->v) % 16 || (uintptr_t)d->workspace % 256 ||
-        (d->q_stride | d->q_head_stride | d->out_stride | d->out_head_stride) % 8 || d->q_stride <= 0 || d->q_head_stride <= 0)
+        (d->q_stride | d->q_head_stride | d->out_stride | d->out_head_stride) % 8 || d->q_stride <= 0 || d->q_head_stride <= 0 ||
+        d->out_stride <= 0 || d->out_head_stride <= 0)
         return -EINVAL;
     DeviceGuard on(d->device);
     if (!on.ok)

@@ -23,7 +23,9 @@
  * same sequence that node j follows: -1 .. j - 1, -1 for the last token before
  * the nodes.  -2 marks a padding node: it sees nothing (out 0, lse -inf), and
  * nothing sees it; its K and V may be anything.  NULL is a chain, parent j - 1.
- * Rows of out and lse that no sequence covers are left as they were.
+ * A sequence without nodes is skipped, whatever its row.  Rows of out and lse
+ * that no sequence covers are left as they were.  A row that sees nothing, or
+ * only scores of -inf, is 0 with lse -inf.
  */
 #ifndef __KVATTN_H__
 #define __KVATTN_H__
@@ -34,10 +36,10 @@
 extern "C" {
 #endif
 
-/* bits the kernels OR into *error; the rows concerned are 0 / -inf unless
- * said otherwise, all others are right */
+/* bits the kernels OR into *error; all rows that are not named are right */
 #define KVATTN_ERR_PAGE    0x1   /* a page id outside [0, num_pages); it counts as zeros */
-#define KVATTN_ERR_SEQ     0x2   /* offsets out of order, or a row or length that fits neither table nor nodes */
+#define KVATTN_ERR_SEQ     0x2   /* a row or length that fits neither table nor nodes: the sequence's rows are
+                                  * 0 / -inf; or offsets out of order or past total_q: the sequence is skipped */
 #define KVATTN_ERR_PARENT  0x4   /* a parent outside [-2, j - 1]: the node is taken for a padding node */
 #define KVATTN_ERR_TIMEOUT 0x8   /* a wait inside the kernel ran out: the results are void */
 

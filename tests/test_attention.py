@@ -137,3 +137,23 @@ def test_the_oracle_on_a_case_worked_by_hand():
     assert lse[:, 1].tolist() == pytest.approx([math.log(2), -math.inf, math.log(3)])
     assert oa.visible(None, 3) == [{0}, {0, 1}, {0, 1, 2}]
     assert oa.visible([-1, -2, 1, 0, 7], 5) == [{0}, None, {2}, {0, 3}, None]
+
+
+@pytest.mark.parametrize("bad", [dict(out_stride=0), dict(out_stride=-1024), dict(out_head_stride=0), dict(out_head_stride=-128)], ids=str)
+def test_results_that_would_lie_over_each_other_are_refused(bad):
+    d = desc(**bad)
+    assert lib.kv_attn_launch(C.addressof(d), None) == -errno.EINVAL
+
+
+def test_too_many_queries_are_refused():
+    d = desc(total_q=(1 << 27) + 1)
+    assert lib.kv_attn_launch(C.addressof(d), None) == -errno.E2BIG
+
+
+def test_a_stream_of_another_device_is_refused():
+    from types import SimpleNamespace
+
+    from demo_b200.pages import _on_stream
+
+    with pytest.raises(ValueError, match="cuda:0"):
+        _on_stream(SimpleNamespace(device_index=1), 0)

@@ -392,3 +392,141 @@ def test_a_step_over_the_pool_and_the_store():
     pool.resize(i32([0, 1, 2]), i32([0, 0, 0]))
     pool.check()
     assert int(pool.free_count.item()) == nb
+
+
+def test_a_path_as_a_tree_is_a_chain():
+    """3000 nodes, each the parent of the next: the bits of a call without
+    parents, whose rows the oracle checks above"""
+    b = Batch([3050, 700], [3000, 650], heads=4, kv_heads=2, dim=64, seed=15)
+    args, _ = b.args()
+    att = b.attention()
+    chain = att(*args, return_lse=True)
+    path = torch.cat([torch.arange(-1, n - 1, dtype=torch.int32, device="cuda") for n in b.nodes])
+    for got, want in zip(att(*args, parents=path, return_lse=True), chain):
+        assert torch.equal(got, want)
+    att.check()
+
+
+def test_positions_up_to_31_bits():
+    """2^31 - 1 tokens on one page that the row names 2048 times: scores 0,
+    values 1; each is exp(0) = 1, and sums of ones are exact up to 2^24, so
+    that only the joined pieces' sums (at most 512 of them) round: 2^-15"""
+    bs, w = 1 << 20, 2048
+    k = torch.zeros(2, 1, bs, 1, 16, dtype=BF16, device="cuda")
+    k[1] = 1
+    layout, kp, vp = cc.layout_from_kv_tensors([k], kv_layout="flash_attn")
+    att = TreeAttention(layout, kp, vp, 1, 1)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    out, lse = att(0, torch.ones(2, 1, 16, dtype=BF16, device="cuda"), i32([[0] * w]), i32([2 ** 31 - 1]), i32([0, 2]), return_lse=True)
+    att.check()
+    assert ((out.double() - 1).abs() <= 2.0 ** -8 + 2.0 ** -14).all()
+    want = torch.tensor([math.log(2 ** 31 - 2), math.log(2 ** 31 - 1)], dtype=torch.float64, device="cuda")[:, None]
+    assert ((lse.double() - want).abs() <= 2.0 ** -15 + 2.0 ** -21 * want).all()
+
+
+@pytest.mark.parametrize("block, kvt", [(16, BF16), (24, BF16), (16, E4M3)], ids=["boxes", "copies", "8bit"])
+def test_pages_past_32_bits(block, kvt):
+    """pages more than 4 GiB into a plane"""
+    esz, kv_heads, dim = (1 if kvt == E4M3 else 2), 8, 128
+    pages = (1 << 32) // (block * kv_heads * dim * esz) + 9
+    store = torch.empty(2, pages, block, kv_heads, dim, dtype=kvt, device="cuda")
+    b = Batch([200, 61], [3, 61], heads=8, kv_heads=kv_heads, dim=dim, block=block, kvt=kvt, seed=16).tree(16)
+    used = b.view.shape[2]
+    for i in range(2):
+        store.view(torch.uint8 if kvt == E4M3 else torch.int16)[i, -used:] = b.view[0, i].view(torch.uint8 if kvt == E4M3 else torch.int16)
+    layout, k, v = cc.layout_from_kv_tensors([store], kv_layout="flash_attn")
+    att = TreeAttention(layout, k, v, 8, kv_heads, k_scale=b.scales[0], v_scale=b.scales[1])
+    args, parents = b.args()
+    table = torch.where(args[2] >= 0, args[2] + (pages - used), args[2])
+    out, lse = att(0, b.q, table, *args[3:], parents=parents, return_lse=True)
+    att.check()
+    close(out, lse, b.expected())
+
+
+def test_rows_of_a_padded_batch():
+    """sequences without nodes, whose rows are no rows: nothing of theirs is
+    looked at"""
+    b = Batch([100, 40], [3, 1], seed=17)
+    args, _ = b.args()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    att = b.attention()
+    out, lse = att(*args[:4], i32([0, 3, 3, 4, 4, 4]), rows=i32([0, -1, 1, 99, -5]), return_lse=True)
+    att.check()
+    close(out, lse, b.expected())
+
+
+def test_a_long_sequence_that_does_not_fit():
+    """its rows are voided by the whole grid, also where there are more
+    sequences than threads look at in one go"""
+    n, m = 20000, 400
+    b = Batch([5] * (m - 1) + [n], [1] * (m - 1) + [n], heads=2, kv_heads=1, dim=16, seed=18)
+    args, _ = b.args()
+    args[3][m - 1] = n - 1
+    att = b.attention()
+    out, lse = att(*args, return_lse=True)
+    with pytest.raises(ValueError, match="length"):
+        att.check()
+    assert not out[m - 1:].any() and torch.isinf(lse[m - 1:]).all()
+    want = oa.attention(b.q[:m - 1], *(b.view[0, i].double() for i in range(2)), b.table.tolist(), b.lens, b.off[:m])
+    close(out[:m - 1], lse[:m - 1], want)
+
+
+def test_offsets_out_of_order_are_skipped():
+    b = Batch([50, 60, 70], [2, 3, 4], seed=19)
+    args, _ = b.args()
+    att = b.attention()
+    for off in ([0, 2, 1, 9], [0, 2, 2, 99], [-4, -1, 5, 9]):
+        out = torch.full_like(b.q, 7.0)
+        a = (*args[:4], torch.tensor(off, dtype=torch.int32, device="cuda"))
+        att(*a, out=out)
+        with pytest.raises(ValueError, match="offsets"):
+            att.check()
+        covered = {i for x, y in zip(off, off[1:]) if 0 <= x <= y <= 9 for i in range(x, y)}
+        for i in range(9):
+            assert (out[i] == 7).all() == (i not in covered), (off, i)
+
+
+@pytest.mark.parametrize("n", [40, 6000])
+def test_scores_of_minus_infinity_alone(n):
+    """count as nothing seen, whether a row is joined from pieces or not"""
+    b = Batch([n, 30], [1, 1], heads=2, kv_heads=1, dim=64, seed=20)
+    b.q[0] = 1
+    b.view[0, 0, torch.tensor(b.table[0, :-(-n // 16)].astype(np.int64)).cuda()] = -math.inf
+    args, _ = b.args()
+    out, lse = b.attention()(*args, return_lse=True)
+    assert not out[0].any() and (lse[0] == -math.inf).all()
+    want = oa.attention(b.q[1:], *(b.view[0, i].double() for i in range(2)), b.table.tolist(), b.lens, [0, 1], rows=[1])
+    close(out[1:], lse[1:], want)
+
+
+def test_memory_in_use_on_another_stream_is_left_alone():
+    """what a call on a side stream allocates is not what the current stream has
+    freed but still has to write"""
+    b = Batch([300, 17], [2, 1], seed=21)
+    args, _ = b.args()
+    att = b.attention()
+    want = att(*args)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for shape, dt in ((want.shape, want.dtype), ((40 << 20,), torch.uint8)):
+        held = torch.empty(shape, dtype=dt, device="cuda")
+        torch.cuda._sleep(200_000_000)
+        held.fill_(7)
+        del held
+        got = att(*args, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_the_first_call_is_captured():
+    b = Batch([300, 17], [2, 1], seed=22)
+    args, _ = b.args()
+    b.attention()(*args)                # loads the kernels
+    att = b.attention()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = att(*args, return_lse=True)
+    att.check()
+    g.replay()
+    att.check()
+    close(out, lse, b.expected())
