@@ -66,9 +66,8 @@ def plane_bases(layout: KVLayout, k_ptrs: Sequence[int], v_ptrs: Sequence[int] |
         if not p:
             raise ValueError("a layer base is null")
         every |= int(p)
-    k = torch.tensor([int(p) for p in k_ptrs], dtype=torch.int64, device=device)
-    v = torch.tensor([int(p) for p in v_ptrs], dtype=torch.int64, device=device) if v_ptrs is not None else None
-    return k, v, every & -every
+    both = torch.tensor([int(p) for p in (*k_ptrs, *(v_ptrs or ()))], dtype=torch.int64, device=device)
+    return both[:layout.num_layers], both[layout.num_layers:] if v_ptrs is not None else None, every & -every
 
 
 class PagePool:
@@ -111,8 +110,8 @@ class PagePool:
         self.layout, self.device = layout, dev
         self.block_table, self.seq_lens = block_table, seq_lens
         self.refs, self.free_list, self.free_count = refs, free_list, free_count
-        self.error = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._marks = torch.zeros(n, dtype=torch.int32, device=dev)
+        zeros = torch.zeros(1 + n, dtype=torch.int32, device=dev)
+        self.error, self._marks = zeros[:1], zeros[1:]
         self._k, self._v, align = plane_bases(layout, k_ptrs, v_ptrs, dev)
         self._index = index = dev.index
         self._state = KvPageState(

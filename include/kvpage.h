@@ -89,7 +89,8 @@ struct kv_page_cache {
  * order is that of the last.  Then the rows that grow take pages, in the order
  * of the call: row i is served if the pages that it and the rows before it in
  * the call ask for are there (status KVPAGE_NO_PAGES otherwise).
- * lens[i] = 0 frees a row.  status: [n] or NULL. */
+ * lens[i] = 0 frees a row.  A row that now ends inside a page which another
+ * row holds too is not to be appended to there.  status: [n] or NULL. */
 int kv_page_resize_launch(const struct kv_page_state *state, const int32_t *rows, const int32_t *lens,
                           uint32_t n, int32_t *status, void *stream);
 
