@@ -101,6 +101,11 @@ template <int K> __device__ __noinline__ void block_scan(int32_t *const *a, uint
     __syncthreads();
 }
 
+/* A call's second kernel is started while the first one runs (launch_after); it
+ * waits here for the first one's results, the first one lets it start there. */
+__device__ __forceinline__ void await_first() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void start_second() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 /* sets bit r; true if it was set already */
 __device__ __forceinline__ bool test_and_set(uint32_t *bits, uint32_t r)
 {
@@ -173,6 +178,7 @@ kv_page_resize_kernel(const kv_page_state s, const int32_t *__restrict__ rows, c
         seen[i] = 0;
     if (threadIdx.x == 0)
         served = all_drop = all_take = 0;
+    await_first();
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         const int32_t r = rows[i];
@@ -435,6 +441,7 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
     const uint32_t rank = cluster_rank(), ctas = cluster_size();
     const uint32_t lane = threadIdx.x & 31, warp0 = rank * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = ctas * (blockDim.x >> 5);
 
+    start_second();
     for (uint32_t i = threadIdx.x; i < 3 * words; i += blockDim.x)
         seen[i] = 0;
     if (threadIdx.x == 0)
@@ -565,7 +572,7 @@ int vector_of(const kv_page_cache *c)
 bool cache_ok(const kv_page_cache *c)
 {
     if (!c || !c->layer_k || !c->error || !c->unit_bytes || !c->block_size || !c->num_layers || !c->num_pages ||
-        c->num_pages > INT32_MAX || (c->base_align & (c->base_align - 1)))
+        c->num_layers > INT32_MAX / 2 || c->num_pages > INT32_MAX || (c->base_align & (c->base_align - 1)))
         return false;
     const uint64_t run = (uint64_t)c->block_size * c->unit_bytes;
     return run < (1ull << 31) && (!c->block_stride || c->block_stride >= run) &&
@@ -593,11 +600,12 @@ __device__ __forceinline__ uint8_t *plane(const Planes &p, uint32_t lk)
 
 /* ------------------------------------------------------------------------
  * copy.  A page in a plane is one run of vectors in every geometry.  Where a run
- * fills CTAs of 2048 vectors, a CTA moves that much of one run.  Shorter runs
- * (4 KiB: one head, 16 tokens) of all planes and pages lie on one line, of which
- * a CTA takes 2048 vectors, so that a thread still has eight loads in flight:
- * 256 half pages of 160 such planes took 95 us with a CTA per run, 40 like this;
- * four pages of 64 planes of 32 KiB 3.6 us with CTAs per run, 5.0 on the line.
+ * fills CTAs of 2048 vectors, a CTA moves that much of one run: four pages of 64
+ * planes of 32 KiB take 3.4 us, 500 of 27 planes of 72 KiB 297 us (6.7 TB/s).
+ * Shorter runs (4 KiB: one head, 16 tokens) go to a warp each, which finds its
+ * page, plane and tokens once: 256 pages of 160 such planes take 53 us (6.3
+ * TB/s), the first half of them 28; with a CTA per run the half took 95, with
+ * CTAs of 2048 vectors that each thread places by itself 37.
  * With a token count, a token-major page stops early and a head-major one skips
  * the tokens behind it.  `pack` is the distance between the entries of the
  * lists: 1, or 3 for fork's pairs.
@@ -609,7 +617,8 @@ constexpr uint32_t kMoveVectors = kMoveThreads * kMoveUnroll;
 struct Copy {
     const int32_t *src, *dst, *tokens;
     uint32_t pack, n, planes_per_grid;  /* planes of one grid row */
-    FastDiv run, per_head, per_token;   /* vectors of a page, of a head, of a token of one */
+    uint32_t run, per_token;            /* vectors of a page, of a token of one head */
+    FastDiv per_head;                   /* of a page's head */
     FastDiv pairs;          /* pages; for long runs, CTAs of one */
 };
 
@@ -618,6 +627,7 @@ template <int VEC>
 __global__ void __launch_bounds__(kMoveThreads) kv_page_copy_run_kernel(const Planes p, const __grid_constant__ Copy c)
 {
     using T = typename VecOf<VEC>::T;
+    await_first();
     const uint32_t i = fdiv(blockIdx.x, c.pairs), x0 = (blockIdx.x - i * c.pairs.d) * kMoveVectors + threadIdx.x;
     const int32_t a = c.src[(uint64_t)i * c.pack], b = c.dst[(uint64_t)i * c.pack];
     const int32_t keep = c.tokens ? min(max(c.tokens[(uint64_t)i * c.pack], 0), (int32_t)p.bs) : (int32_t)p.bs;
@@ -634,7 +644,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_page_copy_run_kernel(const Pl
     const T *from = reinterpret_cast<const T *>(base + (uint64_t)a * p.stride);
     T *to = reinterpret_cast<T *>(base + (uint64_t)b * p.stride);
     const bool part = p.head_bytes && keep < (int32_t)p.bs;
-    const uint32_t all = p.head_bytes ? c.run.d : (uint32_t)keep * c.per_token.d, used = (uint32_t)keep * c.per_token.d;
+    const uint32_t all = p.head_bytes ? c.run : (uint32_t)keep * c.per_token, used = (uint32_t)keep * c.per_token;
     T v[kMoveUnroll];
     bool on[kMoveUnroll];
 #pragma unroll
@@ -650,41 +660,49 @@ __global__ void __launch_bounds__(kMoveThreads) kv_page_copy_run_kernel(const Pl
             to[x0 + u * kMoveThreads] = v[u];
 }
 
+/* a warp per page and plane */
 template <int VEC>
-__global__ void __launch_bounds__(kMoveThreads) kv_page_copy_kernel(const Planes p, const __grid_constant__ Copy c)
+__global__ void __launch_bounds__(kMoveThreads, 8) kv_page_copy_warp_kernel(const Planes p, const __grid_constant__ Copy c)
 {
     using T = typename VecOf<VEC>::T;
-    const uint32_t lk0 = blockIdx.y * c.planes_per_grid;
-    const uint32_t items = min(c.planes_per_grid, p.layers * p.kvs - lk0) * c.n;
-    T v[kMoveUnroll];
-    T *to[kMoveUnroll];
-#pragma unroll
-    for (int u = 0; u < kMoveUnroll; u++) {
-        const uint32_t y = blockIdx.x * kMoveVectors + u * kMoveThreads + threadIdx.x;
-        const uint32_t item = fdiv(y, c.run), x = y - item * c.run.d;
-        to[u] = nullptr;
-        if (item >= items)
-            continue;
-        const uint32_t plane_in = fdiv(item, c.pairs), i = item - plane_in * c.n;
-        const int32_t a = c.src[(uint64_t)i * c.pack], b = c.dst[(uint64_t)i * c.pack];
-        const int32_t keep = c.tokens ? min(max(c.tokens[(uint64_t)i * c.pack], 0), (int32_t)p.bs) : (int32_t)p.bs;
-        const uint32_t head = fdiv(x, c.per_head), token = fdiv(x - head * c.per_head.d, c.per_token);
-        if ((int32_t)token >= keep || a == b)
-            continue;
-        if (a < 0 || (uint32_t)a >= p.pages || b < 0 || (uint32_t)b >= p.pages) {
+    constexpr int kUnroll = 4;
+    const uint32_t lk0 = blockIdx.y * c.planes_per_grid, lane = threadIdx.x % 32;
+    const uint32_t item = blockIdx.x * (kMoveThreads / 32) + threadIdx.x / 32;
+    if (item >= min(c.planes_per_grid, p.layers * p.kvs - lk0) * c.n)
+        return;
+    const uint32_t plane_in = fdiv(item, c.pairs), i = item - plane_in * c.n;
+    await_first();
+    const int32_t a = c.src[(uint64_t)i * c.pack], b = c.dst[(uint64_t)i * c.pack];
+    const int32_t keep = c.tokens ? min(max(c.tokens[(uint64_t)i * c.pack], 0), (int32_t)p.bs) : (int32_t)p.bs;
+    uint8_t *base = plane<VEC>(p, lk0 + plane_in);
+    if (!keep || a == b || !base)
+        return;
+    if (a < 0 || (uint32_t)a >= p.pages || b < 0 || (uint32_t)b >= p.pages) {
+        if (lane == 0)
             atomicOr(p.error, KVPAGE_ERR_PAGE);
-            continue;
-        }
-        uint8_t *base = plane<VEC>(p, lk0 + plane_in);
-        if (base) {
-            v[u] = reinterpret_cast<const T *>(base + (uint64_t)a * p.stride)[x];
-            to[u] = reinterpret_cast<T *>(base + (uint64_t)b * p.stride) + x;
-        }
+        return;
     }
+    const T *from = reinterpret_cast<const T *>(base + (uint64_t)a * p.stride);
+    T *to = reinterpret_cast<T *>(base + (uint64_t)b * p.stride);
+    const uint32_t used = (uint32_t)keep * c.per_token;
+    const bool part = p.head_bytes && keep < (int32_t)p.bs && c.per_head.d < c.run;
+    const uint32_t all = part || keep == (int32_t)p.bs ? c.run : used;
+#pragma unroll 1
+    for (uint32_t x0 = lane; x0 < all; x0 += 32 * kUnroll) {
+        T v[kUnroll];
+        bool on[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kMoveUnroll; u++)
-        if (to[u])
-            *to[u] = v[u];
+        for (int u = 0; u < kUnroll; u++) {
+            const uint32_t x = x0 + u * 32;
+            on[u] = x < all && !(part && x - fdiv(x, c.per_head) * c.per_head.d >= used);
+            if (on[u])
+                v[u] = from[x];
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; u++)
+            if (on[u])
+                to[x0 + u * 32] = v[u];
+    }
 }
 
 /* ------------------------------------------------------------------------
@@ -719,6 +737,7 @@ kv_page_compact_kernel(const Planes p, const kv_page_state s, const int32_t *__r
     const uint32_t i = blockIdx.y;
     const int32_t r = rows[i], st = start[i], o0 = offsets[i], o1 = offsets[i + 1];
     int32_t bad = 0;
+    start_second();
     if (threadIdx.x == 0) {
         s_first = INT32_MAX;
         s_bad = 0;
@@ -834,36 +853,47 @@ int launched()
     return cudaPeekAtLastError() == cudaSuccess ? 0 : -EIO;
 }
 
-constexpr size_t kPlanSmem = (6 * KVPAGE_MAX_CALL + kMaxUnits + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
-
-/* one cluster; the kernels' shared memory limit is raised once per device */
+/* a launch; `after`: as the second kernel of a call (await_first) */
 template <typename... P, typename... A>
-int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, int device, uint32_t threads, size_t smem,
-                cudaStream_t stream, A... args)
+int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t cluster, size_t smem, bool after, cudaStream_t stream, A... args)
 {
-    constexpr uint32_t ctas = kPlanCluster;
-    std::call_once(once[device], [&] {
-        err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
-    });
-    if (err[device] != cudaSuccess)
-        return -EIO;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(ctas);
+    cudaLaunchAttribute attr[2];
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    if (cluster) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    if (after) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
         cudaGetLastError();
         return -EIO;
     }
     return launched();
+}
+
+constexpr size_t kPlanSmem = (6 * KVPAGE_MAX_CALL + kMaxUnits + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
+
+/* one cluster; the kernels' shared memory limit is raised once per device */
+template <typename... P, typename... A>
+int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, int device, uint32_t threads, size_t smem,
+                bool after, cudaStream_t stream, A... args)
+{
+    std::call_once(once[device], [&] {
+        err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
+    });
+    if (err[device] != cudaSuccess)
+        return -EIO;
+    return launch(kernel, dim3(kPlanCluster), threads, kPlanCluster, smem, after, stream, args...);
 }
 
 /* Threads of the cluster's CTAs: barriers of 8 warps are cheap, and a small
@@ -875,13 +905,13 @@ uint32_t plan_threads(const kv_page_state *s, uint32_t n)
 }
 
 int resize_launch(const kv_page_state *s, const int32_t *rows, const int32_t *lens, uint32_t n, int32_t *status,
-                  cudaStream_t stream)
+                  bool after, cudaStream_t stream)
 {
     static std::once_flag once[64];
     static cudaError_t err[64];
     const uint64_t units = n + (uint64_t)n * s->width / kUnit;
     const size_t smem = (6 * (size_t)n + (units < kMaxUnits ? units : kMaxUnits) + 2 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
-    return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_threads(s, n), smem, stream, *s, rows, lens, n, status);
+    return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_threads(s, n), smem, after, stream, *s, rows, lens, n, status);
 }
 
 int call_ok(const kv_page_state *s, uint32_t n)
@@ -895,7 +925,7 @@ int call_ok(const kv_page_state *s, uint32_t n)
 
 template <int VEC>
 int copy_vec(const Planes &p, const int32_t *src, const int32_t *dst, const int32_t *tokens, uint32_t pack, uint32_t n,
-             cudaStream_t stream)
+             bool after, cudaStream_t stream)
 {
     Copy c{};
     c.src = src;
@@ -904,42 +934,34 @@ int copy_vec(const Planes &p, const int32_t *src, const int32_t *dst, const int3
     c.pack = pack;
     c.n = n;
     const uint32_t run = p.bs * (p.unit / VEC), planes = p.layers * p.kvs;
-    c.run = make_fastdiv(run);
-    c.per_token = make_fastdiv((p.head_bytes ? p.head_bytes : p.unit) / VEC);
-    c.per_head = make_fastdiv(p.bs * c.per_token.d);
+    c.run = run;
+    c.per_token = (p.head_bytes ? p.head_bytes : p.unit) / VEC;
+    c.per_head = make_fastdiv(p.bs * c.per_token);
     if (run >= kMoveVectors) {
         c.pairs = make_fastdiv((run + kMoveVectors - 1) / kMoveVectors);
         if ((uint64_t)n * c.pairs.d > INT32_MAX || planes > 65535)
             return -E2BIG;
-        kv_page_copy_run_kernel<VEC><<<dim3(n * c.pairs.d, planes), kMoveThreads, 0, stream>>>(p, c);
-        return launched();
+        return launch(kv_page_copy_run_kernel<VEC>, dim3(n * c.pairs.d, planes), kMoveThreads, 0, 0, after, stream, p, c);
     }
     c.pairs = make_fastdiv(n);
-    /* 31-bit indexes: planes of all pages that fit one row of the grid */
-    const uint64_t one = (uint64_t)n * run;
-    if (one >= (1ull << 31))
-        return -E2BIG;
-    c.planes_per_grid = (uint32_t)(((1ull << 31) - 1) / one);
-    if (c.planes_per_grid > planes)
-        c.planes_per_grid = planes;
+    c.planes_per_grid = INT32_MAX / n < planes ? INT32_MAX / n : planes;    /* 31-bit numbers of page and plane */
     const uint32_t grid_y = (planes + c.planes_per_grid - 1) / c.planes_per_grid;
     if (grid_y > 65535)
         return -E2BIG;
-    const uint32_t grid_x = (uint32_t)((one * c.planes_per_grid + kMoveVectors - 1) / kMoveVectors);
-    kv_page_copy_kernel<VEC><<<dim3(grid_x, grid_y), kMoveThreads, 0, stream>>>(p, c);
-    return launched();
+    const uint32_t grid_x = (n * c.planes_per_grid + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
+    return launch(kv_page_copy_warp_kernel<VEC>, dim3(grid_x, grid_y), kMoveThreads, 0, 0, after, stream, p, c);
 }
 
 int copy_launch(const kv_page_cache *c, const int32_t *src, const int32_t *dst, const int32_t *tokens, uint32_t pack,
-                uint32_t n, cudaStream_t stream)
+                uint32_t n, bool after, cudaStream_t stream)
 {
     const Planes p = planes_of(c);
     switch (vector_of(c)) {
-    case 16: return copy_vec<16>(p, src, dst, tokens, pack, n, stream);
-    case 8: return copy_vec<8>(p, src, dst, tokens, pack, n, stream);
-    case 4: return copy_vec<4>(p, src, dst, tokens, pack, n, stream);
-    case 2: return copy_vec<2>(p, src, dst, tokens, pack, n, stream);
-    default: return copy_vec<1>(p, src, dst, tokens, pack, n, stream);
+    case 16: return copy_vec<16>(p, src, dst, tokens, pack, n, after, stream);
+    case 8: return copy_vec<8>(p, src, dst, tokens, pack, n, after, stream);
+    case 4: return copy_vec<4>(p, src, dst, tokens, pack, n, after, stream);
+    case 2: return copy_vec<2>(p, src, dst, tokens, pack, n, after, stream);
+    default: return copy_vec<1>(p, src, dst, tokens, pack, n, after, stream);
     }
 }
 
@@ -966,9 +988,8 @@ int compact_vec(const Planes &p, const kv_page_state *s, const int32_t *rows, co
     if (per > slices)
         per = (uint32_t)slices;
     const uint32_t ctas = (uint32_t)((slices + per - 1) / per);
-    kv_page_compact_kernel<VEC><<<dim3(ctas, n), kMoveThreads, 0, stream>>>(p, *s, rows, start, keep, offsets, num_keep, n,
-                                                                        vecs, (uint32_t)slices, per, scratch);
-    return launched();
+    return launch(kv_page_compact_kernel<VEC>, dim3(ctas, n), kMoveThreads, 0, 0, false, stream, p, *s, rows, start, keep, offsets,
+                  num_keep, n, vecs, (uint32_t)slices, per, scratch);
 }
 
 }  // namespace
@@ -986,7 +1007,7 @@ extern "C" int kv_page_resize_launch(const struct kv_page_state *s, const int32_
     DeviceGuard on(s->device);
     if (!on.ok)
         return -EIO;
-    return resize_launch(s, rows, lens, n, status, static_cast<cudaStream_t>(stream));
+    return resize_launch(s, rows, lens, n, status, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int kv_page_copy_launch(const struct kv_page_cache *c, const int32_t *src, const int32_t *dst,
@@ -998,10 +1019,12 @@ extern "C" int kv_page_copy_launch(const struct kv_page_cache *c, const int32_t 
         return 0;
     if (!src || !dst)
         return -EINVAL;
+    if (n > INT32_MAX)
+        return -E2BIG;
     DeviceGuard on(c->device);
     if (!on.ok)
         return -EIO;
-    return copy_launch(c, src, dst, tokens, 1, n, static_cast<cudaStream_t>(stream));
+    return copy_launch(c, src, dst, tokens, 1, n, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int kv_page_fork_launch(const struct kv_page_cache *c, const struct kv_page_state *s, const int32_t *parents,
@@ -1023,11 +1046,11 @@ extern "C" int kv_page_fork_launch(const struct kv_page_cache *c, const struct k
     static cudaError_t err[64];
     const size_t smem = (4 * (size_t)n + 3 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int ret = launch_plan(kv_page_fork_kernel, once, err, s->device, plan_threads(s, n), smem, st, *s, parents, children, n,
-                                pairs, status);
+    const int ret = launch_plan(kv_page_fork_kernel, once, err, s->device, plan_threads(s, n), smem, false, st, *s, parents,
+                                children, n, pairs, status);
     if (ret)
         return ret;
-    return copy_launch(c, pairs, pairs + 1, pairs + 2, 3, n, st);
+    return copy_launch(c, pairs, pairs + 1, pairs + 2, 3, n, true, st);
 }
 
 extern "C" int kv_page_compact_launch(const struct kv_page_cache *c, const struct kv_page_state *s, const int32_t *rows,
@@ -1056,5 +1079,5 @@ extern "C" int kv_page_compact_launch(const struct kv_page_cache *c, const struc
     case 2: ret = compact_vec<2>(p, s, rows, start, keep, offsets, num_keep, n, scratch, st); break;
     default: ret = compact_vec<1>(p, s, rows, start, keep, offsets, num_keep, n, scratch, st); break;
     }
-    return ret ? ret : resize_launch(s, rows, scratch, n, status, st);
+    return ret ? ret : resize_launch(s, rows, scratch, n, status, true, st);
 }

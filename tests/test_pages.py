@@ -150,3 +150,10 @@ def test_the_model_keeps_its_invariants():
         held = [int(p) for r in range(6) for p in m.table[r, :-(-int(m.lens[r]) // 4)]]
         assert sorted(set(held) | set(m.free)) == list(range(20)) and not set(held) & set(m.free)
         assert [held.count(p) for p in range(20)] == m.refs.tolist()
+
+
+def test_copies_of_too_many_pages_are_refused():
+    c = cache(num_layers=1)
+    assert lib.kv_page_copy_launch(C.addressof(c), X, X, None, (1 << 31) + 5, None) == -errno.E2BIG
+    c = cache(num_layers=1 << 30)
+    assert lib.kv_page_copy_launch(C.addressof(c), X, X, None, 1, None) == -errno.EINVAL
