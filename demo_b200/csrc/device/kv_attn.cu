@@ -1318,79 +1318,130 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
 /* ------------------------------------------------------------------------
  * join: the pieces of the row tiles that lie across CTAs, in their order.  The
  * tiles' rows, however many each has, are dealt evenly to the grid's warps; a
- * lane has four dimensions of a row, and eight loads are in flight.
+ * lane has four dimensions of a row, and eight loads are in flight.  Where there
+ * are fewer rows than CTAs a row is a CTA's: those of a short call lie in many
+ * pieces (one token's 32, of 2048 positions, in 33 each: 15.5 us instead of
+ * 17.7 with a warp for a row).
  * (Joining in the first kernel, by the CTA that finishes a row tile last, takes
  * no second launch but left long joins to a few CTAs: 424 us instead of 98 for
  * 8 contexts in 37 pieces each.)
  * ---------------------------------------------------------------------- */
+/* a row's maximum and sum, and four dimensions of its result, of some pieces */
+struct Partial {
+    float m = -INFINITY, l = 0;
+    float4 o = make_float4(0, 0, 0, 0);
+
+    /* weighs everything for a maximum of `top` */
+    __device__ __forceinline__ void raise(float top)
+    {
+        const float keep = exp2_approx(m - top);
+        m = top;
+        l *= keep;
+        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+    }
+    __device__ __forceinline__ void add(float m2, float l2, const float4 &v)
+    {
+        const float f = exp2_approx(m2 - m);
+        l += f * l2;
+        o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+    }
+};
+
+/* pieces k0 .. k1 of rows r .. r + R, P of them in flight together; rows from r1 on are not there */
+template <int R, int P>
+__device__ __forceinline__ void join_pieces(const Params &p, const Job &job, uint32_t cta, int32_t r, int32_t r1, int32_t k0, int32_t k1,
+                                            uint32_t c, Partial *x)
+{
+    /* piece k's rows: the first piece's slot, then slot 0 of the CTAs behind */
+    auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (cta + k) : (uint32_t)job.slot) * kRows; };
+#pragma unroll 1
+    for (; k0 < k1; k0 += P) {
+        float2 ml[R][P];
+        float4 v[R][P];
+#pragma unroll
+        for (int k = 0; k < P; k++)
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const bool on = k0 + k < k1 && r + i < r1;
+                const uint64_t row = at(k0 + k) + r + i;
+                ml[i][k] = on ? *reinterpret_cast<const float2 *>(p.part_ml + row * 2) : make_float2(0, 0);
+                v[i][k] = on ? *reinterpret_cast<const float4 *>(p.part_o + row * p.d.head_dim + c) : make_float4(0, 0, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            float top = x[i].m;
+#pragma unroll
+            for (int k = 0; k < P; k++)
+                if (ml[i][k].y != 0)        /* else it sees nothing there, and its sums were not written */
+                    top = fmaxf(top, ml[i][k].x);
+            if (top == -INFINITY)
+                continue;
+            x[i].raise(top);
+#pragma unroll
+            for (int k = 0; k < P; k++)
+                if (ml[i][k].y != 0)
+                    x[i].add(ml[i][k].x, ml[i][k].y, v[i][k]);
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void join_out(const Params &p, const Job &job, int32_t r, uint32_t c, const Partial &x)
+{
+    const kv_attn_desc &d = p.d;
+    const int32_t node = r / (int32_t)p.group, sub = r - node * (int32_t)p.group;
+    const float inv = x.l == 0 ? 0.f : d.v_scale / x.l;
+    T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
+    *reinterpret_cast<uint2 *>(out + c) = make_uint2(Type<T>::pack(x.o.x * inv, x.o.y * inv), Type<T>::pack(x.o.z * inv, x.o.w * inv));
+    if (c == 0 && d.lse)
+        d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] = x.l == 0 ? -INFINITY : (x.m + log2f(x.l)) * kLn2;
+}
+
 /* rows r0 .. r1 of a job, R rows and P pieces in flight together */
 template <typename T, int R, int P>
 __device__ __forceinline__ void join_rows(const Params &p, const Job &job, uint32_t cta, int32_t r0, int32_t r1, uint32_t lane)
 {
-    const kv_attn_desc &d = p.d;
-    /* piece k's rows: the first piece's slot, then slot 0 of the CTAs behind */
-    auto at = [&](int32_t k) { return (uint64_t)(k ? 2 * (cta + k) : (uint32_t)job.slot) * kRows; };
-    for (uint32_t c = lane * 4; c < d.head_dim; c += 128)
+    for (uint32_t c = lane * 4; c < p.d.head_dim; c += 128)
 #pragma unroll 1
         for (int32_t r = r0; r < r1; r += R) {
-            float m[R], l[R];
-            float4 o[R];
-#pragma unroll
-            for (int i = 0; i < R; i++) {
-                m[i] = -INFINITY;
-                l[i] = 0;
-                o[i] = make_float4(0, 0, 0, 0);
-            }
-#pragma unroll 1
-            for (int32_t k0 = 0; k0 < job.ctas; k0 += P) {
-                float2 ml[R][P];
-                float4 v[R][P];
-#pragma unroll
-                for (int k = 0; k < P; k++)
-#pragma unroll
-                    for (int i = 0; i < R; i++) {
-                        const bool on = k0 + k < job.ctas && r + i < r1;
-                        const uint64_t row = at(k0 + k) + r + i;
-                        ml[i][k] = on ? *reinterpret_cast<const float2 *>(p.part_ml + row * 2) : make_float2(0, 0);
-                        v[i][k] = on ? *reinterpret_cast<const float4 *>(p.part_o + row * d.head_dim + c) : make_float4(0, 0, 0, 0);
-                    }
-#pragma unroll
-                for (int i = 0; i < R; i++) {
-                    float top = m[i];
-#pragma unroll
-                    for (int k = 0; k < P; k++)
-                        if (ml[i][k].y != 0)    /* else it sees nothing there, and its sums were not written */
-                            top = fmaxf(top, ml[i][k].x);
-                    if (top == -INFINITY)
-                        continue;
-                    const float keep = exp2_approx(m[i] - top);
-                    m[i] = top;
-                    l[i] *= keep;
-                    o[i] = make_float4(o[i].x * keep, o[i].y * keep, o[i].z * keep, o[i].w * keep);
-#pragma unroll
-                    for (int k = 0; k < P; k++) {
-                        if (ml[i][k].y == 0)
-                            continue;
-                        const float f = exp2_approx(ml[i][k].x - top);
-                        l[i] += f * ml[i][k].y;
-                        o[i] = make_float4(o[i].x + f * v[i][k].x, o[i].y + f * v[i][k].y, o[i].z + f * v[i][k].z, o[i].w + f * v[i][k].w);
-                    }
-                }
-            }
+            Partial x[R];
+            join_pieces<R, P>(p, job, cta, r, r1, 0, job.ctas, c, x);
 #pragma unroll
             for (int i = 0; i < R; i++) {
                 if (r + i >= r1)
                     break;
-                const int32_t node = (r + i) / (int32_t)p.group, sub = r + i - node * (int32_t)p.group;
-                const float inv = l[i] == 0 ? 0.f : d.v_scale / l[i];
-                T *out = static_cast<T *>(d.out) + (int64_t)(job.q0 + node) * d.out_stride + (int64_t)(job.h * p.group + sub) * d.out_head_stride;
-                *reinterpret_cast<uint2 *>(out + c) =
-                    make_uint2(Type<T>::pack(o[i].x * inv, o[i].y * inv), Type<T>::pack(o[i].z * inv, o[i].w * inv));
-                if (c == 0 && d.lse)
-                    d.lse[(int64_t)(job.q0 + node) * d.num_heads + job.h * p.group + sub] =
-                        l[i] == 0 ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+                join_out<T>(p, job, r + i, c, x[i]);
             }
         }
+}
+
+/* one row by the whole CTA: each warp joins some of the pieces, the first one what they have */
+template <typename T>
+__device__ __forceinline__ void join_row(const Params &p, const Job &job, uint32_t cta, int32_t r, uint32_t lane, uint32_t warp)
+{
+    constexpr int kWarps = kJoinThreads / 32;
+    __shared__ Partial of[kWarps][32];
+    const int32_t each = (job.ctas + kWarps - 1) / kWarps, k0 = warp * each, k1 = min(job.ctas, k0 + each);
+    for (uint32_t c0 = 0; c0 < p.d.head_dim; c0 += 128) {
+        const uint32_t c = c0 + lane * 4;
+        Partial x;
+        if (c < p.d.head_dim)
+            join_pieces<1, 8>(p, job, cta, r, r + 1, k0, k1, c, &x);
+        of[warp][lane] = x;
+        __syncthreads();
+        if (warp == 0 && c < p.d.head_dim) {
+            for (int w = 1; w < kWarps; w++) {
+                const Partial y = of[w][lane];
+                if (y.l == 0)
+                    continue;
+                const float top = fmaxf(x.m, y.m);
+                x.raise(top);
+                x.add(y.m, y.l, y.o);
+            }
+            join_out<T>(p, job, r, c, x);
+        }
+        __syncthreads();
+    }
 }
 
 template <typename T>
@@ -1430,8 +1481,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid
     for (int k = 0; k < kEach; k++)
         upto[threadIdx.x * kEach + k] = inc += rows[k];
     __syncthreads();
-    const int32_t warps = gridDim.x * (kJoinThreads / 32), each = (total + warps - 1) / warps;
-    int32_t u = (blockIdx.x * (kJoinThreads / 32) + warp) * each;
+    const bool few = total <= (int32_t)gridDim.x;   /* then a CTA takes a row */
+    const int32_t warps = gridDim.x * (kJoinThreads / 32), each = few ? 1 : (total + warps - 1) / warps;
+    int32_t u = few ? blockIdx.x : (blockIdx.x * (kJoinThreads / 32) + warp) * each;
     const int32_t end = min(total, u + each);
     while (u < end) {
         uint32_t lo = 0, hi = ctas - 1;         /* the job whose rows go past u */
@@ -1445,7 +1497,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attn_join_kernel(const __grid
         const Job job = p.jobs[lo];
         const int32_t r0 = u - (upto[lo] - job.rows), r1 = min(job.rows, r0 + end - u);
         /* most have two pieces: then four rows together */
-        if (job.ctas == 2)
+        if (few)
+            join_row<T>(p, job, lo, r0, lane, warp);
+        else if (job.ctas == 2)
             join_rows<T, 4, 2>(p, job, lo, r0, r1, lane);
         else
             join_rows<T, 1, 8>(p, job, lo, r0, r1, lane);
