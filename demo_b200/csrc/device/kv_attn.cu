@@ -68,7 +68,8 @@ constexpr int kSoftmax = 128;       /* threads of the softmax */
  * 16-byte copies that are widened (8-bit caches) */
 enum Load { kTma, kCopy, kWiden };
 template <Load L> struct Roles {
-    static constexpr int kLoaders = L == kTma ? 64 : 128;           /* kTma: a warp for K and one for V */
+    static constexpr int kLoaders = L == kTma ? 64 : L == kCopy ? 128 : 256;  /* but for kCopy a half for K and one for V */
+    static constexpr int kFill = L == kTma ? 1 : 128;               /* threads that arrive for a tile */
     static constexpr int kThreads = kSoftmax + kLoaders + 64;       /* a warp for the products, one that plans */
 };
 /* Beginning and ending a row tile (Q, the first S, O out) takes as long as about
@@ -273,7 +274,7 @@ struct Shared {
     uint32_t tmem;
     volatile uint32_t dead;         /* a wait ran out: every role leaves */
     volatile uint32_t spoilt[4];    /* [piece % 4] == piece + 1: values of its fed nodes that are not finite were set aside */
-    int64_t share, scan[Roles<kCopy>::kThreads / 32];
+    int64_t share, scan[Roles<kWiden>::kThreads / 32];
     Line line;                      /* the CTA's part of it */
 };
 static_assert(sizeof(Shared) <= 1024, "the last KiB of the dynamic shared memory");
@@ -628,7 +629,7 @@ template <typename T, Load L, int DP> struct Loader {
 
     __device__ void take_rows()
     {
-        const uint32_t t = threadIdx.x - kSoftmax, lane = t % 32, warp = t / 32;
+        const uint32_t t = (threadIdx.x - kSoftmax) % 128, lane = t % 32, warp = t / 32;
         chunk = t % kChunks;
         row = t / kChunks;
         own_row = lane % 16 / kWarpRows * kPass + warp * kWarpRows + lane % kWarpRows;
@@ -701,13 +702,12 @@ template <typename T, Load L, int DP> struct Loader {
         }
     }
 
-    /* 8-bit caches: copied as they are, kRaw - 1 tiles of K or V ahead, to
-     * places in shared memory that only the copying thread uses; that thread
-     * widens them into the rings. */
-    __device__ __forceinline__ uint8_t *raw(uint32_t k, uint32_t c, int i) const
+    /* 8-bit caches: copied as they are, to places in shared memory that only the
+     * copying thread uses, a tile ahead; that thread widens them into the rings. */
+    __device__ __forceinline__ uint8_t *raw(bool v, uint32_t k, uint32_t c, int i) const
     {
-        return ring + (S::kSlotsK + S::kSlotsV) * S::kSlotBytes + (k % S::kRaw) * (S::kSlotBytes / 2) +
-               (c * kPasses + i) * (128 * 16) + (threadIdx.x - kSoftmax) * 16;
+        return ring + (S::kSlotsK + S::kSlotsV) * S::kSlotBytes + (2 * v + k % 2) * (S::kSlotBytes / 2) + (c * kPasses + i) * (128 * 16) +
+               (threadIdx.x - kSoftmax) % 128 * 16;
     }
 
     __device__ bool widen(uint32_t k, bool v)
@@ -719,7 +719,7 @@ template <typename T, Load L, int DP> struct Loader {
             if (c * kColumn + chunk * 16 < p.d.head_dim)
 #pragma unroll
                 for (int i = 0; i < kPasses; i++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(raw(k, c, i));
+                    const uint4 w = *reinterpret_cast<const uint4 *>(raw(v, k, c, i));
                     const uint32_t r = row + i * kPass;
                     uint8_t *to = slot(v) + c * kColumnBytes;
                     *reinterpret_cast<uint4 *>(to + swizzled(r, 2 * chunk)) =
@@ -734,32 +734,13 @@ template <typename T, Load L, int DP> struct Loader {
         return true;
     }
 
-    /* K of a tile comes before V of the tile before: S is needed a softmax
-     * earlier than O, and V's one slot is free only when that O is done */
-    __device__ void run_widen()
+    /* Four warps bring K, four V: with four for both, that widened a tile of
+     * each in turn, their instructions set the pace (OLDFIG). */
+    __device__ void run_widen(bool v)
     {
-        constexpr uint32_t kAhead = S::kRaw > 0 ? S::kRaw - 1 : 0;
         take_rows();
-        uint32_t k = 0, done = 0;           /* tiles fetched, widened: K, K, V, K, V .. V */
-        uint64_t last[kPasses];
+        uint32_t k = 0;                     /* tiles fetched; all but the last are widened */
         Piece e;
-        auto fetch = [&](bool v) {
-            copy_tile(v, [&](uint32_t c, int i) { return smem_u32(raw(k, c, i)); });
-            copy_commit();
-            if (k++ < kAhead)
-                return true;
-            copy_wait_but<kAhead>();
-            done++;
-            return widen(done - 1, done > 1 && (done & 1));
-        };
-        auto swap = [&] {
-#pragma unroll
-            for (int i = 0; i < kPasses; i++) {
-                const uint64_t o = off[i];
-                off[i] = last[i];
-                last[i] = o;
-            }
-        };
         for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
             int32_t t = e.top, page = look_up(e, t);
             for (int32_t left = e.t1 - e.t0; left > 0; left--) {
@@ -767,20 +748,18 @@ template <typename T, Load L, int DP> struct Loader {
                 t = e.behind(t);
                 if (left > 1)
                     page = look_up(e, t);
-                if (!fetch(false))
-                    return;
-                swap();
-                if (k > 1 && !fetch(true))
-                    return;
+                copy_tile(v, [&](uint32_t c, int i) { return smem_u32(raw(v, k, c, i)); });
+                copy_commit();
+                if (k++) {
+                    copy_wait_but<1>();
+                    if (!widen(k - 2, v))
+                        return;
+                }
             }
         }
-        swap();                             /* V of the last tile */
-        if (k && !fetch(true))
-            return;
         copy_wait_all();
-        for (; done < k; done++)
-            if (!widen(done, done > 0 && (!(done & 1) || done + 1 == k)))
-                return;
+        if (k)
+            widen(k - 1, v);
     }
 };
 
@@ -1256,11 +1235,11 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int k = 0; k < S::kSlotsK; k++) {
-            mbar_init(&sh.k_full[k], L == kTma ? 1 : Roles<L>::kLoaders);
+            mbar_init(&sh.k_full[k], Roles<L>::kFill);
             mbar_init(&sh.k_empty[k], 1);
         }
         for (int k = 0; k < S::kSlotsV; k++) {
-            mbar_init(&sh.v_full[k], L == kTma ? 1 : Roles<L>::kLoaders);
+            mbar_init(&sh.v_full[k], Roles<L>::kFill);
             mbar_init(&sh.v_empty[k], 1);
         }
         for (int k = 0; k < 2; k++) {
@@ -1300,7 +1279,7 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
             if constexpr (L == kTma) {
                 load.run_tma(warp != kSoftmax / 32);
             } else if constexpr (L == kWiden)
-                load.run_widen();
+                load.run_widen(warp >= (kSoftmax + 128) / 32);
             else
                 load.run_copy();
             copy_wait_all();
