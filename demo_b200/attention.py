@@ -105,8 +105,14 @@ class TreeAttention:
                 q.stride(2) != 1:
             raise ValueError(f"q: expected a bfloat16 or float16 CUDA tensor [total, {self.num_heads}, {self.head_dim}]")
         if stream is not None:
+            caller = torch.cuda.current_stream(index)
             with _on_stream(stream, index):
-                return self(layer, q, block_table, seq_lens, q_offsets, parents, rows, out, return_lse)
+                res = self(layer, q, block_table, seq_lens, q_offsets, parents, rows, out, return_lse)
+            for t in res if return_lse else (res,):
+                t.record_stream(caller)     # which may be where it is used and dropped
+            return res
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("q: attention over a cache has no gradients; call it under torch.no_grad()")
         total = q.shape[0]
         q_strides = q.stride()
         if 0 in q_strides:                              # an expanded tensor

@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kMoveThreads, 8) kv_page_copy_warp_kernel(cons
  * of them decide alike; 4 bytes of list against 64 bytes or more of slice.
  * The first CTA of a row leaves the new length for resize, or kRefused.
  * Half of 16000 tokens of 64 planes of 2 KiB units: 305 us, 5.2 TB/s; up to 5 of
- * 24 tokens of 64 rows: 20 us, most of it the checks' dependent loads.
+ * 24 tokens of 64 rows: 17 us, most of it the checks' dependent loads.
  * ---------------------------------------------------------------------- */
 template <int VEC>
 __global__ void __launch_bounds__(kMoveThreads, 4)
@@ -982,14 +982,14 @@ int compact_vec(const Planes &p, const kv_page_state *s, const int32_t *rows, co
     if (slices > INT32_MAX)
         return -E2BIG;
     /* A CTA reads and checks its row's list before it moves anything.  Where the
-     * lists are short that is most of its time, and CTAs that fill the GPU about
-     * once take many slices each, side by side (5 of 24 tokens of 64 rows: 37 us
-     * with the resizes, 64 with 8192 CTAs); long lists want many CTAs, since rows
-     * differ in length. */
-    const uint64_t want = num_keep / n < kMoveVectors / 16 ? 888 : 8192;
-    uint32_t per = (uint32_t)((slices * n + want - 1) / want);
-    if (per > slices)
-        per = (uint32_t)slices;
+     * lists are short that is most of its time, and the CTAs that the GPU holds
+     * at once (592) take many slices each, side by side; for many rows twice as
+     * many, so that none has too many batches.  Keeping up to 5 of 24 tokens, with
+     * the resizes: 64 rows 32.7 us with 592, 36.1 with 888, 35.6 with 1184; 256
+     * rows 92, 86, 81.  Long lists want many CTAs, since rows differ in length. */
+    const uint32_t all = num_keep / n >= kMoveVectors / 16 ? 8192 : n <= 148 ? 592 : 1184;
+    const uint32_t row_ctas = all / n ? all / n : 1;
+    const uint32_t per = (uint32_t)((slices + row_ctas - 1) / row_ctas);
     const uint32_t ctas = (uint32_t)((slices + per - 1) / per);
     return launch(kv_page_compact_kernel<VEC>, dim3(ctas, n), kMoveThreads, 0, 0, false, stream, p, *s, rows, start, keep, offsets,
                   num_keep, n, vecs, (uint32_t)slices, per, scratch);

@@ -518,6 +518,18 @@ def test_memory_in_use_on_another_stream_is_left_alone():
         assert torch.equal(got, want)
 
 
+def test_gradients_are_refused():
+    b = Batch([30], [2], seed=23)
+    args, _ = b.args()
+    att = b.attention()
+    want = att(*args)
+    q = b.q.clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradients"):
+        att(0, q, *args[2:])
+    with torch.no_grad():
+        assert torch.equal(att(0, q, *args[2:]), want)
+
+
 def test_the_first_call_is_captured():
     b = Batch([300, 17], [2, 1], seed=22)
     args, _ = b.args()
