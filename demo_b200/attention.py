@@ -153,10 +153,12 @@ class TreeAttention:
     def check(self) -> None:
         """Wait for the device and raise ValueError for what the calls since
         the last check() found wrong in their arguments."""
-        for error, _, _ in self._devices.values():
+        for index, (error, _, _) in self._devices.items():
+            torch.cuda.synchronize(index)       # calls on all streams
             bits = int(error.item())
             if bits:
                 error.zero_()
+                torch.cuda.synchronize(index)
                 raise ValueError("tree attention: " + "; ".join(text for bit, text in _ERRORS if bits & bit))
 
 

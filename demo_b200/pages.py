@@ -195,9 +195,11 @@ class PagePool:
     def check(self) -> None:
         """Wait for the device and raise ValueError for what the calls since
         the last check() found wrong in their arguments."""
+        torch.cuda.synchronize(self.device)     # calls on all streams
         bits = int(self.error.item())
         if bits:
             self.error.zero_()
+            torch.cuda.synchronize(self.device)
             raise ValueError("page pool: " + "; ".join(text for bit, text in _ERRORS if bits & bit))
 
 

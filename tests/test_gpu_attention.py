@@ -518,6 +518,22 @@ def test_memory_in_use_on_another_stream_is_left_alone():
         assert torch.equal(got, want)
 
 
+def test_check_waits_for_every_stream():
+    b = Batch([30], [2], seed=24)
+    args, _ = b.args()
+    att = b.attention()
+    att(*args)
+    args[3].fill_(1)                    # shorter than its nodes
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    att(*args, stream=side)
+    with pytest.raises(ValueError, match="length"):
+        att.check()
+    att.check()
+
+
 def test_gradients_are_refused():
     b = Batch([30], [2], seed=23)
     args, _ = b.args()

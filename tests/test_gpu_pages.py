@@ -350,3 +350,17 @@ def test_results_on_a_side_stream():
     assert got.tolist() == [pg.OK, pg.OK]
     c.model.resize([0, 1], [100, 37])
     c.same()
+
+
+def test_check_waits_for_every_stream():
+    c = Case(GEOMETRIES["hnd"], 60, 4, 8)
+    rows, lens = ints([9]), ints([16])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    got = c.pool.resize(rows, lens, stream=side)
+    with pytest.raises(ValueError, match="row"):
+        c.pool.check()
+    c.pool.check()
+    assert got.tolist() == [pg.INVALID]
