@@ -23,8 +23,8 @@
  * takes 15.5 us (launch, line, one tile, join: latencies); 64 trees of 9 to 32
  * nodes over up to 2048 positions 83 us (361 MB, 4.3 TB/s); 32 chains of 4 nodes
  * over up to 8192 positions of e4m3 141 us (402 MB, 2.9 TB/s: the widening);
- * 8 heads over one: 8 trees of 64 nodes over up to 131072 positions 185 us (172
- * GFLOP, 0.93 PFLOP/s: the chain of products and exponentials).
+ * 8 heads over one: 8 trees of 64 nodes over up to 131072 positions 180 us (172
+ * GFLOP, 0.96 PFLOP/s: the chain of products and exponentials).
  *
  * Warps 0-3 are the softmax (a thread owns a TMEM lane, a row), then come the
  * loaders, a warp that issues the products, and one that finds the next pieces
@@ -421,6 +421,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *a)
                  "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
                  "tcgen05.wait::ld.sync.aligned;"
                  : R8(a, 0), R8(a, 8), R8(a, 16), R8(a, 24) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t *a)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+                 "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : R8(a, 0), R8(a, 8), R8(a, 16), R8(a, 24), R8(a, 32), R8(a, 40), R8(a, 48), R8(a, 56) : "r"(addr) : "memory");
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *a)
@@ -960,12 +970,17 @@ __device__ bool set_aside(const Params &p, const Piece &e, int32_t t, uint8_t *s
     return any;
 }
 
-/* -inf for the scores whose bit is off */
-__device__ __forceinline__ void hide(float *s, uint32_t bits)
+/* N scores of the row, -inf where the bit is off */
+template <int N> __device__ __forceinline__ void scores(uint32_t addr, uint32_t *raw, bool mask, uint64_t bits)
 {
+    if constexpr (N == 64)
+        tmem_ld64(addr, raw);
+    else
+        tmem_ld32(addr, raw);
+    if (mask)
 #pragma unroll
-    for (int c = 0; c < 32; c++)
-        s[c] = bits >> c & 1 ? s[c] : -INFINITY;
+        for (int c = 0; c < N; c++)
+            raw[c] = bits >> c & 1 ? raw[c] : __float_as_uint(-INFINITY);
 }
 
 template <typename T, Load L, int DP>
@@ -1004,21 +1019,21 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
             if (!wait_warp(sh, d.error, &sh.s_full[g & 1], (g >> 1) & 1))
                 return;
             if (work) {
-                /* The maximum first, then the scores again, 32 at a time: the
-                 * second reading is cheap, and a short loop stays in the
-                 * instruction cache beside the other roles'. */
-                uint32_t raw[32];
-                float *s = reinterpret_cast<float *>(raw);
+                /* The maximum first.  Where two loading warps leave registers for
+                 * all scores they stay (8 trees of 64 nodes over up to 131072
+                 * positions: 180 us, 189 read twice); with four or more they are
+                 * read again (64 trees on pages of 24: 89 us, 97 with spills). */
+                constexpr int kHeld = L == kTma ? 64 : 32;
+                uint32_t raw[kHeld];
+                const float *s = reinterpret_cast<const float *>(raw);
                 float now = -INFINITY;
                 tmem_fence_after();
 #pragma unroll 1
-                for (int half = 0; half < kTile; half += 32) {
-                    tmem_ld32(s_at + half, raw);
-                    if (mask)
-                        hide(s, (uint32_t)(bits >> half));
+                for (int part = 0; part < kTile; part += kHeld) {
+                    scores<kHeld>(s_at + part, raw, mask, bits >> part);
                     float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int c = 4; c < 32; c++)
+                    for (int c = 4; c < kHeld; c++)
                         top[c & 3] = fmaxf(top[c & 3], s[c]);
                     now = fmaxf(now, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                 }
@@ -1036,30 +1051,33 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
                     tmem_fence_after();
 #pragma unroll 1
                     for (uint32_t c = 0; c < d.head_dim; c += 16) {
-                        tmem_ld16(o_at + c, raw);
+                        uint32_t o[16];
+                        tmem_ld16(o_at + c, o);
 #pragma unroll
                         for (int k = 0; k < 16; k++)
-                            s[k] *= f;
-                        tmem_st16(o_at + c, raw);
+                            o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tmem_st16(o_at + c, o);
                     }
                 }
                 const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
 #pragma unroll 1
-                for (int half = 0; half < kTile; half += 32) {
-                    tmem_ld32(s_at + half, raw);
-                    if (mask)
-                        hide(s, (uint32_t)(bits >> half));
-                    float sum[4] = {};
-                    uint32_t w[16];
+                for (int part = 0; part < kTile; part += kHeld) {
+                    if (kHeld < kTile)
+                        scores<kHeld>(s_at + part, raw, mask, bits >> part);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float a = exp2_approx(fmaf(s[c], s2, -from)), b = exp2_approx(fmaf(s[c + 1], s2, -from));
-                        sum[c & 2] += a;
-                        sum[(c & 2) + 1] += b;
-                        w[c / 2] = Type<T>::pack(a, b);
+                    for (int half = 0; half < kHeld; half += 32) {
+                        float sum[4] = {};
+                        uint32_t w[16];
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const float a = exp2_approx(fmaf(s[half + c], s2, -from)), b = exp2_approx(fmaf(s[half + c + 1], s2, -from));
+                            sum[c & 2] += a;
+                            sum[(c & 2) + 1] += b;
+                            w[c / 2] = Type<T>::pack(a, b);
+                        }
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        tmem_st16(s_at + (part + half) / 2, w);     /* over scores that have been read */
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st16(s_at + half / 2, w);      /* over scores that have been read */
                 }
                 tmem_wait_st();
                 tmem_fence_before();
