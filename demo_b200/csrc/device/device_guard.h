@@ -10,13 +10,14 @@ struct DeviceGuard {
     explicit DeviceGuard(int device)
     {
         int now = -1;
-        if (device < 0 || cudaGetDevice(&now) != cudaSuccess)
+        if (device < 0)
             return;
-        if (now != device) {
-            if (cudaSetDevice(device) != cudaSuccess)
-                return;
-            before = now;
+        if (cudaGetDevice(&now) != cudaSuccess || (now != device && cudaSetDevice(device) != cudaSuccess)) {
+            cudaGetLastError();     /* reported here, and not left for a later call to find */
+            return;
         }
+        if (now != device)
+            before = now;
         ok = true;
     }
     ~DeviceGuard()

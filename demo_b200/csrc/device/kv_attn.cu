@@ -1622,17 +1622,24 @@ int launch(const Params &p, cudaStream_t stream)
     });
     if (err[dev] != cudaSuccess)
         return -EIO;
+    /* what a launch returns counts, not the thread's last error: that may be an
+     * earlier call's, and without the second kernel the results would be parts */
     const unsigned grid = (unsigned)grid_of(&p.d);
-    kv_attn_kernel<T, L, DP><<<grid, Roles<L>::kThreads, Shape<L, DP>::kSmem, stream>>>(p);
-    g_cc_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-    if (cudaPeekAtLastError() != cudaSuccess)
-        return -EIO;
-    /* started while the first kernel drains; it waits for its results on the device */
     cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(Roles<L>::kThreads);
+    cfg.dynamicSmemBytes = Shape<L, DP>::kSmem;
+    cfg.stream = stream;
+    if (cudaLaunchKernelEx(&cfg, kv_attn_kernel<T, L, DP>, p) != cudaSuccess) {
+        cudaGetLastError();
+        return -EIO;
+    }
+    g_cc_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+    /* started while the first kernel drains; it waits for its results on the device */
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3(2 * grid);
     cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = stream;
+    cfg.dynamicSmemBytes = 0;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;

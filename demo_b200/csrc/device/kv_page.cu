@@ -849,13 +849,10 @@ kv_page_compact_kernel(const Planes p, const kv_page_state s, const int32_t *__r
 }
 
 /* ---- launches ---- */
-int launched()
-{
-    g_cc_kernel_launches.fetch_add(1, std::memory_order_relaxed);
-    return cudaPeekAtLastError() == cudaSuccess ? 0 : -EIO;
-}
-
-/* a launch; `after`: as the second kernel of a call (await_first) */
+/* A launch; `after`: as the second kernel of a call (await_first).  Only what the
+ * launch itself returns counts: the thread's last error may be that of an
+ * earlier call that has nothing to do with this one, and a call that took it
+ * for its own would stop between its two kernels. */
 template <typename... P, typename... A>
 int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t cluster, size_t smem, bool after, cudaStream_t stream, A... args)
 {
@@ -880,7 +877,8 @@ int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t cluster, 
         cudaGetLastError();
         return -EIO;
     }
-    return launched();
+    g_cc_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+    return 0;
 }
 
 constexpr size_t kPlanSmem = (6 * KVPAGE_MAX_CALL + kMaxUnits + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
@@ -892,6 +890,8 @@ int launch_plan(void (*kernel)(P...), std::once_flag *once, cudaError_t *err, in
 {
     std::call_once(once[device], [&] {
         err[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlanSmem);
+        if (err[device] != cudaSuccess)
+            cudaGetLastError();
     });
     if (err[device] != cudaSuccess)
         return -EIO;
