@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import KvAttnDesc, lib
 from .cache import CacheError, KVLayout
-from .pages import _current_stream, _int32, _on_stream
+from .pages import _current_stream, _int32, _on_stream, _used_on
 
 # struct kv_attn_desc in one go: 12 pointers, 8 64-bit numbers, 12 32-bit ones, three floats, the device
 _DESC = struct.Struct("@12PQQqqqqq10I2i3fi")
@@ -97,7 +97,10 @@ class TreeAttention:
         rows         int32 [sequences]: their rows; None: row b
 
         Runs on `stream`, by default the current stream of q's device, to which
-        the results then belong.  May be captured, except for the first call on
+        the results then belong.  The arguments may be dropped when the call
+        returns; the object must outlive its calls, and the graphs that captured
+        them.  Queries that no sequence covers leave their rows of out and lse as
+        they were, which in new tensors is anything.  May be captured, except for the first call on
         a device that was not the current one when the object was made.
         """
         index, kind = q.get_device(), _TYPES.get(q.dtype)
@@ -110,6 +113,7 @@ class TreeAttention:
                 res = self(layer, q, block_table, seq_lens, q_offsets, parents, rows, out, return_lse)
             for t in res if return_lse else (res,):
                 t.record_stream(caller)     # which may be where it is used and dropped
+            _used_on(stream, q, block_table, seq_lens, q_offsets, parents, rows, out)
             return res
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("q: attention over a cache has no gradients; call it under torch.no_grad()")

@@ -43,6 +43,16 @@ def _on_stream(stream: torch.cuda.Stream, index: int):
     return torch.cuda.stream(stream)
 
 
+def _used_on(stream: torch.cuda.Stream | None, *tensors: torch.Tensor | None) -> None:
+    """What a call on `stream` was given: the caller may drop it when the call
+    returns, and its memory must not be handed out again before the stream has
+    come that far."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _int32(name: str, t: torch.Tensor, index: int, numel: int | None = None) -> int:
     """data pointer of a contiguous int32 tensor on CUDA device `index` (-1:
     the CPU); ValueError otherwise"""
@@ -85,8 +95,10 @@ class PagePool:
     kernels.  Calls run on `stream`, by default the current stream of the
     cache's device, in the order they are made; calls for one pool on several
     streams have to be ordered by the caller, and results belong to the stream
-    of their call.  The int32 results of resize,
-    fork and compact say per row pages.OK, NO_PAGES or INVALID, on the device.
+    of their call.  A call's arguments may be dropped when it returns; the pool
+    itself must outlive its calls, and the graphs that captured them.  The int32
+    results of resize, fork and compact say per row pages.OK, NO_PAGES or
+    INVALID, on the device.
     """
 
     def __init__(self, layout: KVLayout, k_ptrs: Sequence[int], v_ptrs: Sequence[int] | None,
@@ -148,6 +160,7 @@ class PagePool:
                                         _int32("lens", lens, self._index, n), n, status.data_ptr(), st)
         if ret:
             raise CacheError("kv_page_resize_launch", ret)
+        _used_on(stream, rows, lens)
         return status
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor, tokens: torch.Tensor | None = None,
@@ -161,6 +174,7 @@ class PagePool:
                                       _int32("tokens", tokens, self._index, n) if tokens is not None else None, n, st)
         if ret:
             raise CacheError("kv_page_copy_launch", ret)
+        _used_on(stream, src, dst, tokens)
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor,
              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
@@ -174,6 +188,7 @@ class PagePool:
                                       out.data_ptr(), st)
         if ret:
             raise CacheError("kv_page_fork_launch", ret)
+        _used_on(stream, parents, children)
         return out[:n]
 
     def compact(self, rows: torch.Tensor, start: torch.Tensor, keep: torch.Tensor, offsets: torch.Tensor,
@@ -190,6 +205,7 @@ class PagePool:
                                          out.data_ptr() + 4 * n, out.data_ptr(), st)
         if ret:
             raise CacheError("kv_page_compact_launch", ret)
+        _used_on(stream, rows, start, keep, offsets)
         return out[:n]
 
     def check(self) -> None:

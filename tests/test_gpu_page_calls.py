@@ -1,5 +1,6 @@
 """Calls of the page operators and of attention that their documentation allows
-beside the ordinary ones: with another call's error pending."""
+beside the ordinary ones: with another call's error pending, with arguments
+that are dropped while another stream still has to read them."""
 import numpy as np
 import pytest
 import torch
@@ -65,3 +66,52 @@ def test_a_device_that_is_not_there_leaves_no_error_behind():
     resize(c, [0], [20])
     fork(c, [0], [1])
     c.same()
+
+
+class Dropped:
+    """Calls on a side stream that is still busy; the arguments are dropped when
+    the call returns, and the current stream takes and fills what memory it can
+    get in their sizes."""
+
+    def __init__(self):
+        self.side = torch.cuda.Stream()
+
+    def __call__(self, call, *arguments):
+        given = [t.clone() for t in arguments]
+        others = [torch.full_like(t, 1) for t in given]
+        sizes = [(t.shape, t.dtype) for t in given]
+        self.side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(self.side):
+            torch.cuda._sleep(100_000_000)
+        result = call(*given, stream=self.side)
+        del given
+        taken = [torch.empty(shape, dtype=dt, device="cuda") for shape, dt in sizes for _ in range(2)]
+        for t, o in zip(taken[::2] + taken[1::2], others * 2):
+            t.copy_(o)
+        torch.cuda.synchronize()
+        return result
+
+
+def test_page_calls_whose_arguments_are_dropped():
+    c = Case(GEOMETRIES["mixed"], 60, 8, 6)
+    m, drop = c.model, Dropped()
+    assert drop(c.pool.resize, ints([0, 5, 3]), ints([41, 17, 30])).tolist() == m.resize([0, 5, 3], [41, 17, 30])
+    c.same()
+    assert drop(c.pool.fork, ints([0, 3]), ints([2, 6])).tolist() == m.fork([0, 3], [2, 6])
+    c.same()
+    got = drop(c.pool.compact, ints([5, 2]), ints([3, 40]), ints([5, 9, 16, 40]), ints([0, 3, 4]))
+    assert got.tolist() == m.compact([5, 2], [3, 40], [5, 9, 16, 40], [0, 3, 4])
+    c.same()
+    drop(c.pool.copy, ints([0, 2, 7]), ints([50, 51, 52]), ints([8, 3, 5]))
+    m.copy([0, 2, 7], [50, 51, 52], [8, 3, 5])
+    c.same()
+
+
+def test_attention_whose_arguments_are_dropped():
+    b = Batch([300, 40, 77], [3, 2, 5], seed=31).tree(31)
+    args, parents = b.args()
+    att = b.attention()
+    want = att(*args, parents=parents)
+    call = lambda *a, stream: att(0, *a[:4], parents=a[4], rows=a[5], stream=stream)
+    assert torch.equal(Dropped()(call, *args[1:], parents, ints([0, 1, 2])), want)
+    att.check()

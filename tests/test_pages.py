@@ -157,3 +157,17 @@ def test_copies_of_too_many_pages_are_refused():
     assert lib.kv_page_copy_launch(C.addressof(c), X, X, None, (1 << 31) + 5, None) == -errno.E2BIG
     c = cache(num_layers=1 << 30)
     assert lib.kv_page_copy_launch(C.addressof(c), X, X, None, 1, None) == -errno.EINVAL
+
+
+def test_what_a_call_on_a_stream_was_given_is_recorded_there():
+    class Tensor:
+        def __init__(self):
+            self.streams = []
+
+        def record_stream(self, stream):
+            self.streams.append(stream)
+
+    a, b = Tensor(), Tensor()
+    pg._used_on(None, a, b)
+    pg._used_on("side", a, None, b)
+    assert a.streams == b.streams == ["side"]
