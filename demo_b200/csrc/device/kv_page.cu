@@ -161,15 +161,15 @@ __device__ __forceinline__ uint32_t row_of(const int32_t *first, uint32_t n, int
  * page freed twice is neither pushed twice nor left negative.
  * ---------------------------------------------------------------------- */
 __global__ void __launch_bounds__(kPlanThreads, 1)
-kv_page_resize_kernel(const kv_page_state s, const int32_t *__restrict__ rows, const int32_t *__restrict__ lens,
-                      uint32_t n, int32_t *__restrict__ status)
+kv_page_resize_kernel(const kv_page_state s, const int32_t *rows, const int32_t *lens, uint32_t n, int32_t *__restrict__ status)
 {
     extern __shared__ int32_t sm[];
     int32_t *row = sm, *old_p = sm + n, *new_p = sm + 2 * n, *need = sm + 3 * n;
     int32_t *drops = sm + 4 * n, *takes = sm + 5 * n;       /* units of the rows before */
+    int32_t *length = sm + 6 * n;                           /* lens, which may be the state's own: read once */
     const uint32_t words = (s.num_rows + 31) / 32;
-    uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 6 * n), *twice = seen + words;
-    int32_t *gone = sm + 6 * n + 2 * words;                 /* pages pushed by the units before */
+    uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 7 * n), *twice = seen + words;
+    int32_t *gone = sm + 7 * n + 2 * words;                 /* pages pushed by the units before */
     __shared__ int32_t served, all_drop, all_take;
     const uint32_t rank = cluster_rank(), ctas = cluster_size();
     const uint32_t lane = threadIdx.x & 31, warp0 = rank * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = ctas * (blockDim.x >> 5);
@@ -205,6 +205,7 @@ kv_page_resize_kernel(const kv_page_state s, const int32_t *__restrict__ rows, c
             row[i] = -1;
             a = b = 0;
         }
+        length[i] = to;
         old_p[i] = a;
         new_p[i] = b;
         need[i] = b > a ? b - a : 0;
@@ -415,7 +416,7 @@ kv_page_resize_kernel(const kv_page_state s, const int32_t *__restrict__ rows, c
         if (want > 0 && fits)
             atomicMax(&served, need[i] + want);
         if (r >= 0 && fits)
-            s.lens[r] = lens[i];
+            s.lens[r] = length[i];
         if (status)
             status[i] = r < 0 ? KVPAGE_INVALID : fits ? KVPAGE_OK : KVPAGE_NO_PAGES;
     }
@@ -881,7 +882,7 @@ int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t cluster, 
     return 0;
 }
 
-constexpr size_t kPlanSmem = (6 * KVPAGE_MAX_CALL + kMaxUnits + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
+constexpr size_t kPlanSmem = (7 * KVPAGE_MAX_CALL + kMaxUnits + 3 * KVPAGE_MAX_ROWS / 32) * sizeof(int32_t);
 
 /* one cluster; the kernels' shared memory limit is raised once per device */
 template <typename... P, typename... A>
@@ -912,7 +913,7 @@ int resize_launch(const kv_page_state *s, const int32_t *rows, const int32_t *le
     static std::once_flag once[64];
     static cudaError_t err[64];
     const uint64_t units = n + (uint64_t)n * s->width / kUnit;
-    const size_t smem = (6 * (size_t)n + (units < kMaxUnits ? units : kMaxUnits) + 2 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
+    const size_t smem = (7 * (size_t)n + (units < kMaxUnits ? units : kMaxUnits) + 2 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
     return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_threads(s, n), smem, after, stream, *s, rows, lens, n, status);
 }
 

@@ -19,7 +19,8 @@
  *   free_count [1]
  * The state's calls are made on one stream, or ordered by the caller; they
  * allocate nothing, do not synchronise, and may be captured into a graph.
- * Their results do not depend on the order in which threads run.
+ * Their results do not depend on the order in which threads run.  What a call
+ * is given is read before the state is written: it may be part of the state.
  *
  * The launch functions return 0, -EINVAL for a malformed argument, -E2BIG
  * past a limit below, -EIO when the launch failed.  What only the device can

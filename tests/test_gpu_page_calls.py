@@ -1,6 +1,7 @@
 """Calls of the page operators and of attention that their documentation allows
 beside the ordinary ones: with another call's error pending, with arguments
-that are dropped while another stream still has to read them."""
+that are dropped while another stream still has to read them, or that are the
+state's own arrays."""
 import numpy as np
 import pytest
 import torch
@@ -115,3 +116,28 @@ def test_attention_whose_arguments_are_dropped():
     call = lambda *a, stream: att(0, *a[:4], parents=a[4], rows=a[5], stream=stream)
     assert torch.equal(Dropped()(call, *args[1:], parents, ints([0, 1, 2])), want)
     att.check()
+
+
+@pytest.mark.parametrize("n", [2, 700, 4096])
+def test_lengths_taken_from_the_state_itself(n):
+    """rows exchange their lengths: row n - 1 - i gets what row i had"""
+    c = Case(("nhd", 1, 1, 8, torch.int16, 4), 6 * n, n, 5)
+    rng = np.random.default_rng(n)
+    resize(c, list(range(n)), rng.integers(0, 21, n).tolist())
+    rows = list(range(n))[::-1]
+    assert c.pool.resize(ints(rows), c.pool.seq_lens).tolist() == c.model.resize(rows, c.model.lens.tolist())
+    c.same()
+
+
+def test_lists_taken_from_the_state_itself():
+    """children named by the table, a start that is the lengths"""
+    c = Case(GEOMETRIES["mixed"], 30, 4, 6)
+    resize(c, [0, 1], [8 * 3 + 1, 8])
+    table = c.pool.block_table                              # pages 0, 1, 2, 3 and 4
+    assert c.model.table[0, :4].tolist() == [0, 1, 2, 3]
+    assert c.pool.fork(table[0, :2], table[0, 2:4]).tolist() == c.model.fork([0, 1], [2, 3])
+    c.same()
+    lens = c.pool.seq_lens
+    got = c.pool.compact(ints([0, 1, 2, 3]), lens, ints([]), ints([0] * 5))     # nothing dropped, nothing kept behind
+    assert got.tolist() == c.model.compact([0, 1, 2, 3], c.model.lens.tolist(), [], [0] * 5)
+    c.same()
