@@ -28,7 +28,7 @@ constexpr int kPlanThreads = 1024;          /* at most; 256 for small calls, who
 constexpr uint32_t kPlanCluster = 8;
 constexpr uint32_t kUnit = 128;             /* table entries that a warp takes together, four to a lane */
 constexpr uint32_t kMaxUnits = 2 * KVPAGE_MAX_CALL;
-constexpr int32_t kRefused = INT32_MIN;     /* compact's length for resize of a row that it has refused and reported */
+constexpr int32_t kRefused = INT32_MIN;     /* in a resize of compact's: the length of a row that it has refused and reported */
 
 /* ---- the cluster's barrier and shared memory ---- */
 __device__ __forceinline__ uint32_t cluster_rank()
@@ -161,7 +161,8 @@ __device__ __forceinline__ uint32_t row_of(const int32_t *first, uint32_t n, int
  * page freed twice is neither pushed twice nor left negative.
  * ---------------------------------------------------------------------- */
 __global__ void __launch_bounds__(kPlanThreads, 1)
-kv_page_resize_kernel(const kv_page_state s, const int32_t *rows, const int32_t *lens, uint32_t n, int32_t *__restrict__ status)
+kv_page_resize_kernel(const kv_page_state s, const int32_t *rows, const int32_t *lens, uint32_t n, int32_t *__restrict__ status,
+                      bool compacted)
 {
     extern __shared__ int32_t sm[];
     int32_t *row = sm, *old_p = sm + n, *new_p = sm + 2 * n, *need = sm + 3 * n;
@@ -200,7 +201,7 @@ kv_page_resize_kernel(const kv_page_state s, const int32_t *rows, const int32_t 
             ok = !test_bit(twice, r) && from >= 0 && a <= s.width && b <= s.width;
         }
         if (!ok) {
-            if (rank == 0 && to != kRefused)
+            if (rank == 0 && !(compacted && to == kRefused))
                 atomicOr(s.error, KVPAGE_ERR_ROW);
             row[i] = -1;
             a = b = 0;
@@ -907,14 +908,16 @@ uint32_t plan_threads(const kv_page_state *s, uint32_t n)
     return units <= kPlanCluster * 8 ? 256 : kPlanThreads;
 }
 
+/* compacted: as the second kernel of compact */
 int resize_launch(const kv_page_state *s, const int32_t *rows, const int32_t *lens, uint32_t n, int32_t *status,
-                  bool after, cudaStream_t stream)
+                  bool compacted, cudaStream_t stream)
 {
     static std::once_flag once[64];
     static cudaError_t err[64];
     const uint64_t units = n + (uint64_t)n * s->width / kUnit;
     const size_t smem = (7 * (size_t)n + (units < kMaxUnits ? units : kMaxUnits) + 2 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
-    return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_threads(s, n), smem, after, stream, *s, rows, lens, n, status);
+    return launch_plan(kv_page_resize_kernel, once, err, s->device, plan_threads(s, n), smem, compacted, stream, *s, rows, lens, n, status,
+                       compacted);
 }
 
 int call_ok(const kv_page_state *s, uint32_t n)

@@ -1,13 +1,14 @@
 """Calls of the page operators and of attention that their documentation allows
 beside the ordinary ones: with another call's error pending, with arguments
-that are dropped while another stream still has to read them, or that are the
-state's own arrays."""
+that are dropped while another stream still has to read them, that are the state's
+own arrays, or that only the device can refuse."""
 import numpy as np
 import pytest
 import torch
 
 from demo_b200 import pages as pg
 from demo_b200._lib import lib
+from oracle import pages_model as pm
 from tests.test_gpu_attention import Batch, close
 from tests.test_gpu_pages import GEOMETRIES, Case, compact, fork, ints, resize
 
@@ -141,3 +142,12 @@ def test_lists_taken_from_the_state_itself():
     got = c.pool.compact(ints([0, 1, 2, 3]), lens, ints([]), ints([0] * 5))     # nothing dropped, nothing kept behind
     assert got.tolist() == c.model.compact([0, 1, 2, 3], c.model.lens.tolist(), [], [0] * 5)
     c.same()
+
+
+def test_every_refused_length_sets_a_bit():
+    for length in (-1, -2 ** 31, 6 * 8 + 1, 2 ** 31 - 1):
+        c = Case(GEOMETRIES["mixed"], 40, 6, 6)
+        resize(c, [0, 1], [20, length])
+        c.same(pm.ERR_ROW)
+        with pytest.raises(ValueError, match="length"):
+            c.pool.check()
