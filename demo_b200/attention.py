@@ -22,6 +22,8 @@ from .pages import _current_stream, _int32, _on_stream, _used_on
 # struct kv_attn_desc in one go: 12 pointers, 8 64-bit numbers, 12 32-bit ones, three floats, the device
 _DESC = struct.Struct("@12PQQqqqqq10I2i3fi")
 _TYPES = {torch.bfloat16: _lib.KVATTN_BF16, torch.float16: _lib.KVATTN_FP16}
+_KV_TYPES = {**_TYPES, torch.float8_e4m3fn: _lib.KVATTN_E4M3}
+_BYTES = (torch.uint8, torch.int8, torch.int16, torch.uint16)      # tensors that say nothing about their values
 
 _ERRORS = ((_lib.KVATTN_ERR_PAGE, "a page id outside the cache"),
            (_lib.KVATTN_ERR_SEQ, "offsets out of order, or a row or length that fits neither table nor nodes"),
@@ -33,14 +35,17 @@ class TreeAttention:
     """Attention of fed tokens over the layers of one paged cache.
 
     layout, k_ptrs, v_ptrs: from cache.layout_from_kv_tensors; K and V planes
-        of 16-bit values of the queries' type, or of float8_e4m3fn values
-        (1-byte elements) that k_scale and v_scale bring back
+        of 16-bit values of the queries' type, or of float8_e4m3fn values that
+        k_scale and v_scale bring back
+    kv_dtype: the values' type where the layout's tensors do not say it (8-bit
+        caches that an engine keeps as uint8).  A layout made by hand, without
+        a dtype, stands for float8_e4m3fn or the queries' type, by its element size
     num_heads, num_kv_heads: query heads and K/V heads of this rank
     scale: of the scores, by default head_dim ** -0.5
     """
 
     def __init__(self, layout: KVLayout, k_ptrs: Sequence[int], v_ptrs: Sequence[int], num_heads: int, num_kv_heads: int,
-                 scale: float | None = None, k_scale: float = 1.0, v_scale: float = 1.0):
+                 scale: float | None = None, k_scale: float = 1.0, v_scale: float = 1.0, kv_dtype: torch.dtype | None = None):
         if layout.kv != 2 or v_ptrs is None:
             raise ValueError("attention needs K and V planes (a K-only latent cache is not supported)")
         if len(k_ptrs) != layout.num_layers or len(v_ptrs) != layout.num_layers:
@@ -49,6 +54,16 @@ class TreeAttention:
             raise ValueError("num_kv_heads must divide num_heads and the layout's width")
         if layout.element_size not in (1, 2):
             raise ValueError("caches of 1 or 2-byte elements")
+        held = layout.dtype
+        if kv_dtype is not None:
+            if held is not None and held is not kv_dtype and held not in _BYTES:
+                raise ValueError(f"kv_dtype: the cache holds {held}, not {kv_dtype}")
+            held = kv_dtype
+        elif held is None and layout.element_size == 1:
+            held = torch.float8_e4m3fn
+        if held is not None and (held not in _KV_TYPES or held.itemsize != layout.element_size):
+            raise ValueError(f"caches of bfloat16, float16 or float8_e4m3fn values, not {held}"
+                             + (" (kv_dtype says what bytes stand for)" if held in _BYTES else ""))
         if num_heads // num_kv_heads > 128:
             raise ValueError("at most 128 query heads per K/V head")
         dim = layout.hidden_dim_size // num_kv_heads
@@ -66,6 +81,7 @@ class TreeAttention:
         self._devices: dict[int, tuple[torch.Tensor, int, int]] = {}     # error bits, their address, workspace bytes
         self._shape = (layout.num_blocks, layout.block_size, num_heads, num_kv_heads, dim, 1 if layout.head_bytes else 0)
         self._scales = (scale, float(k_scale), float(v_scale))
+        self.kv_dtype = held                # None: the queries'
         if torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing():
             self._device(torch.cuda.current_device())
 
@@ -107,6 +123,9 @@ class TreeAttention:
         if index < 0 or kind is None or q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or \
                 q.stride(2) != 1:
             raise ValueError(f"q: expected a bfloat16 or float16 CUDA tensor [total, {self.num_heads}, {self.head_dim}]")
+        kv_type = kind if self.kv_dtype is None else _KV_TYPES[self.kv_dtype]
+        if kv_type != kind and kv_type != _lib.KVATTN_E4M3:
+            raise ValueError(f"q: {q.dtype} queries over a cache of {self.kv_dtype}")
         if stream is not None:
             caller = torch.cuda.current_stream(index)
             with _on_stream(stream, index):
@@ -148,7 +167,7 @@ class TreeAttention:
             q_strides[0] if total > 1 else row, q_strides[1] if heads > 1 else row,
             out_strides[0] if total > 1 else row, out_strides[1] if heads > 1 else row,
             width, n_rows, seqs, total, pages, block, heads, kv_heads, dim, head_major, kind,
-            _lib.KVATTN_E4M3 if self.layout.element_size == 1 else kind, *self._scales, index)
+            kv_type, *self._scales, index)
         ret = lib.kv_attn_launch(desc, _current_stream(index))
         if ret:
             raise CacheError("kv_attn_launch", ret)

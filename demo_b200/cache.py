@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import errno
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Sequence
 
 import numpy as np
@@ -63,6 +63,9 @@ class KVLayout:
     # 0 / 0 = dense token-major, the reference's FlashAttention layout
     block_stride: int = 0    # bytes from one block of a plane to the next
     head_bytes: int = 0      # > 0: head-major blocks [heads][block_size][head_bytes]
+    # the torch.dtype of the tensors that the layout was taken from; transfers
+    # move bytes and do not look at it, attention does.  None: not known
+    dtype: object = field(default=None, compare=False)
 
     @property
     def unit(self) -> int:
@@ -356,7 +359,7 @@ def layout_from_kv_tensors(kv_caches, kv_layout: str | None = None
         raise ValueError(f"unsupported KV tensor shape {tuple(t0.shape)}")
     lay = KVLayout(num_layers=len(layers), num_blocks=int(nb), block_size=int(bs),
                    hidden_dim_size=int(hidden), element_size=esz, kv=kv,
-                   block_stride=int(block_stride), head_bytes=int(head_bytes))
+                   block_stride=int(block_stride), head_bytes=int(head_bytes), dtype=t0.dtype)
     return lay, k, v
 
 

@@ -157,3 +157,60 @@ def test_a_stream_of_another_device_is_refused():
 
     with pytest.raises(ValueError, match="cuda:0"):
         _on_stream(SimpleNamespace(device_index=1), 0)
+
+
+def typed(dtype, **k):
+    return layout(dtype=dtype, element_size=dtype.itemsize, **k)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.float8_e5m2, torch.int16, torch.float8_e4m3fnuz], ids=str)
+def test_caches_of_other_types_are_refused(dtype):
+    with pytest.raises(ValueError, match="values, not"):
+        TreeAttention(typed(dtype), [X], [X], 8, 2)
+
+
+@pytest.mark.parametrize("held, said", [(torch.bfloat16, torch.float16), (torch.float8_e5m2, torch.float8_e4m3fn), (torch.float16, torch.float8_e4m3fn),
+                                        (torch.uint8, torch.float8_e5m2), (torch.uint8, torch.bfloat16), (torch.int16, torch.float8_e4m3fn),
+                                        (torch.int16, torch.float32)], ids=str)
+def test_a_type_that_the_cache_does_not_hold_is_refused(held, said):
+    with pytest.raises(ValueError, match="kv_dtype|values, not"):
+        TreeAttention(typed(held), [X], [X], 8, 2, kv_dtype=said)
+
+
+def test_what_a_cache_holds():
+    make = lambda lay, said=None: TreeAttention(lay, [X], [X], 8, 2, kv_dtype=said).kv_dtype
+    for t in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+        assert make(typed(t)) is make(typed(t), t) is make(layout(element_size=t.itemsize), t) is t
+    assert make(typed(torch.uint8), torch.float8_e4m3fn) is torch.float8_e4m3fn
+    assert make(typed(torch.int16), torch.bfloat16) is torch.bfloat16
+    assert make(layout()) is None and make(layout(element_size=1)) is torch.float8_e4m3fn
+
+
+class OnGpu:
+    """stands for a CUDA tensor in the checks that come before anything is launched"""
+
+    def __init__(self, shape, dtype, index=0):
+        self.t, self.index = torch.zeros(shape, dtype=dtype), index
+
+    def get_device(self):
+        return self.index
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+@pytest.mark.parametrize("held, queries", [(torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)], ids=str)
+def test_queries_of_another_type_than_the_cache_are_refused(held, queries):
+    att = TreeAttention(typed(held), [X], [X], 8, 2)
+    i32 = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="over a cache of"):
+        att(0, OnGpu((4, 8, 128), queries), i32.view(2, 2), i32, i32)
+
+
+def test_layouts_know_what_their_tensors_hold():
+    from demo_b200.cache import layout_from_kv_tensors
+
+    for dtype in (torch.bfloat16, torch.float16, torch.uint8):
+        lay, _, _ = layout_from_kv_tensors([torch.zeros(2, 4, 16, 2, 64, dtype=dtype)])
+        assert lay.dtype is dtype
+        assert lay == KVLayout(1, 4, 16, 128, dtype.itemsize, 2)       # two layouts are the same when their bytes are
