@@ -28,6 +28,7 @@ KVPAGE_ERR_REFS = 0x4
 KVPAGE_ERR_KEEP = 0x8
 KVPAGE_ERR_ALIGN = 0x10
 KVPAGE_OK, KVPAGE_NO_PAGES, KVPAGE_INVALID = 0, 1, 2
+KVPAGE_ANY_DEVICE = -1
 KVPAGE_MAX_CALL = 4096
 KVPAGE_MAX_ROWS = 65536
 KVATTN_ERR_PAGE = 0x1
@@ -288,6 +289,7 @@ SIGNATURES: dict[str, tuple] = {
                                   C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32,
                                   C.c_uint32, C.c_void_p]),
     # include/kvpage.h (structs and arrays by address: the callers keep them)
+    "kv_page_device_of": (C.c_int, [C.c_void_p]),
     "kv_page_resize_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]),
     "kv_page_copy_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
     "kv_page_fork_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,

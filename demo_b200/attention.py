@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import KvAttnDesc, lib
 from .cache import CacheError, KVLayout
-from .pages import _current_stream, _int32, _on_stream, _used_on
+from .pages import _current_stream, _int32, _on_stream, _used_on, planes_on
 
 # struct kv_attn_desc in one go: 12 pointers, 8 64-bit numbers, 12 32-bit ones, three floats, the device
 _DESC = struct.Struct("@12PQQqqqqq10I2i3fi")
@@ -83,9 +83,12 @@ class TreeAttention:
         self._scales = (scale, float(k_scale), float(v_scale))
         self.kv_dtype = held                # None: the queries'
         if torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing():
-            self._device(torch.cuda.current_device())
+            at = lib.kv_page_device_of(self._k[0])      # else its first call will say what is wrong with it
+            if at >= 0 or at == _lib.KVPAGE_ANY_DEVICE:
+                self._device(at if at >= 0 else torch.cuda.current_device())
 
     def _device(self, index: int) -> tuple[torch.Tensor, int, int]:
+        planes_on(index, (*self._k, *self._v))
         d = KvAttnDesc(table_stride=1, width=1, num_rows=1, device=index, scale=self._scales[0], k_scale=self._scales[1])
         d.num_pages, d.block_size, d.num_heads, d.num_kv_heads, d.head_dim, d.head_major = self._shape
         need = lib.kv_attn_workspace_bytes(C.addressof(d))
@@ -116,8 +119,9 @@ class TreeAttention:
         the results then belong.  The arguments may be dropped when the call
         returns; the object must outlive its calls, and the graphs that captured
         them.  Queries that no sequence covers leave their rows of out and lse as
-        they were, which in new tensors is anything.  May be captured, except for the first call on
-        a device that was not the current one when the object was made.
+        they were, which in new tensors is anything.  May be
+        captured, except for the first call of an object that was made before
+        CUDA was used.
         """
         index, kind = q.get_device(), _TYPES.get(q.dtype)
         if index < 0 or kind is None or q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or \

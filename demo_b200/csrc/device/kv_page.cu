@@ -1001,6 +1001,16 @@ int compact_vec(const Planes &p, const kv_page_state *s, const int32_t *rows, co
 
 }  // namespace
 
+extern "C" int kv_page_device_of(const void *ptr)
+{
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, ptr) != cudaSuccess) {
+        cudaGetLastError();
+        return -EINVAL;
+    }
+    return at.type == cudaMemoryTypeDevice ? at.device : at.type == cudaMemoryTypeUnregistered ? -EINVAL : KVPAGE_ANY_DEVICE;
+}
+
 extern "C" int kv_page_resize_launch(const struct kv_page_state *s, const int32_t *rows, const int32_t *lens, uint32_t n,
                                      int32_t *status, void *stream)
 {

@@ -80,6 +80,16 @@ def plane_bases(layout: KVLayout, k_ptrs: Sequence[int], v_ptrs: Sequence[int] |
     return both[:layout.num_layers], both[layout.num_layers:] if v_ptrs is not None else None, every & -every
 
 
+def planes_on(index: int, ptrs: Sequence[int]) -> None:
+    """ValueError unless kernels on CUDA device `index` may follow every base"""
+    for p in ptrs:
+        at = lib.kv_page_device_of(p)
+        if at < 0 and at != _lib.KVPAGE_ANY_DEVICE:
+            raise ValueError("a layer base is not memory that a GPU reaches")
+        if at not in (index, _lib.KVPAGE_ANY_DEVICE):
+            raise ValueError(f"the cache is on cuda:{at}, not on cuda:{index}")
+
+
 class PagePool:
     """The pages of one paged cache and the rows that hold them.
 
@@ -125,6 +135,7 @@ class PagePool:
         zeros = torch.zeros(1 + n, dtype=torch.int32, device=dev)
         self.error, self._marks = zeros[:1], zeros[1:]
         self._k, self._v, align = plane_bases(layout, k_ptrs, v_ptrs, dev)
+        planes_on(dev.index, (*k_ptrs, *(v_ptrs or ())))
         self._index = index = dev.index
         self._state = KvPageState(
             table=block_table.data_ptr(), lens=_int32("seq_lens", seq_lens, index, rows),

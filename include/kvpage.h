@@ -49,6 +49,8 @@ extern "C" {
 #define KVPAGE_NO_PAGES   1     /* not enough free pages: the row is as it was */
 #define KVPAGE_INVALID    2     /* an error bit says why: the row is as it was */
 
+#define KVPAGE_ANY_DEVICE -1
+
 #define KVPAGE_MAX_CALL   4096  /* rows of one resize / fork / compact call */
 #define KVPAGE_MAX_ROWS   65536 /* rows of a table */
 
@@ -82,6 +84,10 @@ struct kv_page_cache {
     uint32_t base_align;     /* a power of two that divides every plane base; 0 = 16 */
     int32_t device;
 };
+
+/* The device whose memory ptr points to, KVPAGE_ANY_DEVICE for memory that all
+ * devices reach (pinned or managed), -EINVAL for any other. */
+int kv_page_device_of(const void *ptr);
 
 /* Set row rows[i] to lens[i] tokens, i < n: pages are given back where that
  * takes fewer, and taken where it takes more (what they hold is not touched).

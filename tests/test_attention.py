@@ -214,3 +214,14 @@ def test_layouts_know_what_their_tensors_hold():
         lay, _, _ = layout_from_kv_tensors([torch.zeros(2, 4, 16, 2, 64, dtype=dtype)])
         assert lay.dtype is dtype
         assert lay == KVLayout(1, 4, 16, 128, dtype.itemsize, 2)       # two layouts are the same when their bytes are
+
+
+@pytest.mark.parametrize("at, match", [(1, "cuda:1, not on cuda:0"), (-errno.EINVAL, "not memory that a GPU reaches")])
+def test_queries_on_another_device_than_the_cache_are_refused(monkeypatch, at, match):
+    monkeypatch.setattr(lib, "kv_page_device_of", lambda p: at)
+    att = TreeAttention(typed(torch.bfloat16), [X], [X], 8, 2)
+    i32 = torch.zeros(4, dtype=torch.int32)
+    n0 = lib.crosscache_kernel_launches()
+    with pytest.raises(ValueError, match=match):
+        att(0, OnGpu((4, 8, 128), torch.bfloat16), OnGpu((2, 2), torch.int32), i32, i32[:3])
+    assert lib.crosscache_kernel_launches() == n0

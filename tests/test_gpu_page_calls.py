@@ -6,8 +6,10 @@ import numpy as np
 import pytest
 import torch
 
+from demo_b200 import cache as cc
 from demo_b200 import pages as pg
-from demo_b200._lib import lib
+from demo_b200._lib import KVPAGE_ANY_DEVICE, lib
+from demo_b200.attention import TreeAttention
 from oracle import pages_model as pm
 from tests.test_gpu_attention import Batch, close
 from tests.test_gpu_pages import GEOMETRIES, Case, compact, fork, ints, resize
@@ -151,3 +153,37 @@ def test_every_refused_length_sets_a_bit():
         c.same(pm.ERR_ROW)
         with pytest.raises(ValueError, match="length"):
             c.pool.check()
+
+
+def test_planes_that_no_kernel_may_follow_are_refused():
+    pageable = torch.zeros(2, 4, 16, 2, 64, dtype=torch.bfloat16)
+    pinned, device = pageable.pin_memory(), pageable.cuda()
+    assert [lib.kv_page_device_of(t.data_ptr()) for t in (pageable, pinned, device)] == [-22, KVPAGE_ANY_DEVICE, 0]
+    layout, k, v = cc.layout_from_kv_tensors([pageable], kv_layout="flash_attn")
+    table = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="not memory that a GPU reaches"):
+        pg.PagePool(layout, k, v, table, ints([0]))
+    att = TreeAttention(layout, k, v, 4, 2)
+    with pytest.raises(ValueError, match="not memory that a GPU reaches"):
+        att(0, torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda"), table, ints([1]), ints([0, 1]))
+
+
+def test_a_cache_in_pinned_memory():
+    t = torch.randint(-9, 9, (2, 6, 4, 1, 8), dtype=torch.int16).pin_memory()
+    layout, k, v = cc.layout_from_kv_tensors([t], kv_layout="flash_attn")
+    pool = pg.PagePool(layout, k, v, ints([-1] * 4).view(1, 4), ints([0]))
+    want = t.clone()
+    want[:, 5] = want[:, 2]
+    pool.copy(ints([2]), ints([5]))
+    pool.check()
+    assert torch.equal(t, want)
+
+
+def test_a_cache_of_bytes_whose_type_is_said():
+    b = Batch([90, 40], [3, 1], seed=32, kvt=torch.float8_e4m3fn)
+    args, _ = b.args()
+    want = b.attention()(*args)
+    layout, k, v = cc.layout_from_kv_tensors([t.view(torch.uint8) for t in b.store], kv_layout="flash_attn")
+    assert (k, v) == (b.k, b.v)
+    att = TreeAttention(layout, k, v, b.heads, b.kv_heads, k_scale=b.scales[0], v_scale=b.scales[1], kv_dtype=torch.float8_e4m3fn)
+    assert torch.equal(att(*args), want)

@@ -171,3 +171,14 @@ def test_what_a_call_on_a_stream_was_given_is_recorded_there():
     pg._used_on(None, a, b)
     pg._used_on("side", a, None, b)
     assert a.streams == b.streams == ["side"]
+
+
+def test_planes_of_another_device_are_refused(monkeypatch):
+    at = {X: 0, 2 * X: 1, 3 * X: -1, 4 * X: -errno.EINVAL}
+    monkeypatch.setattr(lib, "kv_page_device_of", at.get)
+    pg.planes_on(0, [X, 3 * X])             # its own memory, and pinned memory
+    pg.planes_on(1, [2 * X])
+    with pytest.raises(ValueError, match="cuda:1, not on cuda:0"):
+        pg.planes_on(0, [X, 2 * X])
+    with pytest.raises(ValueError, match="not memory that a GPU reaches"):
+        pg.planes_on(0, [X, 4 * X])
