@@ -13,6 +13,7 @@ import struct
 from typing import Sequence
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._lib import KvAttnDesc, lib
@@ -123,6 +124,10 @@ class TreeAttention:
         captured, except for the first call of an object that was made before
         CUDA was used.
         """
+        if (q.requires_grad and torch.is_grad_enabled()) or unpack_dual(q).tangent is not None:
+            raise ValueError("q: attention over a cache has no gradients; call it under torch.no_grad(), without a tangent")
+        if torch.jit.is_tracing():
+            raise ValueError("attention over a cache cannot be traced: it would become a constant")
         index, kind = q.get_device(), _TYPES.get(q.dtype)
         if index < 0 or kind is None or q.dim() != 3 or q.shape[1] != self.num_heads or q.shape[2] != self.head_dim or \
                 q.stride(2) != 1:
@@ -138,8 +143,6 @@ class TreeAttention:
                 t.record_stream(caller)     # which may be where it is used and dropped
             _used_on(stream, q, block_table, seq_lens, q_offsets, parents, rows, out)
             return res
-        if q.requires_grad and torch.is_grad_enabled():
-            raise ValueError("q: attention over a cache has no gradients; call it under torch.no_grad()")
         total = q.shape[0]
         q_strides = q.stride()
         if 0 in q_strides:                              # an expanded tensor

@@ -225,3 +225,29 @@ def test_queries_on_another_device_than_the_cache_are_refused(monkeypatch, at, m
     with pytest.raises(ValueError, match=match):
         att(0, OnGpu((4, 8, 128), torch.bfloat16), OnGpu((2, 2), torch.int32), i32, i32[:3])
     assert lib.crosscache_kernel_launches() == n0
+
+
+def test_gradients_of_every_kind_and_traces_are_refused():
+    """before anything is looked at, so that the refusal shows without a GPU"""
+    from torch.autograd import forward_ad
+
+    att = TreeAttention(layout(), [X], [X], 8, 2)
+    i32 = torch.zeros(4, dtype=torch.int32)
+    q = torch.zeros(4, 8, 128, dtype=torch.bfloat16)
+    call = lambda x: att(0, x, torch.zeros(4, 2, dtype=torch.int32), i32, torch.zeros(5, dtype=torch.int32))
+    with pytest.raises(ValueError, match="no gradients"):
+        call(q.clone().requires_grad_())
+    for guard in (torch.enable_grad(), torch.no_grad()):
+        with guard, forward_ad.dual_level():
+            with pytest.raises(ValueError, match="no gradients"):
+                call(forward_ad.make_dual(q, torch.ones_like(q)))
+            with pytest.raises(ValueError, match="q: expected"):
+                call(q)                             # a tensor without a tangent is no reason
+    with pytest.raises(ValueError, match="no gradients"):
+        torch.func.jvp(call, (q,), (torch.ones_like(q),))
+    with pytest.raises(ValueError, match="no gradients"):
+        torch.func.grad(lambda x: call(x).sum())(q.float())
+    with pytest.raises(Exception, match="cannot be traced"):
+        torch.jit.trace(call, (q,))
+    with torch.no_grad(), pytest.raises(ValueError, match="q: expected"):
+        call(q.clone().requires_grad_())
