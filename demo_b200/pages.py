@@ -125,7 +125,8 @@ class PagePool:
         if (refs is None) != (free_list is None) or (refs is None) != (free_count is None):
             raise ValueError("refs, free_list and free_count: all three or none")
         n = layout.num_blocks
-        if refs is None:
+        fresh = refs is None
+        if fresh:
             refs = torch.zeros(n, dtype=torch.int32, device=dev)
             free_list = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=dev)
             free_count = torch.full((1,), n, dtype=torch.int32, device=dev)
@@ -137,8 +138,11 @@ class PagePool:
         self._k, self._v, align = plane_bases(layout, k_ptrs, v_ptrs, dev)
         planes_on(dev.index, (*k_ptrs, *(v_ptrs or ())))
         self._index = index = dev.index
+        lens = _int32("seq_lens", seq_lens, index, rows)
+        if fresh and bool(seq_lens.any()):      # their pages would be handed out again
+            raise ValueError("seq_lens: a pool that starts with every page free needs empty rows")
         self._state = KvPageState(
-            table=block_table.data_ptr(), lens=_int32("seq_lens", seq_lens, index, rows),
+            table=block_table.data_ptr(), lens=lens,
             refs=_int32("refs", refs, index, n), free_list=_int32("free_list", free_list, index, n),
             free_count=_int32("free_count", free_count, index, 1), marks=self._marks.data_ptr(),
             error=self.error.data_ptr(), table_stride=block_table.stride(0) if rows > 1 else width, width=width,

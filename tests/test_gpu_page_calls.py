@@ -187,3 +187,18 @@ def test_a_cache_of_bytes_whose_type_is_said():
     assert (k, v) == (b.k, b.v)
     att = TreeAttention(layout, k, v, b.heads, b.kv_heads, k_scale=b.scales[0], v_scale=b.scales[1], kv_dtype=torch.float8_e4m3fn)
     assert torch.equal(att(*args), want)
+
+
+def test_a_pool_of_free_pages_refuses_rows_that_hold_some():
+    store = torch.zeros(2, 8, 4, 1, 8, dtype=torch.int16, device="cuda")
+    layout, k, v = cc.layout_from_kv_tensors([store], kv_layout="flash_attn")
+    table = torch.full((3, 2), -1, dtype=torch.int32, device="cuda")
+    for lens in ([0, 5, 0], [0, 0, -1]):
+        with pytest.raises(ValueError, match="needs empty rows"):
+            pg.PagePool(layout, k, v, table, ints(lens))
+    table[1] = ints([3, 4])
+    pool = pg.PagePool(layout, k, v, table, ints([0, 5, 0]), refs=ints([0, 0, 0, 1, 1, 0, 0, 0]), free_list=ints([7, 6, 5, 2, 1, 0, 0, 0]),
+                       free_count=ints([6]))            # with the state that they belong to they are taken
+    assert pool.resize(ints([1]), ints([0])).tolist() == [pg.OK]
+    pool.check()
+    assert pool.free_list.tolist() == [7, 6, 5, 2, 1, 0, 3, 4]
