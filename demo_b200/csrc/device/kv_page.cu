@@ -45,9 +45,13 @@ __device__ __forceinline__ uint32_t cluster_size()
     return r;
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 __device__ __forceinline__ void cluster_sync()
 {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 
 /* store v at `p`'s place in the shared memory of CTA `rank` of the cluster */
@@ -429,7 +433,9 @@ kv_page_resize_kernel(const kv_page_state s, const int32_t *rows, const int32_t 
 /* ------------------------------------------------------------------------
  * fork's plan: what each child gets, the tables and the references; the pages
  * to copy go to pairs[3 * i] = (source, destination, tokens), 0 tokens where
- * there is nothing to copy.  One cluster, a warp per child.
+ * there is nothing to copy.  One cluster, a warp per child.  The parents' pages
+ * are looked through before any are dealt out, so that a child that would share
+ * a bad one takes none; the warp that finds it tells every CTA.
  * ---------------------------------------------------------------------- */
 __global__ void __launch_bounds__(kPlanThreads, 1)
 kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, const int32_t *__restrict__ children,
@@ -438,12 +444,16 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
     extern __shared__ int32_t sm[];
     int32_t *from = sm, *child = sm + n, *length = sm + 2 * n, *need = sm + 3 * n;
     const uint32_t words = (s.num_rows + 31) / 32;
-    uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 4 * n), *twice = seen + words, *parent = seen + 2 * words;
+    int32_t *bad_parent = sm + 4 * n;
+    uint32_t *seen = reinterpret_cast<uint32_t *>(sm + 5 * n), *twice = seen + words, *parent = seen + 2 * words;
     __shared__ int32_t served;
     const uint32_t rank = cluster_rank(), ctas = cluster_size();
     const uint32_t lane = threadIdx.x & 31, warp0 = rank * (blockDim.x >> 5) + (threadIdx.x >> 5), warps = ctas * (blockDim.x >> 5);
 
     start_second();
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
+        bad_parent[i] = 0;
+    cluster_arrive();
     for (uint32_t i = threadIdx.x; i < 3 * words; i += blockDim.x)
         seen[i] = 0;
     if (threadIdx.x == 0)
@@ -475,57 +485,89 @@ kv_page_fork_kernel(const kv_page_state s, const int32_t *__restrict__ parents, 
             len = 0;
         }
         length[i] = len;
-        need[i] = len % (int32_t)s.block_size != 0;
     }
     const int32_t have = free_pages(s);
+    __syncthreads();
+    cluster_wait();                 /* every CTA's bad_parent is zero */
+    int32_t kept[4] = {};           /* the first pages of the warp's first child */
+    for (uint32_t i = warp0; i < n; i += warps) {
+        if (child[i] < 0)
+            continue;
+        const int32_t *tp = s.table + (int64_t)from[i] * s.table_stride;
+        const int32_t held = (int32_t)pages_of(length[i], s.block_size);
+        bool bad = false;
+#pragma unroll 1
+        for (int32_t k = lane; k - (int32_t)lane < held; k += kUnit) {
+            int32_t page[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                page[j] = k + 32 * j < held ? tp[k + 32 * j] : 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                bad |= (uint32_t)page[j] >= s.num_pages;
+                if (i == warp0 && k == (int32_t)lane)
+                    kept[j] = page[j];
+            }
+        }
+        if (__any_sync(~0u, bad) && lane < ctas)
+            store_cluster(&bad_parent[i], lane, 1);
+    }
+    cluster_sync();                 /* every CTA has read the lengths and the count, and looked through its pages */
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        if (bad_parent[i]) {
+            if (rank == 0)
+                atomicOr(s.error, KVPAGE_ERR_PAGE);
+            child[i] = -1;
+            length[i] = 0;
+        }
+        need[i] = length[i] % (int32_t)s.block_size != 0;
+    }
     int32_t wanted;
     int32_t *arrays[1] = {need};
     block_scan<1>(arrays, n, &wanted);
-    cluster_sync();                 /* every CTA has read the lengths and the count */
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
         if (length[i] % (int32_t)s.block_size && need[i] < have)
             atomicMax(&served, need[i] + 1);
     for (uint32_t i = warp0; i < n; i += warps) {
         const int32_t c = child[i], len = length[i];
         const int32_t full = len / (int32_t)s.block_size, tail = len % (int32_t)s.block_size;
-        const bool fits = c >= 0 && (!tail || need[i] < have);
-        int32_t src = -1, dst = -1;
+        const int32_t *tp = s.table + (int64_t)(c >= 0 ? from[i] : 0) * s.table_stride;
+        bool fits = c >= 0 && (!tail || need[i] < have);
+        const int32_t src = fits && tail ? tp[full] : 0, dst = fits && tail ? s.free_list[have - 1 - need[i]] : 0;
+        const bool lost = (uint32_t)dst >= s.num_pages;     /* not a page: nobody's from now on */
+        fits = fits && !lost;
         if (fits) {
-            const int32_t *tp = s.table + (int64_t)from[i] * s.table_stride;
             int32_t *tc = s.table + (int64_t)c * s.table_stride;
 #pragma unroll 1
             for (int32_t k = lane; k < full; k += kUnit) {
                 int32_t page[4];
+                const bool held = i == warp0 && k == (int32_t)lane;
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    page[j] = k + 32 * j < full ? tp[k + 32 * j] : 0;
+                    page[j] = held ? kept[j] : k + 32 * j < full ? tp[k + 32 * j] : 0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if (k + 32 * j >= full)
                         break;
                     tc[k + 32 * j] = page[j];
-                    if (page[j] >= 0 && (uint32_t)page[j] < s.num_pages)
-                        atomicAdd(&s.refs[page[j]], 1);
-                    else
-                        atomicOr(s.error, KVPAGE_ERR_PAGE);
+                    atomicAdd(&s.refs[page[j]], 1);
                 }
             }
             if (tail && lane == 0) {
-                src = tp[full];
-                dst = s.free_list[have - 1 - need[i]];
                 tc[full] = dst;
-                if (dst >= 0 && (uint32_t)dst < s.num_pages)
-                    s.refs[dst] = 1;        /* a bad id of either: the copy sets the error bit */
+                s.refs[dst] = 1;
             }
         }
         if (lane == 0) {
-            pairs[3 * i] = fits && tail ? src : 0;
-            pairs[3 * i + 1] = fits && tail ? dst : 0;
+            if (lost)
+                atomicOr(s.error, KVPAGE_ERR_PAGE);
+            pairs[3 * i] = src;
+            pairs[3 * i + 1] = dst;
             pairs[3 * i + 2] = fits ? tail : 0;
             if (fits)
                 s.lens[c] = len;
             if (status)
-                status[i] = fits ? KVPAGE_OK : c < 0 ? KVPAGE_INVALID : KVPAGE_NO_PAGES;
+                status[i] = fits ? KVPAGE_OK : c < 0 || lost ? KVPAGE_INVALID : KVPAGE_NO_PAGES;
         }
     }
     __syncthreads();
@@ -1061,7 +1103,7 @@ extern "C" int kv_page_fork_launch(const struct kv_page_cache *c, const struct k
         return -EIO;
     static std::once_flag once[64];
     static cudaError_t err[64];
-    const size_t smem = (4 * (size_t)n + 3 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
+    const size_t smem = (5 * (size_t)n + 3 * ((s->num_rows + 31) / 32)) * sizeof(int32_t);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ret = launch_plan(kv_page_fork_kernel, once, err, s->device, plan_threads(s, n), smem, false, st, *s, parents,
                                 children, n, pairs, status);

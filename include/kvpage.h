@@ -91,6 +91,8 @@ int kv_page_device_of(const void *ptr);
 
 /* Set row rows[i] to lens[i] tokens, i < n: pages are given back where that
  * takes fewer, and taken where it takes more (what they hold is not touched).
+ * An id in the free list that is no page goes to the row whose turn it is as it
+ * stands, with KVPAGE_ERR_PAGE set, and is nobody's again once it is given back.
  * First all rows that shrink give back their entries.  A page whose last
  * reference goes is pushed; where several rows drop it, its place in the
  * order is that of the last.  Then the rows that grow take pages, in the order
@@ -112,7 +114,9 @@ int kv_page_copy_launch(const struct kv_page_cache *cache, const int32_t *src, c
  * it shares the parent's full pages and gets a copy of the tokens of a partly
  * filled last page, in a page of its own, so that both can be appended to.
  * Pages are taken in the order of the call as in resize.  A row may be the
- * parent of many.  pairs: scratch of 3 * n int32. */
+ * parent of many.  A child whose parent holds an id that is no page, or whose
+ * turn it is for one of the free list, stays empty (KVPAGE_INVALID; the latter
+ * id is off the list).  pairs: scratch of 3 * n int32. */
 int kv_page_fork_launch(const struct kv_page_cache *cache, const struct kv_page_state *state,
                         const int32_t *parents, const int32_t *children, uint32_t n, int32_t *pairs,
                         int32_t *status, void *stream);

@@ -59,7 +59,10 @@ class Pages:
             for k in range(need):
                 p = self.free.pop()
                 self.table[r, old + k] = p
-                self.refs[p] = 1
+                if 0 <= p < self.pages:
+                    self.refs[p] = 1
+                else:                       # the free list was wrong: the row has it as it stands
+                    self.error |= ERR_PAGE
             self.lens[r] = x
             status.append(OK)
         return status
@@ -83,10 +86,19 @@ class Pages:
                 self.error |= ERR_ROW
                 status.append(INVALID)
                 continue
+            if any(not 0 <= page < self.pages for page in self.table[p, :self._npages(self.lens[p])]):
+                self.error |= ERR_PAGE
+                status.append(INVALID)
+                continue
             full, tail = divmod(int(self.lens[p]), self.block)
             asked += tail > 0
             if tail and asked > have:
                 status.append(NO_PAGES)
+                continue
+            if tail and not 0 <= self.free[-1] < self.pages:
+                self.free.pop()
+                self.error |= ERR_PAGE
+                status.append(INVALID)
                 continue
             self.table[c, :full] = self.table[p, :full]
             for page in self.table[p, :full]:

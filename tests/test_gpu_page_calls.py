@@ -202,3 +202,65 @@ def test_a_pool_of_free_pages_refuses_rows_that_hold_some():
     assert pool.resize(ints([1]), ints([0])).tolist() == [pg.OK]
     pool.check()
     assert pool.free_list.tolist() == [7, 6, 5, 2, 1, 0, 3, 4]
+
+
+def held_and_free(c):
+    """every page that a row holds, or that is free, once per holder"""
+    m = c.model
+    held = [int(p) for r in range(m.rows) for p in m.table[r, :m._npages(m.lens[r])] if 0 <= p < m.pages]
+    assert not set(held) & set(m.free) and [held.count(p) for p in range(m.pages)] == m.refs.tolist()
+
+
+@pytest.mark.parametrize("where", ["full", "tail", "last_full"])
+@pytest.mark.parametrize("page", [-1, 60, 2 ** 31 - 1])
+def test_children_of_a_row_with_a_bad_page_stay_empty(where, page):
+    """the other children get their pages as if it had not been named"""
+    c = Case(GEOMETRIES["mixed"], 60, 12, 6)
+    resize(c, [0, 1, 2], [8 * 4 + 3, 8 * 5, 8 * 2 + 7])
+    r, k = {"full": (0, 1), "tail": (0, 4), "last_full": (1, 4)}[where]
+    was = int(c.model.table[r, k])
+    c.pool.block_table[r, k] = page
+    c.model.table[r, k] = page
+    fork(c, [2, 0, 1, 2, 0, 1], [3, 4, 5, 6, 7, 8])
+    c.same(pm.ERR_PAGE)
+    c.model.table[r, k] = was
+    held_and_free(c)
+    assert (c.model.lens[[4, 7]] == 0).all() == (r == 0) and (c.model.lens[[5, 8]] == 0).all() == (r == 1)
+
+
+def test_many_children_of_rows_with_bad_pages():
+    """more children than the plan has warps"""
+    c = Case(("nhd", 1, 1, 8, torch.int16, 16), 4000, 700, 40)
+    rng = np.random.default_rng(4)
+    resize(c, list(range(20)), rng.integers(1, 40 * 16, 20).tolist())
+    was = c.model.table.copy()
+    for r in (3, 11, 12):
+        k = int(rng.integers(0, -(-int(c.model.lens[r]) // 16)))
+        c.pool.block_table[r, k] = -5
+        c.model.table[r, k] = -5
+    fork(c, rng.integers(0, 20, 680).tolist(), rng.permutation(np.arange(20, 700)).tolist())
+    c.same(pm.ERR_PAGE)
+    c.model.table[:20] = was[:20]
+    held_and_free(c)
+
+
+def test_ids_of_the_free_list_that_are_no_pages():
+    """fork refuses the child, resize hands them out as they stand"""
+    c = Case(GEOMETRIES["mixed"], 60, 12, 6)
+    resize(c, [0], [8 * 2 + 3])
+    for at, bad in ((-2, 99), (-5, -1)):
+        c.model.free[at] = bad
+        c.pool.free_list[int(c.pool.free_count) + at] = bad
+    fork(c, [0, 0, 0], [1, 2, 3])
+    c.same(pm.ERR_PAGE)
+    held_and_free(c)
+    assert c.model.lens[:4].tolist() == [19, 19, 0, 19]
+    c.model.error = 0
+    with pytest.raises(ValueError, match="page id"):
+        c.pool.check()
+    resize(c, [4, 5], [8, 17])
+    c.same(pm.ERR_PAGE)
+    assert c.model.table[5, 0] == -1
+    resize(c, [4, 5], [0, 0])
+    c.same(pm.ERR_PAGE)
+    held_and_free(c)
