@@ -630,11 +630,15 @@ bool state_ok(const kv_page_state *s)
            s->block_size && s->block_size <= INT32_MAX;
 }
 
+__device__ __forceinline__ uint8_t *base_of(const Planes &p, uint32_t lk)
+{
+    return reinterpret_cast<uint8_t *>((p.kvs == 2 && (lk & 1) ? p.layer_v : p.layer_k)[p.kvs == 2 ? lk >> 1 : lk]);
+}
+
 template <int VEC>
 __device__ __forceinline__ uint8_t *plane(const Planes &p, uint32_t lk)
 {
-    const uint32_t l = p.kvs == 2 ? lk >> 1 : lk;
-    uint8_t *base = reinterpret_cast<uint8_t *>((p.kvs == 2 && (lk & 1) ? p.layer_v : p.layer_k)[l]);
+    uint8_t *base = base_of(p, lk);
     if (!base || reinterpret_cast<uintptr_t>(base) % VEC) {
         atomicOr(p.error, KVPAGE_ERR_ALIGN);
         return nullptr;
@@ -758,8 +762,9 @@ __global__ void __launch_bounds__(kMoveThreads, 8) kv_page_copy_warp_kernel(cons
  * slice: some bytes of each token) and walks their tokens in order: load a
  * batch into registers, barrier, store it.  Slices are independent.
  *
- * Every CTA checks its row's whole list before it moves a byte, so that all
- * of them decide alike; 4 bytes of list against 64 bytes or more of slice.
+ * Every CTA checks its row's whole list and every plane's base before it moves a
+ * byte, so that all of them decide alike; 4 bytes of list against 64 bytes or
+ * more of slice.
  * The first CTA of a row leaves the new length for resize, or kRefused.
  * Half of 16000 tokens of 64 planes of 2 KiB units: 305 us, 5.2 TB/s; up to 5 of
  * 24 tokens of 64 rows: 17 us, most of it the checks' dependent loads.
@@ -792,6 +797,9 @@ kv_page_compact_kernel(const Planes p, const kv_page_state s, const int32_t *__r
     for (uint32_t k = threadIdx.x; k < n; k += kMoveThreads)
         if (k != i && rows[k] == r)
             bad = KVPAGE_ERR_ROW;
+    for (uint32_t lk = threadIdx.x; lk < p.layers * p.kvs; lk += kMoveThreads)
+        if (!plane<VEC>(p, lk))
+            bad |= KVPAGE_ERR_ALIGN;
     int32_t len = 0;
     if (r < 0 || (uint32_t)r >= s.num_rows) {
         bad = KVPAGE_ERR_ROW;
@@ -873,14 +881,12 @@ kv_page_compact_kernel(const Planes p, const kv_page_state s, const int32_t *__r
                 to[u] = nullptr;
                 if (tok_row < per_pass && j < tokens && g < group && q + g < q1) {
                     const uint32_t lk = (q + g) / slices_per_plane, sl = q + g - lk * slices_per_plane;
-                    uint8_t *base = plane<VEC>(p, lk);
+                    uint8_t *base = base_of(p, lk);
                     const uint32_t o = (sl * slice_vecs + vec) * VEC;
                     /* byte o of a token's unit: a head-major page holds head o / head_bytes apart */
                     const uint64_t at = p.head_bytes ? (uint64_t)(o / p.head_bytes) * p.bs * p.head_bytes + o % p.head_bytes : o;
-                    if (base) {
-                        v[u] = *reinterpret_cast<const T *>(base + src_off[j] + at);
-                        to[u] = reinterpret_cast<T *>(base + dst_off[j] + at);
-                    }
+                    v[u] = *reinterpret_cast<const T *>(base + src_off[j] + at);
+                    to[u] = reinterpret_cast<T *>(base + dst_off[j] + at);
                 }
             }
             __syncthreads();

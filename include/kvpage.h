@@ -42,7 +42,7 @@ extern "C" {
 #define KVPAGE_ERR_REFS   0x4   /* a page given back by a row that no longer held it; compact: a token to be moved
                                  * into a page that another row holds too */
 #define KVPAGE_ERR_KEEP   0x8   /* compact: kept tokens not strictly ascending within [start, length) */
-#define KVPAGE_ERR_ALIGN  0x10  /* a null or misaligned layer base */
+#define KVPAGE_ERR_ALIGN  0x10  /* a null or misaligned layer base: copies leave that plane out, compact refuses its rows */
 
 /* a row's result in status[] */
 #define KVPAGE_OK         0

@@ -264,3 +264,22 @@ def test_ids_of_the_free_list_that_are_no_pages():
     resize(c, [4, 5], [0, 0])
     c.same(pm.ERR_PAGE)
     held_and_free(c)
+
+
+@pytest.mark.parametrize("base", ["null", "misaligned"])
+def test_compact_with_a_bad_base_leaves_its_rows_alone(base):
+    """the bytes that could not be moved in one plane are not given up in the others"""
+    c = Case(GEOMETRIES["mixed"], 40, 4, 6)
+    resize(c, [0, 1], [20, 30])
+    k = c.pool._k.clone()
+    c.pool._k[1] = 0 if base == "null" else int(k[1]) + 8
+    got = c.pool.compact(ints([0, 1]), ints([3, 0]), ints([9, 17, 2]), ints([0, 2, 3]))
+    assert got.tolist() == [pg.INVALID] * 2
+    c.model.error = 16
+    c.same(16)
+    with pytest.raises(ValueError, match="layer base"):
+        c.pool.check()
+    c.model.error = 0
+    c.pool._k.copy_(k)
+    compact(c, [0, 1], [3, 0], [[9, 17], [2]])
+    c.same()
