@@ -299,6 +299,7 @@ SIGNATURES: dict[str, tuple] = {
     # include/kvattn.h
     "kv_attn_workspace_bytes": (C.c_int64, [C.c_void_p]),
     "kv_attn_launch": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "kv_attn_launch_stalled": (C.c_int, [C.c_void_p, C.c_void_p]),
     # include/kvhash.h
     "kv_block_hash_launch": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),

@@ -80,7 +80,7 @@ constexpr int kPieceCost = 3;
 constexpr int kPlanned = 4;         /* pieces that the planning warp is ahead */
 constexpr int kJoinThreads = 256;
 constexpr int kMaxCtas = 512;       /* of the first kernel */
-constexpr uint32_t kSpinLimit = 1u << 20;
+constexpr uint32_t kSpinLimit = 1u << 20, kStallLimit = 1u << 14;   /* polls of a wait; of one that a test lets run out */
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 /* DP: head_dim rounded up to whole columns.  K of the next tile is used a
@@ -117,6 +117,7 @@ struct Params {
     uint32_t box;
     uint32_t min_share;     /* tiles that a CTA takes at least */
     uint32_t wide_out;      /* rows of out start on 32 bytes */
+    uint32_t stall;         /* kv_attn_launch_stalled */
     Job *jobs;              /* workspace: [CTAs] row tiles to be joined, by the CTA that has their first tiles */
     float *part_ml;         /* [2 * CTAs][128][2] maximum and sum of a piece */
     float *part_o;          /* [2 * CTAs][128][dim] */
@@ -269,9 +270,12 @@ struct Shared {
     uint64_t s_full[2], p_full[2];  /* of tiles in turn */
     uint64_t o_done[2], o_free;     /* O of a tile is complete; O of a piece has been read */
     uint64_t q_full, q_empty;
+    uint64_t settled;               /* every product has been computed */
     uint64_t planned[kPlanned], taken[kPlanned];
     Piece pieces[kPlanned];         /* one without tiles ends the work */
     uint32_t tmem;
+    uint32_t limit;                 /* polls of a wait */
+    uint32_t end_at[2], end_parity[2], end_q;   /* where the loaders of K, V and Q stopped */
     volatile uint32_t dead;         /* a wait ran out: every role leaves */
     volatile uint32_t spoilt[4];    /* [piece % 4] == piece + 1: values of its fed nodes that are not finite were set aside */
     int64_t share, scan[Roles<kWiden>::kThreads / 32];
@@ -289,7 +293,7 @@ __device__ __noinline__ bool wait_long(Shared &sh, int32_t *error, uint32_t bar,
     for (uint32_t i = 0; !mbar_try_wait(bar, parity); i++) {
         if (sh.dead)
             return false;
-        if (i >= kSpinLimit) {
+        if (i >= sh.limit) {
             sh.dead = 1;
             atomicOr(error, KVATTN_ERR_TIMEOUT);
             return false;
@@ -303,6 +307,14 @@ __device__ __noinline__ bool wait_long(Shared &sh, int32_t *error, uint32_t bar,
 __device__ __forceinline__ bool wait(Shared &sh, int32_t *error, uint32_t bar, uint32_t parity)
 {
     return mbar_try_wait(bar, parity) || wait_long(sh, error, bar, parity);
+}
+
+/* the same for what is in flight after a wait ran out, whatever comes of it */
+__device__ void settle(const Shared &sh, uint32_t bar, uint32_t parity)
+{
+    for (uint32_t i = 0; i < sh.limit && !mbar_try_wait(bar, parity); i++)
+        if (i > 64)
+            __nanosleep(32);
 }
 
 /* the same for a whole warp, whose lanes go on together or not at all */
@@ -592,6 +604,10 @@ template <typename T, Load L, int DP> struct Loader {
         const uint32_t bars = uniform(smem_u32(v ? sh.v_full : sh.k_full)), frees = uniform(smem_u32(v ? sh.v_empty : sh.k_empty));
         const CUtensorMap *map = v ? &p.v_map : &p.k_map;
         uint32_t at = 0, parity = 1;
+        auto stop = [&] {                   /* for land() */
+            if (lane == 0)
+                sh.end_at[v] = at, sh.end_parity[v] = parity;
+        };
         Piece e;
         for (uint32_t piece = 0; take(p, sh, piece, e); piece++) {
             const int32_t *tab = p.d.table + (int64_t)e.row * p.d.table_stride;
@@ -610,7 +626,7 @@ template <typename T, Load L, int DP> struct Loader {
                 if (left > 1)
                     next = lane < boxes && pos < end ? tab[fdiv(pos, p.block)] : 0;     /* in flight while the tile is loaded */
                 if (!wait_warp(sh, p.d.error, frees + at * 8, parity))
-                    return;
+                    return stop();
                 const uint32_t bar = bars + at * 8;
                 uint32_t to = base + at * S::kSlotBytes;
                 if (elect())
@@ -630,6 +646,15 @@ template <typename T, Load L, int DP> struct Loader {
                 }
             }
         }
+        stop();
+    }
+
+    /* after a wait ran out: the last load of each slot, of the lap that run_tma
+     * ended in, of the one before, or none (a phase that counts as over) */
+    static __device__ void land(Shared &sh, bool v)
+    {
+        for (uint32_t k = 0; k < (v ? S::kSlotsV : S::kSlotsK); k++)
+            settle(sh, smem_u32(v ? &sh.v_full[k] : &sh.k_full[k]), k < sh.end_at[v] ? sh.end_parity[v] ^ 1 : sh.end_parity[v]);
     }
 
     /* ---- 16 bytes at a time: pages of any size ---- */
@@ -788,6 +813,7 @@ __device__ __forceinline__ void load_q(const Params &p, Shared &sh, uint8_t *q_s
     if (elect()) {
         const uint32_t bar = smem_u32(&sh.q_full);
         mbar_expect(bar, p.columns * p.nodes.d * p.group * (kColumn * 2));
+        sh.end_q++;
         for (uint32_t c = 0; c < p.columns; c++)    /* rows behind the sequence's are another's, and not used */
             tma_load(smem_u32(q_smem) + c * (kRows * kColumn * 2), &p.q_map, c * kColumn, head, q, bar);
     }
@@ -1254,12 +1280,14 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
+        const bool stall = p.stall && blockIdx.x == 0;
+        sh.limit = stall ? kStallLimit : kSpinLimit;
         for (int k = 0; k < S::kSlotsK; k++) {
             mbar_init(&sh.k_full[k], Roles<L>::kFill);
             mbar_init(&sh.k_empty[k], 1);
         }
         for (int k = 0; k < S::kSlotsV; k++) {
-            mbar_init(&sh.v_full[k], Roles<L>::kFill);
+            mbar_init(&sh.v_full[k], Roles<L>::kFill + (stall && k == 0));     /* one arrival that nobody makes */
             mbar_init(&sh.v_empty[k], 1);
         }
         for (int k = 0; k < 2; k++) {
@@ -1274,8 +1302,10 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
         mbar_init(&sh.o_free, kSoftmax / 32);
         mbar_init(&sh.q_full, 1);
         mbar_init(&sh.q_empty, 1);
+        mbar_init(&sh.settled, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.dead = 0;
+        sh.end_q = 0;
         for (int k = 0; k < 4; k++)
             sh.spoilt[k] = 0;
     }
@@ -1311,11 +1341,24 @@ __global__ void __launch_bounds__(Roles<L>::kThreads, Shape<L, DP>::kCtas) kv_at
     } else if (threadIdx.x == 0) {
         atomicOr(p.d.error, KVATTN_ERR_TIMEOUT);
     }
-    if (sh.dead)
-        for (int k = 0; k < 1000; k++)          /* what is in flight lands before the CTA leaves */
-            __nanosleep(1000);
     tmem_fence_before();
     __syncthreads();
+    if (sh.dead) {
+        /* shared memory and TMEM are given up when the copies have landed and the products are done */
+        if (warp == kThreads / 32 - 2) {
+            if (elect())
+                mma_commit(&sh.settled);
+            __syncwarp();
+            settle(sh, smem_u32(&sh.settled), 0);
+            if (sh.end_q)
+                settle(sh, smem_u32(&sh.q_full), (sh.end_q - 1) & 1);
+        } else if (L == kTma && (warp == kSoftmax / 32 || warp == kSoftmax / 32 + 1)) {
+            Loader<T, L, DP>::land(sh, warp != kSoftmax / 32);
+        }
+        for (int k = 0; L != kTma && k < 100; k++)
+            __nanosleep(1000);                  /* the arrivals of 16-byte copies, which come behind the copies */
+        __syncthreads();
+    }
     tmem_fence_after();
     if (warp == kThreads / 32 - 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "n"(S::kTmem) : "memory");
@@ -1688,7 +1731,7 @@ extern "C" int64_t kv_attn_workspace_bytes(const struct kv_attn_desc *d)
     return (int64_t)workspace(d).bytes;
 }
 
-extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
+static int attn_launch(const struct kv_attn_desc *d, uint32_t stall, void *stream)
 {
     if (!desc_ok(d))
         return -EINVAL;
@@ -1709,6 +1752,7 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
         return -EINVAL;
     Params p{};
     p.d = *d;
+    p.stall = stall;
     p.stride = d->block_stride ? d->block_stride
                                : (uint64_t)d->block_size * d->num_kv_heads * d->head_dim * (d->kv_type == KVATTN_E4M3 ? 1 : 2);
     p.group = d->num_heads / d->num_kv_heads;
@@ -1729,3 +1773,7 @@ extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream)
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return d->q_type == KVATTN_BF16 ? launch_load<__nv_bfloat16>(p, st) : launch_load<__half>(p, st);
 }
+
+extern "C" int kv_attn_launch(const struct kv_attn_desc *d, void *stream) { return attn_launch(d, 0, stream); }
+
+extern "C" int kv_attn_launch_stalled(const struct kv_attn_desc *d, void *stream) { return attn_launch(d, 1, stream); }

@@ -93,6 +93,12 @@ int64_t kv_attn_workspace_bytes(const struct kv_attn_desc *desc);
  * KVATTN_MAX_QUERIES, or -EIO when the launch failed. */
 int kv_attn_launch(const struct kv_attn_desc *desc, void *stream);
 
+/* For tests of the failure detection: the same, but in the grid's first CTA
+ * (where it has work) the first tile of V counts as never loaded.  The waits for
+ * it run out after some milliseconds, KVATTN_ERR_TIMEOUT is set, and what is
+ * in flight settles before the CTA leaves.  The results are void. */
+int kv_attn_launch_stalled(const struct kv_attn_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
