@@ -80,7 +80,9 @@ constexpr int kPieceCost = 3;
 constexpr int kPlanned = 4;         /* pieces that the planning warp is ahead */
 constexpr int kJoinThreads = 256;
 constexpr int kMaxCtas = 512;       /* of the first kernel */
-constexpr uint32_t kSpinLimit = 1u << 20, kStallLimit = 1u << 14;   /* polls of a wait; of one that a test lets run out */
+/* polls of a wait, at 4 us each (the hardware waits before it answers): about a
+ * second; of one that a test lets run out */
+constexpr uint32_t kSpinLimit = 1u << 18, kStallLimit = 1u << 12;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 /* DP: head_dim rounded up to whole columns.  K of the next tile is used a
@@ -341,6 +343,22 @@ __device__ __forceinline__ bool take(const Params &p, Shared &sh, uint32_t piece
     return e.t1 > e.t0;
 }
 
+/* The planning warp waits for whole pieces, which take as long as their context
+ * is: a minute at most.  Where another role's wait runs out it leaves with it. */
+__device__ __noinline__ bool wait_taken(Shared &sh, int32_t *error, uint32_t bar, uint32_t parity)
+{
+    for (uint32_t i = 0; !mbar_try_wait(bar, parity); i++) {
+        if (sh.dead)
+            return false;
+        if (i >= 64 * sh.limit) {
+            sh.dead = 1;
+            atomicOr(error, KVATTN_ERR_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+
 /* the planning warp: finding a piece is a chain of loads and divisions, which
  * the others would wait for (7000 cycles a piece when each did it itself) */
 __device__ __forceinline__ void plan(const Params &p, Shared &sh, Line line)
@@ -351,7 +369,8 @@ __device__ __forceinline__ void plan(const Params &p, Shared &sh, Line line)
         more = line.next(p, sh.share, e);
         if (!more)
             e.t0 = e.t1 = 0;
-        if (!wait_warp(sh, p.d.error, &sh.taken[k], piece / kPlanned & 1 ^ 1))
+        const uint32_t bar = smem_u32(&sh.taken[k]), parity = piece / kPlanned & 1 ^ 1;
+        if (!__all_sync(~0u, mbar_try_wait(bar, parity) || wait_taken(sh, p.d.error, bar, parity)))
             return;
         if (threadIdx.x % 32 == 0) {
             sh.pieces[k] = e;

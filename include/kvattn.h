@@ -41,7 +41,7 @@ extern "C" {
 #define KVATTN_ERR_SEQ     0x2   /* a row or length that fits neither table nor nodes: the sequence's rows are
                                   * 0 / -inf; or offsets out of order or past total_q: the sequence is skipped */
 #define KVATTN_ERR_PARENT  0x4   /* a parent outside [-2, j - 1]: the node is taken for a padding node */
-#define KVATTN_ERR_TIMEOUT 0x8   /* a wait inside the kernel ran out: the results are void */
+#define KVATTN_ERR_TIMEOUT 0x8   /* a wait inside the kernel ran out, after about a second: the results are void */
 
 #define KVATTN_BF16 0
 #define KVATTN_FP16 1
@@ -95,7 +95,7 @@ int kv_attn_launch(const struct kv_attn_desc *desc, void *stream);
 
 /* For tests of the failure detection: the same, but in the grid's first CTA
  * (where it has work) the first tile of V counts as never loaded.  The waits for
- * it run out after some milliseconds, KVATTN_ERR_TIMEOUT is set, and what is
+ * it run out after some 20 milliseconds, KVATTN_ERR_TIMEOUT is set, and what is
  * in flight settles before the CTA leaves.  The results are void. */
 int kv_attn_launch_stalled(const struct kv_attn_desc *desc, void *stream);
 
