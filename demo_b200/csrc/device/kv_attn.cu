@@ -1149,7 +1149,8 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
         const bool whole = e.whole();
         const float from = (m == -INFINITY ? 0.f : m) - Type<T>::kBias;
         const uint32_t slot = 2 * blockIdx.x + (piece ? 1 : 0);
-        const float inv = !active || l == 0 ? 0.f : whole ? d.v_scale / l : 1.f;
+        const bool something = active && l != 0;        /* else 0, also where O is not finite: 0 * V of a weight of 0 */
+        const float inv = !something ? 0.f : whole ? d.v_scale / l : 1.f;
         const bool spoilt = __any_sync(~0u, sh.spoilt[piece % 4] == piece + 1);
         if (__any_sync(~0u, valid)) {
             if (spoilt)
@@ -1164,7 +1165,7 @@ __device__ void softmax(const Params &p, Shared &sh, uint8_t *ring)
                 if (whole && valid) {
 #pragma unroll
                     for (int k = 0; k < 8; k++)
-                        w[k] = active ? Type<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0;
+                        w[k] = something ? Type<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0;
                     if (p.wide_out) {
                         store32(out + c, w);
                     } else {

@@ -10,6 +10,7 @@ from demo_b200 import cache as cc
 from demo_b200 import pages as pg
 from demo_b200._lib import KVPAGE_ANY_DEVICE, lib
 from demo_b200.attention import TreeAttention
+from oracle import attention as oa
 from oracle import pages_model as pm
 from tests.test_gpu_attention import Batch, close
 from tests.test_gpu_pages import GEOMETRIES, Case, compact, fork, ints, resize
@@ -283,3 +284,19 @@ def test_compact_with_a_bad_base_leaves_its_rows_alone(base):
     c.pool._k.copy_(k)
     compact(c, [0, 1], [3, 0], [[9, 17], [2]])
     c.same()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=str)
+@pytest.mark.parametrize("n", [40, 6000])
+def test_scores_of_minus_infinity_over_values_that_are_not_finite(n, value):
+    """are nothing seen all the same: 0 with lse -inf, joined from pieces or not"""
+    b = Batch([n, 30], [1, 1], heads=2, kv_heads=1, dim=64, seed=33)
+    b.q[0] = 1
+    held = torch.tensor(b.table[0, :-(-n // 16)].astype(np.int64)).cuda()
+    b.view[0, 0, held] = -float("inf")
+    b.view[0, 1, held] = value
+    args, _ = b.args()
+    out, lse = b.attention()(*args, return_lse=True)
+    assert not out[0].any() and (lse[0] == -float("inf")).all()
+    want = oa.attention(b.q[1:], *(b.view[0, i].double() for i in range(2)), b.table.tolist(), b.lens, [0, 1], rows=[1])
+    close(out[1:], lse[1:], want)
