@@ -20,11 +20,12 @@
  * next tile is computed under the softmax of this one.
  *
  * On a B200, 32 heads over 8 K/V heads of dim 128: one token over 2048 positions
- * takes 15.5 us (launch, line, one tile, join: latencies); 64 trees of 9 to 32
- * nodes over up to 2048 positions 83 us (361 MB, 4.3 TB/s); 32 chains of 4 nodes
- * over up to 8192 positions of e4m3 141 us (402 MB, 2.9 TB/s: the widening);
- * 8 heads over one: 8 trees of 64 nodes over up to 131072 positions 180 us (172
- * GFLOP, 0.96 PFLOP/s: the chain of products and exponentials).
+ * takes 15.5 us (launch, line, one tile, join: latencies); a batch of 64 trees of
+ * 9 to 32 nodes over 500 to 2048 positions with 344 MB of K and V 86 us (4.0 TB/s);
+ * one of 32 chains of 4 nodes over 4000 to 8192 positions of e4m3 with 394 MB
+ * 149 us (2.6 TB/s: the widening); 8 heads over one: a batch of 8 trees of 64
+ * nodes over 32768 to 131072 positions with 173 GFLOP 210 us (0.82 PFLOP/s: the
+ * chain of products and exponentials).
  *
  * Warps 0-3 are the softmax (a thread owns a TMEM lane, a row), then come the
  * loaders, a warp that issues the products, and one that finds the next pieces
@@ -495,7 +496,9 @@ template <> struct Type<__nv_bfloat16> {
         __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<uint32_t *>(&v);
     }
-    static __device__ uint32_t widen(uint16_t two)      /* two e4m3 values, exactly */
+    /* two e4m3 values, exactly: four conversions (there is none from 8 bits to
+     * bf16, so by way of fp16 and 32 bits), where fp16 takes one */
+    static __device__ uint32_t widen(uint16_t two)
     {
         const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3));
         const float2 f = __half22float2(h);
@@ -916,7 +919,10 @@ __device__ void products(const Params &p, Shared &sh, uint8_t *q_smem, uint8_t *
 /* ------------------------------------------------------------------------
  * softmax: thread = row.  m lags behind the true maximum by up to kLazy (in
  * powers of two), so that O, which lives in TMEM, is rescaled rarely; the
- * result is the same quotient.
+ * result is the same quotient.  The weights are rounded to the 16-bit type of
+ * the products (half a step, 2^-8 of a weight in bf16, 2^-11 in fp16), which is
+ * what the tensor cores take; their sum is that of the unrounded ones, and m, l
+ * and O are held in 32 bits.
  * ---------------------------------------------------------------------- */
 /* The positions p0 .. p0 + 64 that a node sees, a bit each.  j is the node, or
  * in a tree the nearest of its line (the node itself, its ancestors) that stands

@@ -19,12 +19,16 @@
  *   free_count [1]
  * The state's calls are made on one stream, or ordered by the caller; they
  * allocate nothing, do not synchronise, and may be captured into a graph.
- * Their results do not depend on the order in which threads run.  What a call
- * is given is read before the state is written: it may be part of the state.
+ * Their results do not depend on the order in which threads run, but for the
+ * place in the free list of a page that a call gives back too often
+ * (KVPAGE_ERR_REFS).  What a call is given is read before the state is written:
+ * it may be part of the state.
  *
  * The launch functions return 0, -EINVAL for a malformed argument, -E2BIG
  * past a limit below, -EIO when the launch failed.  What only the device can
- * see sets bits in *error and is left alone; the rest of the call is done.
+ * see sets bits in *error and is left alone, the rest of the call is done:
+ * rows with status KVPAGE_INVALID are as they were, and where a call does
+ * anything else with what is wrong, it says so below.
  */
 #ifndef __KVPAGE_H__
 #define __KVPAGE_H__
