@@ -31,7 +31,9 @@ def attention(q, k_pages, v_pages, table, lens, q_offsets, parents=None, rows=No
     2^-23 |s| + 2^-21: d in all, relative to a weight.  Each weight is rounded
     (u), the two sums over n positions lose n 2^-24 each, the result is
     rounded (u |out|).  With A the weighted mean of |v|:
-    out_tol = u |out| + (u + 2 d + 2 n 2^-24) A,  lse_tol = 2 d + n 2^-24 + 2^-22 |lse|.
+    out_tol = u |out| + t + (u + 2 d + 2 n 2^-24) A,  lse_tol = 2 d + n 2^-24 + 2^-22 |lse|,
+    where t = u times the smallest normal number of q's type: below it the
+    type's steps no longer shrink with the value (fp16: 2^-24, half a step 2^-25).
     """
     u = torch.finfo(q.dtype).eps / 2
     total, heads, dim = q.shape
@@ -69,6 +71,6 @@ def attention(q, k_pages, v_pages, table, lens, q_offsets, parents=None, rows=No
                 a = (w / z) @ vv.abs()
                 sl = slice(h * group, (h + 1) * group)
                 out[first + j, sl], lse[first + j, sl] = o, (m + z.log())[:, 0]
-                out_tol[first + j, sl] = u * o.abs() + (u + 2 * d + 2 * len(at) * 2.0 ** -24) * a
+                out_tol[first + j, sl] = u * o.abs() + u * torch.finfo(q.dtype).smallest_normal + (u + 2 * d + 2 * len(at) * 2.0 ** -24) * a
                 lse_tol[first + j, sl] = 2 * d[:, 0] + len(at) * 2.0 ** -24 + 2.0 ** -22 * lse[first + j, sl].abs()
     return out, lse, out_tol, lse_tol

@@ -251,3 +251,13 @@ def test_gradients_of_every_kind_and_traces_are_refused():
         torch.jit.trace(call, (q,))
     with torch.no_grad(), pytest.raises(ValueError, match="q: expected"):
         call(q.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("dtype, half_step", [(torch.float16, 2.0 ** -25), (torch.bfloat16, 2.0 ** -134)], ids=str)
+def test_the_bound_of_results_below_the_normal_range(dtype, half_step):
+    """a result that is exact in 64 bits and halfway between two numbers of the type"""
+    q = torch.zeros(1, 1, 16, dtype=dtype)
+    v = torch.full((1, 1, 1, 16), 3 * half_step, dtype=torch.float64)
+    out, _, tol, _ = oa.attention(q, torch.zeros(1, 1, 1, 16, dtype=torch.float64), v, [[0]], [1], [0, 1])
+    off = (out.to(dtype).double() - out).abs()
+    assert (off == half_step).all() and (off <= tol).all()
