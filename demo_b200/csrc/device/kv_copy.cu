@@ -303,8 +303,8 @@ constexpr int kBulkStages = KVCOPY_BULK_STAGES;
 static_assert(kBulkStages >= 2 && (uint64_t)kBulkStages * kBulkTileBytes <= 227u * 1024u - 256u,
               "bulk ring must fit the 227 KiB of shared memory a CTA can have");
 static_assert(kBulkTileBytes % 16 == 0, "bulk copies move multiples of 16 bytes");
-constexpr uint32_t kBulkSpinLimit = 1u << 24;   /* polls of ~128 ns back-off: ~2 s */
-constexpr uint32_t kStallSpinLimit = 1u << 14;  /* fault-detection test: a few ms */
+constexpr uint32_t kBulkSpinLimit = 1u << 18;   /* polls, which the hardware holds for 4 us each: ~1 s */
+constexpr uint32_t kStallSpinLimit = kBulkSpinLimit / 64;   /* fault-detection test: ~16 ms */
 
 struct BulkParams {
     const uint64_t *layer_k;

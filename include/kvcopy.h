@@ -49,7 +49,7 @@ extern "C" {
 #define KVCOPY_FLAG_TEST_STALL  0x100 /* fault-detection tests only, bulk path:
                                        * CTA 0 arms its first stage's mbarrier
                                        * for 16 bytes it never copies, so that
-                                       * wait runs out after a few ms (no copy
+                                       * wait runs out after ~16 ms (no copy
                                        * is in flight on that stage); the
                                        * kernel sets KVCOPY_ERR_TIMEOUT, drains
                                        * its other loads and returns.  The

@@ -125,3 +125,16 @@ def test_stall_flag_is_ignored_by_the_register_path_and_unknown_flags_are_reject
     d.flags = 0x40
     assert lib.kv_copy_launch(C.byref(d), None) == -errno.EINVAL
     assert lib.kv_copy_path(C.byref(d)) == -errno.EINVAL
+
+
+def test_a_wait_that_runs_out_takes_about_a_second():
+    """the test's limit is a 64th of the ordinary one: the wait and the drain
+    behind it, both to the end of it, take about 33 ms, the ordinary ones 2 s"""
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kv = DeviceKV(CASE)
+    recs = [torch.zeros(gen.record_bytes(CASE), dtype=torch.uint8, device="cuda") for _ in range(CASE["chunks"])]
+    bids = to_dev(gen.block_ids(CASE).astype(np.int64))
+    d = _desc(kv.kp, kv.vp, recs, bids, err, 1, KVCOPY_FLAG_BULK | KVCOPY_FLAG_TEST_STALL)
+    runs = [_run(d, err) for _ in range(3)]
+    assert all(ret == 0 and bits == KVCOPY_ERR_TIMEOUT for ret, bits, _ in runs), runs
+    assert min(secs for _, _, secs in runs) < 0.1, runs
