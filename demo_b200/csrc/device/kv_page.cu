@@ -649,7 +649,7 @@ __device__ __forceinline__ uint8_t *plane(const Planes &p, uint32_t lk)
 /* ------------------------------------------------------------------------
  * copy.  A page in a plane is one run of vectors in every geometry.  Where a run
  * fills CTAs of 2048 vectors, a CTA moves that much of one run: four pages of 64
- * planes of 32 KiB take 3.4 us, 500 of 27 planes of 72 KiB 297 us (6.7 TB/s).
+ * planes of 32 KiB take 3.6 us, 500 of 27 planes of 72 KiB 297 us (6.7 TB/s).
  * Shorter runs (4 KiB: one head, 16 tokens) go to a warp each, which finds its
  * page, plane and tokens once: 256 pages of 160 such planes take 53 us (6.3
  * TB/s), the first half of them 28; with a CTA per run the half took 95, with

@@ -40,7 +40,7 @@ extern "C" {
 #define KVATTN_ERR_PAGE    0x1   /* a page id outside [0, num_pages); it counts as zeros */
 #define KVATTN_ERR_SEQ     0x2   /* a row or length that fits neither table nor nodes: the sequence's rows are
                                   * 0 / -inf; or offsets out of order or past total_q: the sequence is skipped
-                                  * (queries that two others then both cover get the result of one of them) */
+                                  * (the results of queries that two others then both cover are unspecified) */
 #define KVATTN_ERR_PARENT  0x4   /* a parent outside [-2, j - 1]: the node is taken for a padding node */
 #define KVATTN_ERR_TIMEOUT 0x8   /* a wait inside the kernel ran out, after about a second: the results are void */
 
