@@ -117,9 +117,9 @@ class TreeAttention:
         rows         int32 [sequences]: their rows; None: row b
 
         Runs on `stream`, by default the current stream of q's device, to which
-        the results then belong.  The arguments may be dropped when the call
-        returns; the object must outlive its calls, and the graphs that captured
-        them.  Queries that no sequence covers leave their rows of out and lse as
+        the results then belong.  With `stream` the arguments may be dropped when
+        the call returns (on the current stream torch's own rules hold); the
+        object must outlive its calls, and the graphs that captured them.  Queries that no sequence covers leave their rows of out and lse as
         they were, which in new tensors is anything.  May be
         captured, except for the first call of an object that was made before
         CUDA was used.

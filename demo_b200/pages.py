@@ -105,10 +105,11 @@ class PagePool:
     kernels.  Calls run on `stream`, by default the current stream of the
     cache's device, in the order they are made; calls for one pool on several
     streams have to be ordered by the caller, and results belong to the stream
-    of their call.  A call's arguments may be dropped when it returns; the pool
-    itself must outlive its calls, and the graphs that captured them.  The int32
-    results of resize, fork and compact say per row pages.OK, NO_PAGES or
-    INVALID, on the device.
+    of their call.  The arguments of a call with `stream` may be dropped when it
+    returns (on the current stream torch's own rules hold); the pool itself must
+    outlive its calls, and the graphs that captured them.  The int32 results of
+    resize, fork and compact say per row pages.OK, NO_PAGES or INVALID, on the
+    device.
     """
 
     def __init__(self, layout: KVLayout, k_ptrs: Sequence[int], v_ptrs: Sequence[int] | None,
